@@ -1,0 +1,537 @@
+// Attention over 8-bit caches and shared prefixes: the kernels that take every head size, page size and type, the kernel that joins
+// the parts of a unit, and the entry points, which choose between these and the tensor-core kernels.
+//
+// attention_rows_any_kernel: tiles of query rows (attention_rows.cuh) in float arithmetic.  A block holds a tile's queries, and runs of
+// KEYS key and value rows one after the other, in shared memory as floats; scores by 4 x 4 (2 x 2) rows x keys per thread along the
+// head's dimensions, the rows' softmax by 256 / ROWS threads each, weights times values by 4 (2) rows x dimensions per thread; both
+// products two multiply-adds to an instruction.  Bound by these and by the shared memory's reads (two of 16 bytes per eight
+// of them for the scores).  ROWS 16 for tiles of at most 16 rows: with 128 only one thread in eight would have work.
+// attention_single_any_kernel: a warp per key in turn, lanes along the head's dimensions; for single tokens where the kernel of
+// attention_single8.cuh has no instance.  Both visit or use no row that a query does not see: numbers that are not finite
+// stay where they are.
+#include "attention_single8.cuh"
+
+__device__ __forceinline__ void ar_fma2(float2& d, float2 a, float2 b) {
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 d, {%0, %1};\n\t"
+        "fma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
+        : "+f"(d.x), "+f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+
+#define AA_THREADS 256
+template <int ROWS> struct AnyShape {
+    static constexpr int KEYS = ROWS == 128 ? 32 : 64;
+    static constexpr int RPT = ROWS == 128 ? 4 : 2, KPT = ROWS == 128 ? 4 : 2;
+    static constexpr int RG = ROWS / RPT, KG = KEYS / KPT;          // groups of rows, of keys (and of dimensions)
+    static_assert(RG * KG == AA_THREADS, "");
+};
+__host__ __device__ inline int aa_stride(int d) { return ((d + 3) & ~3) + 4; }
+template <int ROWS> static size_t aa_smem(int d) {
+    return (size_t)(ROWS * aa_stride(d) + 2 * AnyShape<ROWS>::KEYS * aa_stride(d) + ROWS * (AnyShape<ROWS>::KEYS + 4)) * 4;
+}
+
+template <int FORM, typename QT, int ROWS, int DP>
+__global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const RowArgs a) {
+    using S = AnyShape<ROWS>;
+    constexpr int KEYS = S::KEYS, RPT = S::RPT, KPT = S::KPT, RG = S::RG, KG = S::KG;
+    constexpr int DT = (DP + 4 * KG - 1) / (4 * KG);               // pieces of four dimensions per thread
+    constexpr int TPR = AA_THREADS / ROWS;                         // threads of a row's softmax
+    extern __shared__ __align__(16) float aa_smem_raw[];
+    __shared__ uint32_t s_row[KEYS];
+    __shared__ float s_ks[KEYS], s_vs[KEYS];
+    __shared__ int s_pos[ROWS], s_token[ROWS], s_odd;
+    __shared__ float s_corr[ROWS];
+    const int d = a.d, ld = aa_stride(d), nv = (d + 3) / 4;
+    float* sq = aa_smem_raw;
+    float* sk = sq + ROWS * ld;
+    float* sv = sk + KEYS * ld;
+    float* sp = sv + KEYS * ld;
+    constexpr int LP = KEYS + 4;
+    const int tid = threadIdx.x, rg = tid / KG, kg = tid % KG, g = a.plan.group;
+    const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
+    ST_PDL_TRIGGER();
+    RowWalk walk;
+    walk.begin(a.plan, blockIdx.x);
+    RowPiece pc;
+    while (walk.next(a.plan, pc)) {
+        const int rows = pc.t.n_tok * g;
+        __syncthreads();                                            // the piece before is done with shared memory
+        for (int r = tid; r < ROWS; r += AA_THREADS) {
+            const int token = r < rows ? (a.plan.items ? a.plan.items[pc.t.first + r / g] : pc.t.first + r / g) : -1;
+            s_token[r] = token;
+            s_pos[r] = token >= 0 ? a.positions[token] : -1;
+        }
+        __syncthreads();
+        for (int i = tid; i < ROWS * nv * 4; i += AA_THREADS) {
+            const int r = i / (nv * 4), e = i - r * nv * 4;
+            const int token = s_token[r];
+            sq[r * ld + e] = token >= 0 && e < d
+                ? to_f32(((const QT*)a.q)[(size_t)token * a.q_stride + (size_t)(pc.head * g + r % g) * d + e]) * a.scale_log2 : 0.f;
+        }
+        const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
+        const int* bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
+        float ref = -INFINITY, sum = 0.f;                           // of row tid / TPR
+        float2 acc[RPT][DT][2];
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+#pragma unroll
+            for (int c = 0; c < DT; ++c) acc[i][c][0] = acc[i][c][1] = make_float2(0.f, 0.f);
+        const int k_begin = (pc.t.key_lo & ~(AR_CHUNK - 1)) + pc.chunk0 * AR_CHUNK;
+        const int k_end = min(k_begin + pc.chunks * AR_CHUNK, pc.t.key_hi);
+        for (int k0 = k_begin; k0 < k_end; k0 += KEYS) {
+            __syncthreads();
+            if (tid == 0) s_odd = 0;
+            for (int j = tid; j < KEYS; j += AA_THREADS) {
+                const int key = k0 + j;
+                uint32_t row = 0xffffffffu;
+                if (key >= pc.t.key_lo && key < k_end) {
+                    const int page = a.kv.page(bt, key);
+                    if (page >= 0) row = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, a.kv.page_index(key));
+                    else if (a.kv.status) *a.kv.status = 1;
+                }
+                s_row[j] = row;
+                s_ks[j] = FORM < C8_BF16 && row != 0xffffffffu ? a.kv.scales[row] : 1.f;
+                s_vs[j] = FORM < C8_BF16 && row != 0xffffffffu ? a.kv.scales[row + to_values] : 1.f;
+            }
+            __syncthreads();
+            // rows as floats; what lies past d or has no key is zero
+            bool odd = false;
+            for (int i = tid; i < KEYS * nv; i += AA_THREADS) {
+                const int j = i / nv, e = (i - j * nv) * 4;
+                const uint32_t row = s_row[j];
+                float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+                if (row != 0xffffffffu) {
+                    const size_t at = (size_t)row * d + e, vt = (size_t)(row + to_values) * d + e;
+                    if (d % 4 == 0 && FORM == C8_F32) {
+                        const float4 x = *reinterpret_cast<const float4*>(a.kv.pool + at * 4), y = *reinterpret_cast<const float4*>(a.kv.pool + vt * 4);
+                        k[0] = x.x; k[1] = x.y; k[2] = x.z; k[3] = x.w;
+                        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+                    } else if (d % 4 == 0 && FORM < C8_BF16) {
+                        uint32_t h[4];
+                        c8_halves<FORM>(*reinterpret_cast<const uint32_t*>(a.kv.pool + at), h[0], h[1]);
+                        c8_halves<FORM>(*reinterpret_cast<const uint32_t*>(a.kv.pool + vt), h[2], h[3]);
+                        const float2 x = sg_unpack<true>(h[0]), y = sg_unpack<true>(h[1]), z = sg_unpack<true>(h[2]), w = sg_unpack<true>(h[3]);
+                        k[0] = x.x; k[1] = x.y; k[2] = y.x; k[3] = y.y;
+                        v[0] = z.x; v[1] = z.y; v[2] = w.x; v[3] = w.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (e + c < d) { k[c] = c8_value<FORM>(a.kv.pool, at + c); v[c] = c8_value<FORM>(a.kv.pool, vt + c); }
+                    }
+                    if (FORM < C8_BF16) {
+                        const float s = s_vs[j];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) v[c] *= s;
+                    }
+                    odd |= !(isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3]));
+                }
+                store4(sk + j * ld + e, make_float4(k[0], k[1], k[2], k[3]));
+                store4(sv + j * ld + e, make_float4(v[0], v[1], v[2], v[3]));
+            }
+            if (odd) s_odd = 1;
+            __syncthreads();
+            // ---- scores
+            if (rg < rows) {
+                float2 z[RPT][KPT];
+#pragma unroll
+                for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                    for (int j = 0; j < KPT; ++j) z[i][j] = make_float2(0.f, 0.f);
+                for (int e = 0; e < nv * 4; e += 4) {
+                    float4 x[RPT], y[KPT];
+#pragma unroll
+                    for (int i = 0; i < RPT; ++i) x[i] = load4(sq + (rg + RG * i) * ld + e);
+#pragma unroll
+                    for (int j = 0; j < KPT; ++j) y[j] = load4(sk + (kg + KG * j) * ld + e);
+#pragma unroll
+                    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                        for (int j = 0; j < KPT; ++j) {
+                            ar_fma2(z[i][j], make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y));
+                            ar_fma2(z[i][j], make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w));
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < RPT; ++i) {
+                    const int r = rg + RG * i, pos = s_pos[r];
+                    const int low = a.window > 0 ? pos - a.window + 1 : 0;
+#pragma unroll
+                    for (int j = 0; j < KPT; ++j) {
+                        const int jj = kg + KG * j, key = k0 + jj;
+                        const bool seen = s_row[jj] != 0xffffffffu && key <= pos && key >= low;
+                        sp[r * LP + jj] = seen ? (z[i][j].x + z[i][j].y) * s_ks[jj] : -INFINITY;
+                    }
+                }
+            }
+            __syncthreads();
+            // ---- softmax of row tid / TPR
+            {
+                const int r = tid / TPR, sub = tid % TPR;
+                constexpr int N = KEYS / TPR;
+                float z[N], mx = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    z[j] = r < rows ? sp[r * LP + sub + TPR * j] : -INFINITY;
+                    mx = fmaxf(mx, z[j]);
+                }
+#pragma unroll
+                for (int o = TPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const float m = fmaxf(ref, mx), use = m == -INFINITY ? 0.f : m;
+                const float corr = ref == -INFINITY ? 0.f : exp2f(ref - m);
+                float l = 0.f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float p = exp2f(z[j] - use);
+                    l += p;
+                    sp[r * LP + sub + TPR * j] = p;
+                }
+                sum = sum * corr + l;
+                ref = m;
+                if (sub == 0) s_corr[r] = corr;
+            }
+            __syncthreads();
+            // ---- weights times values: rows rg + RG i, dimensions 4 (kg + KG c) .. + 3
+            if (rg < rows) {
+                const bool guard = s_odd != 0;                      // a weight of zero must not meet a value that is not finite
+#pragma unroll
+                for (int i = 0; i < RPT; ++i) {
+                    const float corr = s_corr[rg + RG * i];
+#pragma unroll
+                    for (int c = 0; c < DT; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) { acc[i][c][h].x *= corr; acc[i][c][h].y *= corr; }
+                }
+                const int n_keys = min(KEYS, k_end - k0);
+                for (int j = 0; j < n_keys; ++j) {
+                    float p[RPT];
+#pragma unroll
+                    for (int i = 0; i < RPT; ++i) p[i] = sp[(rg + RG * i) * LP + j];
+#pragma unroll
+                    for (int c = 0; c < DT; ++c) {
+                        const int e = 4 * (kg + KG * c);
+                        if (e >= nv * 4) continue;
+                        const float4 v = load4(sv + j * ld + e);
+#pragma unroll
+                        for (int i = 0; i < RPT; ++i) {
+                            if (guard && p[i] == 0.f) continue;
+                            ar_fma2(acc[i][c][0], make_float2(p[i], p[i]), make_float2(v.x, v.y));
+                            ar_fma2(acc[i][c][1], make_float2(p[i], p[i]), make_float2(v.z, v.w));
+                        }
+                    }
+                }
+            }
+        }
+        // ---- the piece's sums: out, or into its slot
+        {
+            const int sub = tid % TPR;
+#pragma unroll
+            for (int o = TPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            __syncthreads();
+            float* s_sum = sp;
+            if (sub == 0) { s_sum[tid / TPR] = sum; s_sum[ROWS + tid / TPR] = ref; }
+            __syncthreads();
+            const bool direct = a.direct && pc.whole;
+            const size_t slot = (size_t)(pc.unit + blockIdx.x) * AR_ROWS;
+            if (!direct)
+                for (int r = tid; r < rows; r += AA_THREADS) { a.parts.r[slot + r] = s_sum[ROWS + r]; a.parts.l[slot + r] = s_sum[r]; }
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+                const int r = rg + RG * i;
+                if (r >= rows) continue;
+                const float l = s_sum[r], inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                for (int c = 0; c < DT; ++c) {
+                    const int e = 4 * (kg + KG * c);
+                    const float o[4] = {acc[i][c][0].x, acc[i][c][0].y, acc[i][c][1].x, acc[i][c][1].y};
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        if (e + h >= d) continue;
+                        if (!direct) a.parts.o[(slot + r) * d + e + h] = o[h];
+                        else if (s_pos[r] >= 0)
+                            ((QT*)a.out)[((size_t)s_token[r] * a.plan.nh + pc.head * g + r % g) * d + e + h] = from_f32<QT>(o[h] * inv);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---- joining the parts of units that a cut goes through ------------------------------------------------------------
+template <typename QT>
+__global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs a) {
+    const int tile = blockIdx.x / a.plan.nkv, head = blockIdx.x % a.plan.nkv, d = a.d, g = a.plan.group;
+    const RowTile t = ar_tile(a.plan, tile);
+    const int n = ar_chunks(t);
+    if (n == 0) return;
+    const int x0 = t.start + head * n, c0 = ar_owner(a.plan, x0), c1 = ar_owner(a.plan, x0 + n - 1);
+    if (c0 == c1) return;                                           // one block had it all and has stored it
+    ST_PDL_WAIT();
+    const size_t unit = (size_t)tile * a.plan.nkv + head;
+    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < t.n_tok * g * d; i += gridDim.y * blockDim.x) {
+        const int r = i / d, e = i - r * d, token = a.plan.items ? a.plan.items[t.first + r / g] : t.first + r / g;
+        if (token < 0 || a.positions[token] < 0) continue;
+        float m = -INFINITY, l = 0.f, o = 0.f;
+        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(a.parts.r + (unit + c) * AR_ROWS + r));
+        for (int c = c0; c <= c1; ++c) {
+            const size_t at = (unit + c) * AR_ROWS + r;
+            const float w = ar_weight(__ldcg(a.parts.r + at), m);
+            l += w * __ldcg(a.parts.l + at);
+            o += w * __ldcg(a.parts.o + at * d + e);
+        }
+        ((QT*)a.out)[((size_t)token * a.plan.nh + head * g + r % g) * d + e] = from_f32<QT>(l == 0.f ? 0.f : o / l);
+    }
+}
+
+// ---- single tokens, anything ----------------------------------------------------------------------------------------
+template <int FORM, typename QT>
+__global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleArgs a) {
+    extern __shared__ float smem[];
+    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, head = blockIdx.y, key_head = head / a.group, d = a.d;
+    const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
+    if (pos < 0) {
+        if (a.info) ST_PDL_WAIT();
+        return;
+    }
+    const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
+    int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    if (a.info) lo = max(lo, a.info[3 * item]);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+    const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
+    float q[8], acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int e = lane + 32 * i;
+        q[i] = e < d ? to_f32(((const QT*)a.q)[((size_t)token * a.nh + head) * d + e]) * a.scale_log2 : 0.f;
+        acc[i] = 0.f;
+    }
+    float ref = -INFINITY, sum = 0.f;
+    for (int b = lo + (split * W + warp) * 32; b <= pos; b += a.splits * W * 32) {
+        uint32_t row = 0xffffffffu;
+        float ks = 1.f, vs = 1.f;
+        if (b + lane <= pos) {
+            const int page = a.kv.page(bt, b + lane);
+            if (page >= 0) {
+                row = a.kv.row0(page, 0, key_head) + a.kv.offset(b + lane, a.kv.page_index(b + lane));
+                if (FORM < C8_BF16) { ks = a.kv.scales[row]; vs = a.kv.scales[row + to_values]; }
+            } else if (a.kv.status) {
+                *a.kv.status = 1;
+            }
+        }
+        float z = -INFINITY;
+        const int n = min(32, pos - b + 1);
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const uint32_t r = __shfl_sync(0xffffffffu, row, j);
+            float dot = 0.f;
+            if (r != 0xffffffffu) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (lane + 32 * i < d) dot += q[i] * c8_value<FORM>(a.kv.pool, (size_t)r * d + lane + 32 * i);
+            }
+            dot = warp_sum(dot);
+            if (lane == j && r != 0xffffffffu) z = dot * ks;
+        }
+        const float mx = warp_max(z), m = fmaxf(ref, mx), use = m == -INFINITY ? 0.f : m;
+        const float corr = ref == -INFINITY ? 0.f : exp2f(ref - m), p = exp2f(z - use);
+        ref = m;
+        sum = sum * corr + p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] *= corr;
+        const float w = p * vs;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const uint32_t r = __shfl_sync(0xffffffffu, row, j);
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (r != 0xffffffffu) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (lane + 32 * i < d) acc[i] += wj * c8_value<FORM>(a.kv.pool, (size_t)(r + to_values) * d + lane + 32 * i);
+            }
+        }
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) { smem[warp] = ref; smem[W + warp] = sum; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < d) smem[2 * W + warp * d + lane + 32 * i] = acc[i];
+    sg_finish<QT>(a, smem, W, 1, 1, d, token, item, head, key_head);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+// Warps for a (token, key head) and how they are put into blocks and clusters.  Sixteen warps for every SM keep enough loads in
+// flight; a pair gets its share of them, though a warp should have two runs of keys at least, in blocks of four warps (more blocks
+// than four warps each need share an SM better than large ones), in clusters of up to eight blocks; only where eight
+// such blocks are too few, in larger blocks.
+SingleShape sg_shape(long long n_pairs, int max_keys, int keys_per_run) {
+    const long long runs = (max_keys + keys_per_run - 1) / keys_per_run;
+    long long want = (16ll * st_sm_count() + n_pairs - 1) / n_pairs;
+    if (want > (runs + 1) / 2) want = (runs + 1) / 2;
+    SingleShape s{1, 4};
+    if (want <= 1) { s.warps = runs > 1 ? 4 : 1; if (runs <= 2) s.warps = (int)(runs < 1 ? 1 : runs); return s; }
+    while (s.splits < 8 && s.splits * s.warps < want) s.splits *= 2;
+    while (s.warps < SG_MAX_WARPS && s.splits * s.warps < want) s.warps *= 2;
+    return s;
+}
+
+template <int FORM, typename QT> static int aa_single(SingleArgs a, int max_keys, cudaStream_t s) {
+    const SingleShape shape = sg_shape((long long)a.n_items * a.nh, max_keys, 32);
+    a.splits = shape.splits;
+    a.row_blocks = 1;
+    const int warps = shape.warps < 4 ? shape.warps : 4;
+    return sg_launch("single_any", attention_single_any_kernel<FORM, QT>, a, warps, (size_t)warps * (a.d + 2) * 4, a.nh, s);
+}
+
+template <int FORM, typename QT, int ROWS> static int aa_rows(const RowArgs& a, cudaStream_t s) {
+    const size_t smem = aa_smem<ROWS>(a.d);
+    const int grid = a.plan.ctas;
+    if (a.d <= 64) {
+        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 64>), smem);
+        attention_rows_any_kernel<FORM, QT, ROWS, 64><<<grid, AA_THREADS, smem, s>>>(a);
+    } else if (a.d <= 128) {
+        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 128>), smem);
+        attention_rows_any_kernel<FORM, QT, ROWS, 128><<<grid, AA_THREADS, smem, s>>>(a);
+    } else {
+        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 256>), smem);
+        attention_rows_any_kernel<FORM, QT, ROWS, 256><<<grid, AA_THREADS, smem, s>>>(a);
+    }
+    return st_launch_status();
+}
+template <int FORM, typename QT> static int aa_rows(const RowArgs& a, int max_rows, cudaStream_t s) {
+    return max_rows <= 16 ? aa_rows<FORM, QT, 16>(a, s) : aa_rows<FORM, QT, 128>(a, s);
+}
+
+static bool ar_types(int act, int form) {
+    return form == C8_INT8 || form == C8_E4M3 ? act == 0 || act == 1 : form == C8_BF16 ? act == 1 : form == C8_F32 && act == 0;
+}
+static int ar_single(const SingleArgs& a, int act, int form, int max_keys, cudaStream_t s) {
+    const bool fast = a.kv.page_size % 8 == 0 && (a.d == 32 || a.d == 64 || a.d == 80 || a.d == 96 || a.d == 128) &&
+                      form != C8_F32;
+    if (fast) {
+        if (form == C8_INT8) return sg_int8(a, act == 0, max_keys, s);
+        if (form == C8_E4M3) return sg_e4m3(a, act == 0, max_keys, s);
+        return sg_bf16(a, max_keys, s);
+    }
+    if (form == C8_INT8) return act == 0 ? aa_single<C8_INT8, float>(a, max_keys, s) : aa_single<C8_INT8, bf16>(a, max_keys, s);
+    if (form == C8_E4M3) return act == 0 ? aa_single<C8_E4M3, float>(a, max_keys, s) : aa_single<C8_E4M3, bf16>(a, max_keys, s);
+    if (form == C8_BF16) return aa_single<C8_BF16, bf16>(a, max_keys, s);
+    return aa_single<C8_F32, float>(a, max_keys, s);
+}
+static int ar_rows(RowArgs a, int act, int form, int max_rows, cudaStream_t s) {
+    if (form == C8_INT8) return act == 0 ? aa_rows<C8_INT8, float>(a, max_rows, s) : aa_rows<C8_INT8, bf16>(a, max_rows, s);
+    if (form == C8_E4M3) return act == 0 ? aa_rows<C8_E4M3, float>(a, max_rows, s) : aa_rows<C8_E4M3, bf16>(a, max_rows, s);
+    if (form == C8_BF16) return aa_rows<C8_BF16, bf16>(a, max_rows, s);
+    return aa_rows<C8_F32, float>(a, max_rows, s);
+}
+
+// Blocks among which a plan's line of chunks is dealt out: as many as run at the same time.
+static int ar_ctas(const RowArgs& a) {
+    const int most = st_sm_count() * (a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
+    return a.plan.total < most ? (a.plan.total > 0 ? a.plan.total : 1) : most;
+}
+static RowParts ar_parts(float* scratch, long long slots) {
+    return RowParts{scratch, scratch + slots * AR_ROWS, scratch + 2 * slots * AR_ROWS};
+}
+
+struct RowCall {            // what the entry points take in common, as the caller lays it out
+    const void* q;
+    void* out;
+    const void* pool;
+    const float* scales;
+    const int* table;
+    const int* positions;
+    const int* seq_of_token;
+    const int* slots;
+    const int* items;
+    const int* tiles;
+    const int* info;
+    float* scratch;
+    int* status;
+    long long q_stride, num_pages, scratch_floats;
+    int max_pages, n_layers, layer, nh, nkv, d, page_size, window, act, form;
+    int n_items, n_tiles, total, max_rows, max_keys;
+    float scale;
+};
+static_assert(sizeof(RowCall) == 13 * 8 + 3 * 8 + 15 * 4 + 4, "the caller lays this out field by field");
+
+static int ar_check(const RowCall& c) {
+    if (c.nh <= 0 || c.nkv <= 0 || c.nh % c.nkv || c.d <= 0 || c.page_size <= 0 || c.layer < 0 || c.layer >= c.n_layers || c.max_pages <= 0 ||
+        c.num_pages <= 0 || !c.status || !(c.scale > 0.f) || c.window < 0 || !aligned16(c.pool) || !aligned16(c.scales))
+        return ST_ERR_BAD_ARG;
+    if (!ar_types(c.act, c.form)) return ST_ERR_BAD_DTYPE;
+    if ((c.form < C8_BF16) != (c.scales != nullptr)) return ST_ERR_BAD_ARG;
+    if (c.d > 256 || c.nh > 65535 || c.num_pages > 0x7fffffffll || !c8_rows_fit(c.num_pages, c.n_layers, c.nkv, c.page_size)) return ST_ERR_TOO_LARGE;
+    return 0;
+}
+static PagedKV ar_kv(const RowCall& c) {
+    return PagedKV{(const unsigned char*)c.pool, c.scales, c.table, c.max_pages, (int)c.num_pages, c.n_layers, c.layer, c.nkv, c.page_size,
+                   c8_shift(c.page_size), c.status};
+}
+static SingleArgs ar_single_args(const RowCall& c) {
+    SingleArgs a{};
+    a.q = c.q; a.out = c.out; a.kv = ar_kv(c); a.items = c.items; a.positions = c.positions; a.seq_of_token = c.seq_of_token;
+    a.slots = c.slots; a.nh = c.nh; a.group = c.nh / c.nkv; a.d = c.d; a.n_items = c.n_items; a.scale_log2 = c.scale * AR_LOG2E;
+    a.window = c.window;
+    return a;
+}
+static RowArgs ar_row_args(const RowCall& c) {
+    RowArgs a{};
+    a.q = c.q; a.out = c.out; a.q_stride = c.q_stride > 0 ? c.q_stride : (long long)c.nh * c.d; a.kv = ar_kv(c);
+    a.positions = c.positions; a.seq_of_token = c.seq_of_token; a.slots = c.slots; a.d = c.d;
+    a.scale_log2 = c.scale * AR_LOG2E; a.window = c.window;
+    a.plan = RowPlan{c.tiles, c.items, c.n_tiles, c.total, 1, c.nh, c.nkv, c.nh / c.nkv};
+    a.plan.ctas = ar_ctas(a);
+    return a;
+}
+
+ST_EXPORT int st_attention_rows_per_tile() { return AR_ROWS; }
+ST_EXPORT int st_attention_rows_chunk() { return AR_CHUNK; }
+// single tokens; max_keys: about the longest of them (it decides how the work is spread, nothing else)
+ST_EXPORT int st_attention_single8(const RowCall* c, void* stream) {
+    const int bad = ar_check(*c);
+    if (bad) return bad;
+    if (c->n_items <= 0) return 0;
+    return ar_single(ar_single_args(*c), c->act, c->form, c->max_keys, (cudaStream_t)stream);
+}
+
+// tiles of tokens that follow one another in a request
+ST_EXPORT int st_attention_tiles8(const RowCall* c, void* stream) {
+    const int bad = ar_check(*c);
+    if (bad) return bad;
+    if (c->n_tiles <= 0 || c->total <= 0) return 0;
+    if (c->nh / c->nkv > AR_ROWS) return ST_ERR_TOO_LARGE;
+    RowArgs a = ar_row_args(*c);
+    const long long slots = (long long)c->n_tiles * c->nkv + a.plan.ctas;
+    if (c->scratch_floats < slots * (long long)ar_part_floats(c->d)) return ST_ERR_BAD_ARG;
+    if (slots > (1 << 30) / AR_ROWS) return ST_ERR_TOO_LARGE;
+    a.parts = ar_parts(c->scratch, slots);
+    a.direct = 1;
+    const cudaStream_t s = (cudaStream_t)stream;
+    const int r = ar_rows(a, c->act, c->form, c->max_rows, s);
+    if (r || a.plan.ctas == 1) return r;
+    const dim3 grid(c->n_tiles * c->nkv, 4);
+    return c->act == 0 ? st_launch_pdl("rows_join", attention_rows_join_kernel<float>, grid, dim3(256), 0, s, a)
+                       : st_launch_pdl("rows_join", attention_rows_join_kernel<bf16>, grid, dim3(256), 0, s, a);
+}
+
+// single tokens in groups that share their first keys: the prefixes' parts, then every token's own keys and the whole
+ST_EXPORT int st_attention_shared(const RowCall* c, void* stream) {
+    const int bad = ar_check(*c);
+    if (bad) return bad;
+    if (c->n_items <= 0) return 0;
+    if (c->nh / c->nkv > AR_ROWS || c->q_stride > 0) return ST_ERR_BAD_ARG;
+    const cudaStream_t s = (cudaStream_t)stream;
+    SingleArgs single = ar_single_args(*c);
+    if (c->total > 0) {
+        RowArgs a = ar_row_args(*c);
+        const long long slots = (long long)c->n_tiles * c->nkv + a.plan.ctas;
+        if (c->scratch_floats < slots * (long long)ar_part_floats(c->d)) return ST_ERR_BAD_ARG;
+        if (slots > (1 << 30) / AR_ROWS) return ST_ERR_TOO_LARGE;
+        a.parts = ar_parts(c->scratch, slots);
+        a.direct = 0;
+        const int r = ar_rows(a, c->act, c->form, c->max_rows, s);
+        if (r) return r;
+        single.info = c->info;
+        single.plan = a.plan;
+        single.parts = a.parts;
+    }
+    return ar_single(single, c->act, c->form, c->max_keys, s);
+}

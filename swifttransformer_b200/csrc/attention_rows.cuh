@@ -1,0 +1,144 @@
+// What the attention kernels over 8-bit caches and over shared prefixes have in common: the tiles of query rows a plan names,
+// how their work is dealt out, and the parts of a row's softmax that different blocks leave for one another.
+//
+// A row is one (token, query head).  A tile holds the rows of up to 128 / g tokens, for one key head, g = query heads per key
+// head: row r is head r % g of the group of token r / g.  The tile's keys [key_lo, key_hi) are walked in chunks of AR_CHUNK.
+// All chunks of all (tile, key head) pairs, one pair's behind the other's, form one line of `total` chunks which is cut
+// into `ctas` runs of equal length: every block gets the same work however unequal the tiles are, and a pair that a cut goes
+// through ("unit") is put together from parts.  Part (unit u, block c) has slot u + c: a new slot begins with every unit and with
+// every block, so no two parts share one.
+//
+// A part of a row is (R, l, O): p_j = 2^(s_j - R), s in units of log2, l = sum p_j, O = sum p_j v_j, all float; R is a number near
+// the largest s_j (the exact maximum is not needed: only the common factor).  Parts are joined by 2^(R - max R).
+#pragma once
+#include "cache8.cuh"
+
+#define AR_ROWS 128
+#define AR_CHUNK 128
+#define AR_LOG2E 1.4426950408889634f
+
+// a tile of a plan: six numbers in the plan's array
+struct RowTile { int first, n_tok, seq, key_lo, key_hi, start; };   // start: the line's chunk where key head 0's share begins
+
+struct RowPlan {
+    const int* tiles;        // [n_tiles][6]
+    const int* items;        // tokens in the tiles' order, or null: tile tokens are first, first + 1, ...
+    int n_tiles, total, ctas;
+    int nh, nkv, group;      // group = nh / nkv
+};
+// where parts lie: per slot AR_ROWS rows (R, l) and AR_ROWS x d of O
+struct RowParts {
+    float* r;
+    float* l;
+    float* o;
+};
+__host__ __device__ inline size_t ar_part_floats(int d) { return (size_t)AR_ROWS * (2 + d); }
+
+// what the kernels of tiles get
+struct RowArgs {
+    const void* q;
+    void* out;
+    long long q_stride;              // elements between the query rows of neighbouring tokens
+    PagedKV kv;
+    RowPlan plan;
+    RowParts parts;
+    const int* positions;
+    const int* seq_of_token;
+    const int* slots;
+    int d, window;
+    int direct;                      // a unit that one block has wholly goes to `out`; else every piece to its slot
+    float scale_log2;
+};
+
+__device__ __forceinline__ RowTile ar_tile(const RowPlan& p, int i) {
+    const int* t = p.tiles + 6 * i;
+    return RowTile{__ldg(t), __ldg(t + 1), __ldg(t + 2), __ldg(t + 3), __ldg(t + 4), __ldg(t + 5)};
+}
+__device__ __forceinline__ int ar_chunks(const RowTile& t) {
+    return t.key_hi > t.key_lo ? (t.key_hi - (t.key_lo & ~(AR_CHUNK - 1)) + AR_CHUNK - 1) / AR_CHUNK : 0;
+}
+// the first chunk of block c's run, and the block whose run holds chunk x
+__device__ __forceinline__ int ar_run(const RowPlan& p, int c) { return (int)((long long)p.total * c / p.ctas); }
+__device__ __forceinline__ int ar_owner(const RowPlan& p, int x) {
+    int c = (int)((long long)x * p.ctas / p.total);
+    while (c + 1 < p.ctas && ar_run(p, c + 1) <= x) ++c;
+    while (c > 0 && ar_run(p, c) > x) --c;
+    return c;
+}
+
+// A block's way along its run: pieces of one (tile, key head) pair.
+struct RowPiece {
+    RowTile t;
+    int tile, head;          // head: key head
+    int unit, chunk0, chunks;   // chunks of the unit done here, from chunk0 on
+    bool whole;              // this piece is all of its unit
+};
+struct RowWalk {
+    int at, end, tile;
+    RowTile t;
+    __device__ __forceinline__ void begin(const RowPlan& p, int c) {
+        at = ar_run(p, c);
+        end = ar_run(p, c + 1);
+        // the last tile that starts at or before `at` (tiles without chunks start where the next one does)
+        int lo = 0, hi = p.n_tiles - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (__ldg(p.tiles + 6 * mid + 5) <= at) lo = mid; else hi = mid - 1;
+        }
+        tile = lo;
+        t = ar_tile(p, tile);
+    }
+    __device__ __forceinline__ bool next(const RowPlan& p, RowPiece& out) {
+        if (at >= end) return false;
+        int n = ar_chunks(t);
+        while (at >= t.start + n * p.nkv) {
+            if (++tile >= p.n_tiles) return false;
+            t = ar_tile(p, tile);
+            n = ar_chunks(t);
+        }
+        const int in = at - t.start;
+        out.t = t;
+        out.tile = tile;
+        out.head = in / n;
+        out.unit = tile * p.nkv + out.head;
+        out.chunk0 = in - out.head * n;
+        out.chunks = min(n - out.chunk0, end - at);
+        out.whole = out.chunks == n;
+        at += out.chunks;
+        return true;
+    }
+};
+
+// Cut and joined parts of row `row` of unit (tile, head) -> sums over e0, e0 + step, ... of d: calls f(weight, O row, l) per part.
+template <typename F>
+__device__ __forceinline__ void ar_each_part(const RowPlan& p, const RowTile& t, int tile, int head, F f) {
+    const int n = ar_chunks(t);
+    if (n == 0) return;
+    const int x0 = t.start + head * n, unit = tile * p.nkv + head;
+    const int c1 = ar_owner(p, x0 + n - 1);
+    for (int c = ar_owner(p, x0); c <= c1; ++c) f(unit + c);
+}
+
+__device__ __forceinline__ float ar_exp2(float x) {      // 2 ulp, exp2(-inf) = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// the weight of a part with reference r beside the largest reference m (none: -inf)
+__device__ __forceinline__ float ar_weight(float r, float m) { return r == -INFINITY ? 0.f : ar_exp2(r - m); }
+
+static inline int ar_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
+}
+// dynamic shared memory above 48 KB is asked for once per kernel and device
+#define AR_ALLOW_SMEM(kernel, bytes)                                                                                     \
+    do {                                                                                                                 \
+        static size_t allowed[64] = {0};                                                                                 \
+        size_t& have = allowed[ar_device()];                                                                             \
+        if ((size_t)(bytes) > 48 * 1024 && have < (size_t)(bytes)) {                                                     \
+            const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes)); \
+            if (err != cudaSuccess) { cudaGetLastError(); return (int)err; }                                             \
+            have = (size_t)(bytes);                                                                                      \
+        }                                                                                                                \
+    } while (0)

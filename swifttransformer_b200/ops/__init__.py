@@ -1947,3 +1947,8 @@ def hc_step_conv(lanes: torch.Tensor, pending: Optional[tuple], coef: torch.Tens
                                  _p(tmp), _p(out), _dt(out), _p(positions), _p(seq_of_token), _p(slots), _stream()),
            "hc_step_conv")
     return out
+
+
+# ------------------------------------------------------------ caches in 8 bits, shared prefixes
+from .cache8 import (CACHE8_TYPES, RowPlan, attention_cache8_single, attention_cache8_tiles, attention_shared_prefix,  # noqa: E402
+                     cache8_pool, cache8_rows, portion_plan, qkv_to_cache8, shared_prefix_plan)

@@ -1,0 +1,318 @@
+"""Caches in 8 bits, attention over them, and attention for batches that share a prefix.
+
+An 8-bit cache is a pair of tensors: ``pool`` [pages, layers, 2, kv heads, page size, head size] of ``torch.int8`` or
+``torch.float8_e4m3fn`` and ``scales`` [pages, layers, 2, kv heads, page size] of float32.  An element stands for its code times
+its row's scale.  A row x is stored with the scale max(max|x| / M, 2^-126), M = 127 for int8 and 448 for e4m3, and the codes
+x / scale rounded to the nearest number of the form, ties to even; a row with a NaN or an infinity has the scale NaN.  The reference
+keeps its cache in the type of its activations (src/csrc/kernel/kvcache_mgmt.cu:29-80).
+
+Against bfloat16 a cache takes 0.53 (head size 64) or 0.52 (128) of the memory, and a decode step reads that much less.  int8
+stores a row's elements to 1 / 254 of its largest, e4m3 every element to 1 / 16 of itself.
+
+All functions take the index tensors of the other paged operations: ``positions`` and ``seq_of_token`` per token, ``slots`` per
+request, ``block_table`` [slots, pages], int32 on the device.  A token whose position is negative is padding and left out.
+``status`` (int32, by default a word that ``ops.kernel_status`` reads) is set to 1 when a key that a query needs has no page; such
+keys count as absent, and a query without any key gets zeros.  Calls launch on the current stream and keep no state of their own.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import KernelError, _check, _p, _stream, _tc_status_word, lib, sm_count
+
+CACHE8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_FORMS = {torch.int8: 0, torch.float8_e4m3fn: 1, torch.bfloat16: 2, torch.float32: 3}
+_ACTS = {torch.float32: 0, torch.bfloat16: 1}
+_I32 = torch.int32
+# query rows of a tile, keys of a chunk (the library's; see st_attention_rows_per_tile, st_attention_rows_chunk)
+ROWS_PER_TILE = 128
+ROWS_CHUNK = 128
+
+
+def cache8_pool(num_pages: int, n_layers: int, nkv: int, page_size: int, d: int, dtype: torch.dtype, device):
+    """An empty 8-bit cache (pool, scales): every row reads back as zeros."""
+    if dtype not in CACHE8_TYPES:
+        raise KernelError(f"an 8-bit cache is int8 or float8_e4m3fn, not {dtype}")
+    shape = (num_pages, n_layers, 2, nkv, page_size)
+    return (torch.zeros(shape + (d,), dtype=torch.int8, device=device).view(dtype),
+            torch.zeros(shape, dtype=torch.float32, device=device))
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(what)
+
+
+def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """All tensors on one CUDA device, the current one: the launch goes there."""
+    if not first.is_cuda:
+        raise KernelError("this engine runs on a CUDA device only; got a CPU tensor")
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise KernelError(f"{what}: tensors on different devices")
+    if index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _index(what: str, name: str, t: torch.Tensor, dim: int = 1) -> None:
+    if t.dtype != _I32 or t.dim() != dim or not t.is_contiguous():
+        raise KernelError(f"{what}: {name} is a contiguous int32 tensor of {dim} dimension(s)")
+
+
+def _pool8(what: str, pool: torch.Tensor, scales: Optional[torch.Tensor], layer: int) -> None:
+    _need(pool.dim() == 6 and pool.shape[2] == 2 and pool.is_contiguous(),
+          f"{what}: the pool is a contiguous [pages, layers, 2, kv heads, page size, head size]")
+    _need(pool.dtype in _FORMS, f"{what}: unsupported cache type {pool.dtype}")
+    if pool.dtype in CACHE8_TYPES:
+        _need(scales is not None and scales.dtype == torch.float32 and scales.shape == pool.shape[:5] and scales.is_contiguous(),
+              f"{what}: an 8-bit pool comes with contiguous float32 scales [pages, layers, 2, kv heads, page size]")
+    else:
+        _need(scales is None, f"{what}: scales belong to 8-bit pools")
+    _need(0 <= layer < pool.shape[1], f"{what}: the pool has no layer {layer}")
+
+
+def qkv_to_cache8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: Optional[torch.Tensor], pool: torch.Tensor,
+                  scales: torch.Tensor, layer: int, positions: torch.Tensor, seq_of_token: torch.Tensor, slots: torch.Tensor,
+                  block_table: torch.Tensor, nh: int, nkv: int, d: int, status: Optional[torch.Tensor] = None,
+                  write_kv: bool = True) -> None:
+    """q_out = q + bias; the rows k + bias and v + bias (float32 sums) quantised into an 8-bit cache at each token's position.
+
+    ``qkv`` [tokens, (nh + 2 nkv) d] float32 or bfloat16; ``bias`` float32 or None; ``q_out`` [tokens, nh d] of qkv's type, or None: the
+    queries stay where they are.  ``write_kv`` False: only the queries move.  Head sizes up to 256."""
+    what = "qkv_to_cache8"
+    n = qkv.shape[0]
+    _same_device(what, qkv, bias, q_out, pool, scales, positions, seq_of_token, slots, block_table, status)
+    _need(qkv.dtype in _ACTS and qkv.is_contiguous() and qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * d,
+          f"{what}: qkv is a contiguous [tokens, (nh + 2 nkv) d] of float32 or bfloat16")
+    _need(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == qkv.shape[1]),
+          f"{what}: the bias is contiguous float32, one number per column")
+    _need(q_out is None or (q_out.dtype == qkv.dtype and q_out.shape == (n, nh * d) and q_out.is_contiguous()),
+          f"{what}: q_out is a contiguous [tokens, nh d] of qkv's type")
+    _pool8(what, pool, scales, layer)
+    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
+    _need(pool.shape[3] == nkv and pool.shape[5] == d, f"{what}: the pool has other heads or sizes")
+    for name, t, dim in (("positions", positions, 1), ("seq_of_token", seq_of_token, 1), ("slots", slots, 1),
+                         ("block_table", block_table, 2)):
+        _index(what, name, t, dim)
+    _need(positions.numel() >= n and seq_of_token.numel() >= n, f"{what}: a position and a request for every token")
+    st = status if status is not None else _tc_status_word(qkv.device)
+    _check(lib().st_qkv_to_cache8(_p(qkv), _p(bias), _p(q_out), _p(pool), _p(scales), _p(positions), _p(seq_of_token), _p(slots),
+                                  _p(block_table), block_table.shape[1], pool.shape[0], pool.shape[1], layer, n, nh, nkv, d,
+                                  pool.shape[4], int(write_kv), _p(st), _ACTS[qkv.dtype], _FORMS[pool.dtype], _stream()), what)
+
+
+def cache8_rows(pool: torch.Tensor, scales: torch.Tensor, layer: int, out: torch.Tensor, positions: torch.Tensor,
+                seq_of_token: torch.Tensor, slots: torch.Tensor, block_table: torch.Tensor,
+                status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = the keys of all heads, then the values of all heads, of position ``positions[t]`` of request ``seq_of_token[t]``:
+    [tokens, 2 nkv d] float32 or bfloat16, code times scale.  A position without a page gives zeros."""
+    what = "cache8_rows"
+    _same_device(what, out, pool, scales, positions, seq_of_token, slots, block_table, status)
+    _pool8(what, pool, scales, layer)
+    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
+    nkv, page_size, d = pool.shape[3:]
+    n = out.shape[0]
+    _need(out.dtype in _ACTS and out.is_contiguous() and out.shape == (n, 2 * nkv * d),
+          f"{what}: out is a contiguous [tokens, 2 nkv d] of float32 or bfloat16")
+    for name, t, dim in (("positions", positions, 1), ("seq_of_token", seq_of_token, 1), ("slots", slots, 1),
+                         ("block_table", block_table, 2)):
+        _index(what, name, t, dim)
+    _need(positions.numel() >= n and seq_of_token.numel() >= n, f"{what}: a position and a request for every row")
+    st = status if status is not None else _tc_status_word(out.device)
+    _check(lib().st_cache8_rows(_p(pool), _p(scales), _p(out), _p(positions), _p(seq_of_token), _p(slots), _p(block_table),
+                                block_table.shape[1], pool.shape[0], pool.shape[1], layer, n, nkv, d, page_size, _p(st),
+                                _ACTS[out.dtype], _FORMS[pool.dtype], _stream()), what)
+    return out
+
+
+# ------------------------------------------------------------------ plans
+class RowPlan:
+    """Which query rows share a pass over which keys: made on the host once per step, used by all its layers.
+
+    ``tiles``: int32 [n_tiles, 6] on the device: first token (or place in ``items``), tokens, request (-1: that of the first
+    item), first and last + 1 key, and where the tile's chunks begin in the line of all chunks.  ``items``: the tokens of
+    a plan for shared prefixes in the tiles' order; ``info`` [items, 3]: keys shared with the group, tile, place in the tile."""
+
+    def __init__(self, kind: str, nh: int, nkv: int, device):
+        _need(nkv > 0 and nh > 0 and nh % nkv == 0, f"{nh} heads cannot share {nkv} key/value heads")
+        _need(nh // nkv <= ROWS_PER_TILE, f"at most {ROWS_PER_TILE} query heads to a key head")
+        self.kind, self.nh, self.nkv, self.window = kind, nh, nkv, 0
+        self.device = torch.device(device)
+        self.n_tiles = self.n_items = self.total = self.max_rows = self.max_own = self.n_tokens = self.n_seqs = 0
+        self.tiles = self.items = self.info = None
+
+    @property
+    def tokens_per_tile(self) -> int:
+        return ROWS_PER_TILE // (self.nh // self.nkv)
+
+    def _chunks(self, lo: int, hi: int) -> int:
+        return -(-(hi - lo // ROWS_CHUNK * ROWS_CHUNK) // ROWS_CHUNK) if hi > lo else 0
+
+    def _upload(self, tiles, items=None, info=None) -> None:
+        start = 0
+        rows = []
+        for first, n, seq, lo, hi in tiles:
+            rows.append((first, n, seq, lo, hi, start))
+            start += self._chunks(lo, hi) * self.nkv
+        _need(start < 1 << 31 and len(rows) * self.nkv < 1 << 22, "a plan of more keys than one call serves")
+        self.total, self.n_tiles = start, len(rows)
+        self.max_rows = max((r[1] for r in rows), default=0) * (self.nh // self.nkv)
+        flat = np.asarray(rows, dtype=np.int32).reshape(-1)
+        parts = [flat] + [np.asarray(x, dtype=np.int32).reshape(-1) for x in (items, info) if x is not None]
+        dev = torch.from_numpy(np.concatenate(parts)).to(self.device)
+        self.tiles = dev[:flat.size]
+        if items is not None:
+            self.items = dev[flat.size:flat.size + parts[1].size]
+            self.info = dev[flat.size + parts[1].size:]
+            self.n_items = parts[1].size
+
+
+def portion_plan(lens: Sequence[int], starts: Sequence[int], nh: int, nkv: int, window: int = 0, device="cuda") -> RowPlan:
+    """The plan of a step in which request i brings ``lens[i]`` tokens, one behind the other, and has ``starts[i]`` in the cache."""
+    plan = RowPlan("portion", nh, nkv, device)
+    _need(len(lens) == len(starts) and all(n >= 0 for n in lens) and all(s >= 0 for s in starts) and window >= 0,
+          "portion_plan: a length and a start per request, none negative")
+    plan.window, per, tiles, first = int(window), plan.tokens_per_tile, [], 0
+    for seq, (n, start) in enumerate(zip(lens, starts)):
+        for off in range(0, n, per):
+            m, pos = min(per, n - off), start + off
+            tiles.append((first + off, m, seq, max(0, pos - window + 1) if window else 0, pos + m))
+        first += n
+    plan.n_tokens, plan.n_seqs = first, len(lens)
+    plan._upload(tiles)
+    return plan
+
+
+def shared_prefix_plan(groups: Sequence[Sequence[int]], shared: Sequence[int], nh: int, nkv: int, device="cuda",
+                       max_own: int = 0) -> RowPlan:
+    """The plan of a step of single tokens: ``groups[i]`` lists the tokens whose requests have their first ``shared[i]`` keys in common
+    (0: none).  ``max_own``: about the most keys a token has behind its shared ones (it decides how the work is spread)."""
+    plan = RowPlan("shared", nh, nkv, device)
+    _need(len(groups) == len(shared) and all(s >= 0 for s in shared), "shared_prefix_plan: a shared length per group, none negative")
+    per, tiles, items, info = plan.tokens_per_tile, [], [], []
+    for tokens, n in zip(groups, shared):
+        for off in range(0, len(tokens), per):
+            part = [int(t) for t in tokens[off:off + per]]
+            tiles.append((len(items), len(part), -1, 0, int(n)))
+            info += [(int(n), len(tiles) - 1, k) for k in range(len(part))]
+            items += part
+    _need(all(t >= 0 for t in items) and len(set(items)) == len(items), "shared_prefix_plan: every token at most once, none negative")
+    plan.n_tokens, plan.max_own = max(items, default=-1) + 1, int(max_own)
+    plan._upload(tiles, items, info)
+    return plan
+
+
+# ------------------------------------------------------------------ attention
+_CALL = struct.Struct("=13Q3q15if")
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale, window, status, *,
+            items=None, n_items=0, plan=None, max_keys=0) -> None:
+    _same_device(what, q, pool, scales, out, positions, seq_of_token, slots, block_table, status, items,
+                 plan.tiles if plan is not None else None)
+    _pool8(what, pool, scales, layer)
+    n_pages, n_layers, _, nkv, page_size, d = pool.shape
+    n = out.shape[0]
+    _need(nh > 0 and nh % nkv == 0, f"{what}: {nh} heads cannot share {nkv} key/value heads")
+    _need(q.dtype in _ACTS and out.dtype == q.dtype, f"{what}: queries and results are float32 or bfloat16, of one type")
+    _need(pool.dtype in CACHE8_TYPES or pool.dtype == q.dtype, f"{what}: a {pool.dtype} cache with {q.dtype} queries")
+    _need(q.dim() == 2 and out.is_contiguous() and q.shape == out.shape and q.shape[1] == nh * d and q.stride(1) == 1,
+          f"{what}: q and out are [tokens, nh d], out contiguous, q's rows contiguous")
+    stride = q.stride(0) if n > 1 else nh * d
+    _need(scale > 0.0, f"{what}: the scale is positive")
+    _need(window >= 0, f"{what}: the window is not negative")
+    _index(what, "positions", positions)
+    _index(what, "slots", slots)
+    _index(what, "block_table", block_table, 2)
+    if seq_of_token is not None:
+        _index(what, "seq_of_token", seq_of_token)
+    if items is not None:
+        _index(what, "items", items)
+    _need(positions.numel() >= n and (seq_of_token is None or seq_of_token.numel() >= n),
+          f"{what}: a position and a request for every token")
+    if stride != nh * d:
+        _need(plan is not None and plan.kind == "portion" and stride >= nh * d, f"{what}: q is contiguous")
+    else:
+        stride = 0
+    st = status if status is not None else _tc_status_word(q.device)
+    scratch = None
+    n_tiles = total = max_rows = 0
+    tiles = info = None
+    if plan is not None:
+        _need(plan.nh == nh and plan.nkv == nkv, f"{what}: the plan is for {plan.nh} heads over {plan.nkv}")
+        _need(plan.n_tokens <= n and plan.n_seqs <= slots.numel(), f"{what}: the plan names tokens or requests that are not there")
+        tiles, info, items = plan.tiles, plan.info, plan.items
+        n_items, n_tiles, total, max_rows = plan.n_items, plan.n_tiles, plan.total, plan.max_rows
+        if total:
+            # parts of rows that several blocks leave: a slot per (tile, key head) and one per block
+            scratch = torch.empty((n_tiles * nkv + 3 * sm_count(q.device)) * ROWS_PER_TILE * (2 + d), dtype=torch.float32,
+                                  device=q.device)
+    call = _CALL.pack(q.data_ptr(), out.data_ptr(), pool.data_ptr(), _ptr(scales), block_table.data_ptr(), positions.data_ptr(),
+                      _ptr(seq_of_token), slots.data_ptr(), _ptr(items), _ptr(tiles), _ptr(info), _ptr(scratch), st.data_ptr(),
+                      stride, n_pages, scratch.numel() if scratch is not None else 0,
+                      block_table.shape[1], n_layers, layer, nh, nkv, d, page_size, window, _ACTS[q.dtype], _FORMS[pool.dtype],
+                      n_items, n_tiles, total, max_rows, max_keys, scale)
+    _check(entry(call, _stream()), what)
+
+
+def attention_cache8_single(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, layer: int, out: torch.Tensor,
+                            items: Optional[torch.Tensor], n_items: int, positions: torch.Tensor, seq_of_token: torch.Tensor,
+                            slots: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float, window: int = 0, max_kv: int = 0,
+                            status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of single query tokens over an 8-bit cache: what ``attention_decode`` does over a bfloat16 one.  ``q`` and ``out``
+    [tokens, nh d] float32 or bfloat16; ``items`` lists the token indices that are served (-1: none; None: tokens 0 .. n_items - 1),
+    the rows of ``out`` of other tokens stay.  ``max_kv``: about the most keys a token reads (0: what the block table has room
+    for); it decides how the work is spread, not the result's meaning."""
+    what = "attention_cache8_single"
+    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
+    _need(0 <= n_items <= (items.numel() if items is not None else out.shape[0]), f"{what}: n_items tokens are not there")
+    reach = block_table.shape[-1] * pool.shape[4] if pool.dim() == 6 else 0
+    keys = min(max_kv, reach) if max_kv > 0 else reach
+    if window > 0:
+        keys = min(keys, window)
+    _attend(what, lib().st_attention_single8, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale,
+            window, status, items=items, n_items=n_items, max_keys=keys)
+    return out
+
+
+def attention_cache8_tiles(q: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor, layer: int, out: torch.Tensor, plan: RowPlan,
+                           positions: torch.Tensor, slots: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
+                           window: int = 0, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of portions of prompts over an 8-bit cache: what ``attention_prefill`` does over a bfloat16 one.  ``plan``: from
+    ``portion_plan``, of the same heads and window.  ``q`` may be the first columns of the q|k|v product (any row stride).  The
+    portions' own keys and values have been written (``qkv_to_cache8``)."""
+    what = "attention_cache8_tiles"
+    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
+    _need(plan.kind == "portion" and plan.window == window, f"{what}: the plan is from portion_plan, for this window")
+    _attend(what, lib().st_attention_tiles8, q, pool, scales, layer, out, positions, None, slots, block_table, nh, scale, window,
+            status, plan=plan)
+    return out
+
+
+def attention_shared_prefix(q: torch.Tensor, pool: torch.Tensor, layer: int, out: torch.Tensor, plan: RowPlan,
+                            positions: torch.Tensor, seq_of_token: torch.Tensor, slots: torch.Tensor, block_table: torch.Tensor,
+                            nh: int, scale: float, window: int = 0, scales: Optional[torch.Tensor] = None,
+                            status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of single query tokens whose requests share their first keys: the result of ``attention_decode`` for every token of
+    ``plan`` (from ``shared_prefix_plan``), with a group's shared keys and values read once for the group, through the block table of its
+    first token's request.  The cache is of q's type, or an 8-bit one with its ``scales``.
+
+    A token's position may lie anywhere, inside the shared keys too: it sees keys 0 .. its own position (``window`` > 0: the last
+    ``window`` of these).  A value that is not finite reaches, in bfloat16 caches, all rows of its group that share it, also those
+    whose window or position hides it; in the other forms only rows that see it."""
+    what = "attention_shared_prefix"
+    _need(plan.kind == "shared", f"{what}: the plan is from shared_prefix_plan")
+    keys = plan.max_own if plan.max_own > 0 else block_table.shape[-1] * pool.shape[4] if pool.dim() == 6 else 0
+    _attend(what, lib().st_attention_shared, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale,
+            window, status, plan=plan, max_keys=keys)
+    return out
