@@ -415,16 +415,20 @@ static int ar_single(const SingleArgs& a, int act, int form, int max_keys, cudaS
     if (form == C8_BF16) return aa_single<C8_BF16, bf16>(a, max_keys, s);
     return aa_single<C8_F32, float>(a, max_keys, s);
 }
+static bool ar_tc(const RowArgs& a, int act, int form) {
+    return act == 1 && form != C8_F32 && a.d % 16 == 0 && a.d <= 128 && aligned16(a.q) && aligned16(a.out) && a.q_stride % 8 == 0;
+}
 static int ar_rows(RowArgs a, int act, int form, int max_rows, cudaStream_t s) {
+    if (ar_tc(a, act, form)) return ar_rows_tc(a, form, s);
     if (form == C8_INT8) return act == 0 ? aa_rows<C8_INT8, float>(a, max_rows, s) : aa_rows<C8_INT8, bf16>(a, max_rows, s);
     if (form == C8_E4M3) return act == 0 ? aa_rows<C8_E4M3, float>(a, max_rows, s) : aa_rows<C8_E4M3, bf16>(a, max_rows, s);
     if (form == C8_BF16) return aa_rows<C8_BF16, bf16>(a, max_rows, s);
     return aa_rows<C8_F32, float>(a, max_rows, s);
 }
 
-// Blocks among which a plan's line of chunks is dealt out: as many as run at the same time.
-static int ar_ctas(const RowArgs& a) {
-    const int most = st_sm_count() * (a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
+// Blocks among which a plan's line of chunks is dealt out: as many as run at the same time, one per SM of the tensor-core kernel.
+static int ar_ctas(const RowArgs& a, int act, int form) {
+    const int most = st_sm_count() * (ar_tc(a, act, form) ? 1 : a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
     return a.plan.total < most ? (a.plan.total > 0 ? a.plan.total : 1) : most;
 }
 static RowParts ar_parts(float* scratch, long long slots) {
@@ -478,7 +482,7 @@ static RowArgs ar_row_args(const RowCall& c) {
     a.positions = c.positions; a.seq_of_token = c.seq_of_token; a.slots = c.slots; a.d = c.d;
     a.scale_log2 = c.scale * AR_LOG2E; a.window = c.window;
     a.plan = RowPlan{c.tiles, c.items, c.n_tiles, c.total, 1, c.nh, c.nkv, c.nh / c.nkv};
-    a.plan.ctas = ar_ctas(a);
+    a.plan.ctas = ar_ctas(a, c.act, c.form);
     return a;
 }
 

@@ -142,3 +142,7 @@ static inline int ar_device() {
             have = (size_t)(bytes);                                                                                      \
         }                                                                                                                \
     } while (0)
+
+// tiles on the tensor cores (attention_rows_tc.cu): bfloat16 queries, 8-bit and bfloat16 caches, head sizes that are multiples of 16
+// up to 128
+int ar_rows_tc(const RowArgs& a, int form, cudaStream_t s);

@@ -1,0 +1,615 @@
+// Attention of tiles of query rows (attention_rows.cuh) over 8-bit and bfloat16 paged caches on tcgen05: portions of prompts, and
+// groups of tokens over the prefix they share.
+//
+// Mathematics: as in attention_single8.cuh.  Codes of an 8-bit cache and queries (scaled by a power of two per row) are halves, the rows'
+// scales stay outside: s_j = (q . c_j) ks_j, P_j = p_j vs_j in half; over bfloat16 caches queries, keys, P and values are
+// bfloat16.  S = Q K^T of 128 rows x 64 keys and O += P V are tcgen05 products with their sums in tensor memory; P goes there
+// straight from the softmax threads' registers (the product's A operand).
+//
+// One block per SM walks its run of the plan's chunks.  Two groups of four softmax warps take every second tile of 64 keys of a
+// piece, each with its own S, O and P in tensor memory, key and value buffers (two each) and issuing warp; at the piece's end
+// the first group reads the second's O from tensor memory (the lanes are the same rows) and stores the sum.  Four warps bring
+// keys, four bring values, for both groups in turn, and run ahead across pieces:
+//   8-bit forms: 16-byte loads to registers, several tiles ahead (32 KB per SM under way: memory needs that), conversion to
+//   halves, stores into the 128-byte swizzled layout the matrix descriptors expect.  Conversion is the price of the format: about
+//   2.5 instructions per four codes against the softmax's 4 per score; with one row of 128 codes per thread, two warps each, it
+//   bounded the kernel, so there are four.
+//   bfloat16: asynchronous copies into that layout, as many tiles ahead as there are buffers.
+// Page sizes are arbitrary: every thread looks up its row's page, a tile ahead of its loads.
+// With the row's scales go their largest value scale per tile, from which the softmax threads take the power of two that keeps P in
+// a half's range (attention_single8.cuh), and a mark where a key has no page.
+//
+// Bound by the softmax (an exponential per score, 16 a clock and SM) at head size 64, by softmax and conversion together at 128, and by
+// memory for prefixes shared by few rows.  Waits are bounded; one that expires marks the block dead, the other waits end, `status`
+// gets 3, tensor memory is freed and the kernel returns.
+#include "attention_rows.cuh"
+#include "tcgen05.cuh"
+
+#define RT_THREADS 640                   // 8 softmax warps, 4 for keys, 4 for values, 2 issuing products, 2 to fill the last four
+// Registers a thread keeps after the block has shared them out anew; the sum must not pass what the launch got, 640 x 96.
+#define RT_REGS_SOFTMAX 144
+#define RT_REGS_OTHER 64
+static_assert(256 * RT_REGS_SOFTMAX + 384 * RT_REGS_OTHER <= RT_THREADS * 96, "more registers than the block owns");
+#define RT_META 4                        // tiles whose scales are kept: see below
+
+__device__ __forceinline__ void rt_mbar_arrive(uint32_t mbar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(mbar) : "memory");
+}
+// Named barriers.  1-4: a softmax group and the warp that issues its products (160 threads): 0 "S has been read", 1 "P has been written".
+// 5: all softmax threads and both issuing warps, once per piece: its queries are in place.  6: the second group's share of a
+// piece is complete.  7: the first group has read it.  8: the whole block.  A softmax warp that has given up waiting meets the issuing
+// warp at 1-4 instead of only arriving, so that it cannot come round twice.
+__device__ __forceinline__ void rt_arrive(int wg, int which) {
+    const int id = 2 * wg + which;
+    if (id == 0) asm volatile("bar.arrive 1, 160;\n" ::: "memory");
+    else if (id == 1) asm volatile("bar.arrive 2, 160;\n" ::: "memory");
+    else if (id == 2) asm volatile("bar.arrive 3, 160;\n" ::: "memory");
+    else asm volatile("bar.arrive 4, 160;\n" ::: "memory");
+}
+__device__ __forceinline__ void rt_sync(int wg, int which) {
+    const int id = 2 * wg + which;
+    if (id == 0) asm volatile("bar.sync 1, 160;\n" ::: "memory");
+    else if (id == 1) asm volatile("bar.sync 2, 160;\n" ::: "memory");
+    else if (id == 2) asm volatile("bar.sync 3, 160;\n" ::: "memory");
+    else asm volatile("bar.sync 4, 160;\n" ::: "memory");
+}
+__device__ __forceinline__ void rt_piece_sync() { asm volatile("bar.sync 5, 320;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_share_arrive() { asm volatile("bar.arrive 6, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_share_sync() { asm volatile("bar.sync 6, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_taken_arrive() { asm volatile("bar.arrive 7, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_taken_sync() { asm volatile("bar.sync 7, 256;\n" ::: "memory"); }
+
+// the keys of a piece: tiles of 64 from k0 on, below k_end
+struct RtKeys { int k0, k_end, n; };
+__device__ __forceinline__ RtKeys rt_keys(const RowPiece& p) {
+    RtKeys k;
+    k.k0 = (p.t.key_lo & ~(AR_CHUNK - 1)) + p.chunk0 * AR_CHUNK;
+    k.k_end = min(k.k0 + p.chunks * AR_CHUNK, p.t.key_hi);
+    k.n = (k.k_end - k.k0 + TC_BN - 1) / TC_BN;
+    return k;
+}
+__device__ __forceinline__ int rt_share(int n, int wg) { return (n - wg + 1) >> 1; }    // tiles of a group
+
+// what the softmax threads need to know of a tile, beside S
+struct RtMeta {
+    float ks[RT_META][TC_BN], vs[RT_META][TC_BN];
+    float vmax[RT_META][4];              // the largest value scale of each bringing warp's rows
+    int hole[RT_META][4];                // whether one of its keys has no page
+    unsigned char ok[RT_META][TC_BN];
+};
+
+// the line of tiles as a bringing warp sees it
+struct RtStream {
+    RowWalk walk;
+    RowPiece pc;
+    RtKeys keys;
+    const int* bt;
+    int i;
+    bool have;
+    __device__ __forceinline__ void piece(const RowArgs& a) {
+        have = walk.next(a.plan, pc);
+        i = 0;
+        if (!have) return;
+        keys = rt_keys(pc);
+        const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
+        bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
+    }
+};
+
+template <int FORM, int DP>
+__global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const RowArgs a) {
+    constexpr bool HALF = FORM != C8_BF16;
+    constexpr int DB = DP / 64;                                        // blocks of 64 dimensions
+    constexpr uint32_t Q_BLK = TC_BM * 128, KV_BLK = TC_BN * 128;      // bytes of a [rows][64] block
+    constexpr uint32_t Q_BUF = DB * Q_BLK, BUF = DB * KV_BLK;
+    constexpr uint32_t ALL_BYTES = 2 * Q_BUF + 8 * BUF;
+    constexpr int WG_COLS = 256, T_O = 64, T_P = 64 + DP;              // a group's columns: S, O, P
+    extern __shared__ unsigned char rt_raw[];
+    __shared__ __align__(16) RtMeta s_meta[2];
+    __shared__ float s_mrg[2][128];
+    // per group: S done, O done, "landed" for K0 K1 V0 V1, "free" for the same, and the scales of four tiles
+    __shared__ __align__(8) unsigned long long s_mbar[2][10 + RT_META];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_dead;
+    const uint32_t base = (tc_smem(rt_raw) + 1023u) & ~1023u;
+    const int tid = threadIdx.x, warp = tc_warp(), lane = tid & 31;
+    const int d = a.d, g = a.plan.group;
+    {
+        uint32_t dyn;
+        asm volatile("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
+        if (base + ALL_BYTES > tc_smem(rt_raw) + dyn) {
+            if (tid == 0) atomicExch(a.kv.status, 4);
+            return;
+        }
+    }
+    const uint32_t sQ = base;                                          // two query buffers
+    auto buf_of = [&](int wg, int which, int b) { return base + 2 * Q_BUF + (uint32_t)((wg * 2 + which) * 2 + b) * BUF; };
+    auto bar = [&](int wg, int i) { return tc_smem(&s_mbar[wg][i]); };
+    constexpr int M_S = 0, M_O = 1, M_FULL = 2, M_FREE = 6, M_META = 10;
+    if (tid == 0) {
+        for (int w = 0; w < 2; ++w) {
+            for (int k = 0; k < 10 + RT_META; ++k)
+                tc_mbar_init(bar(w, k), k >= M_META ? (HALF ? 8 : 4) : k >= M_FULL && k < M_FREE ? 4 : 1);
+        }
+        tc_mbar_init_fence();
+        s_dead = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem(&s_tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    ST_PDL_TRIGGER();
+    const uint32_t tmem = s_tmem;
+    volatile int* dead = &s_dead;
+    auto tile_addr = [](uint32_t tile, int r, int c) -> uint32_t { return tile + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_OTHER));
+        if (warp < 18) {
+            // ---- the warp that issues a group's products
+            const int wg = warp - 16;
+            const uint32_t t_wg = tmem + wg * WG_COLS;
+            constexpr uint32_t type = HALF ? 0u : (1u << 7) | (1u << 10);
+            constexpr uint32_t idesc_s = (1u << 4) | type | ((TC_BN / 8) << 17) | ((TC_BM / 16) << 24);
+            constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((DP / 8) << 17) | ((TC_BM / 16) << 24);
+            const uint64_t dk = tc_desc(buf_of(wg, 0, 0), 16, 1024), dv = tc_desc(buf_of(wg, 1, 0), KV_BLK, 1024);
+            const uint32_t mb_s = bar(wg, M_S), mb_o = bar(wg, M_O), mb_full = bar(wg, M_FULL), mb_free = bar(wg, M_FREE);
+            bool alive = true;
+            uint32_t n = 0;              // tiles of this group so far: buffer n & 1, phase (n >> 1) & 1
+            RowWalk walk;
+            walk.begin(a.plan, blockIdx.x);
+            RowPiece pc;
+            for (int k = 0; walk.next(a.plan, pc); ++k) {
+                const int mine = rt_share(rt_keys(pc).n, wg);
+                const uint64_t dq = tc_desc(sQ + (k & 1) * Q_BUF, 16, 1024);
+                auto issue_s = [&](uint32_t x) {
+                    const int b = x & 1;
+                    if (alive) alive = tc_wait_warp(mb_full + 8 * b, (x >> 1) & 1, dead);
+                    if (alive) {
+                        tc_fence_after_sync();
+                        if (tc_elect()) {
+#pragma unroll
+                            for (int kk = 0; kk < DP / 16; ++kk)
+                                tc_mma(t_wg, dq + (((kk >> 2) * Q_BLK + (kk & 3) * 32) >> 4),
+                                       dk + ((b * BUF + (kk >> 2) * KV_BLK + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+                            tc_commit(mb_s);
+                            tc_commit(mb_free + 8 * b);
+                        }
+                    }
+                    __syncwarp();
+                };
+                rt_piece_sync();
+                if (mine > 0) issue_s(n);
+                for (int i = 0; i < mine; ++i) {
+                    const uint32_t x = n + i;
+                    const int b = x & 1;
+                    rt_sync(wg, 0);      // S(i) is in the softmax threads' registers
+                    if (i + 1 < mine) issue_s(x + 1);
+                    rt_sync(wg, 1);      // P(i) is written, O += P V of tile i - 1 has completed
+                    if (alive) alive = tc_wait_warp(mb_full + 8 * (2 + b), (x >> 1) & 1, dead);
+                    if (alive) {
+                        tc_fence_after_sync();
+                        if (tc_elect()) {
+#pragma unroll
+                            for (int jj = 0; jj < TC_BN / 16; ++jj)
+                                tc_mma_ts(t_wg + T_O, t_wg + T_P + jj * 8, dv + ((b * BUF + jj * 2048) >> 4), idesc_o, i > 0 || jj > 0);
+                            tc_commit(mb_o);
+                            tc_commit(mb_free + 8 * (2 + b));
+                        }
+                    }
+                    __syncwarp();
+                }
+                n += mine;
+            }
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_OTHER));
+        // ---- four warps bring keys (which = 0), four bring values: two threads per row, half of its dimensions each
+        const int which = warp >= 12, p = (tid - 256) & 127, row = p >> 1, half = p & 1, w4 = p >> 5;
+        uint32_t n0 = 0, n1 = 0;         // tiles of each group so far
+        bool alive = true;
+        RtStream st;
+        st.walk.begin(a.plan, blockIdx.x);
+        st.piece(a);
+        // the next tile of the line: this thread's row of the pool (or none), and its flags
+        constexpr uint32_t NONE = 0xffffffffu;
+        uint32_t at = NONE;              // looked up a tile ahead of its loads
+        int flags = 0;                   // 1: there is a tile; 2: the group; 4: a key that a row may see has no page
+        auto look = [&]() {
+            at = NONE;
+            flags = 0;
+            if (!st.have) return;
+            const int key = st.keys.k0 + TC_BN * st.i + row;
+            flags = 1 | (st.i & 1) << 1;
+            if (key >= st.pc.t.key_lo && key < st.keys.k_end) {
+                const int page = a.kv.page(st.bt, key);
+                if (page >= 0) at = a.kv.row0(page, which, st.pc.head) + a.kv.offset(key, a.kv.page_index(key));
+                else flags |= 4;
+            }
+            if (++st.i >= st.keys.n) st.piece(a);
+        };
+        auto wait_free = [&](int wg) -> bool {
+            const uint32_t x = wg ? n1 : n0;
+            if (x >= 2) return tc_wait_warp(bar(wg, M_FREE + which * 2 + (x & 1)), ((x - 2) >> 1) & 1, dead);
+            return true;
+        };
+        // scales and marks of a tile, into the place of its turn.  RT_META places: the tile four before in this group has been
+        // read when this one's buffer is free, because S of the tile two before was issued after the softmax threads were done with
+        // the one before that.
+        auto meta = [&](int wg, float scale, int fl) {
+            RtMeta& m = s_meta[wg];
+            const int x = (wg ? n1 : n0) & (RT_META - 1);
+            if (which == 0) {
+                const bool hole = (fl & 4) != 0;
+                if (half == 0) {
+                    if (HALF) m.ks[x][row] = scale;
+                    m.ok[x][row] = hole ? 0 : 1;
+                }
+                const bool any = __any_sync(0xffffffffu, hole);
+                if (lane == 0) {
+                    m.hole[x][w4] = any;
+                    if (any) *a.kv.status = 1;
+                }
+            } else if (HALF) {
+                if (half == 0) m.vs[x][row] = scale;
+                float v = scale;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+                if (lane == 0) m.vmax[x][w4] = v;
+            }
+        };
+        auto landed = [&](int wg, uint32_t x) {
+            tc_fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                rt_mbar_arrive(bar(wg, M_FULL + which * 2 + (x & 1)));
+                if (HALF || which == 0) rt_mbar_arrive(bar(wg, M_META + (x & (RT_META - 1))));
+            }
+        };
+        if constexpr (HALF) {
+            constexpr int NB = DP / 32;                  // 16-byte pieces of a half row
+            constexpr int DEPTH = 8 / NB;                // tiles under way: 32 registers
+            uint4 data[DEPTH][NB];
+            float scale[DEPTH];
+            int fl[DEPTH];
+            auto fill = [&](int s) {                     // loads of the tile looked up before, and the next look
+                fl[s] = flags;
+                scale[s] = at != NONE ? __ldg(a.kv.scales + at) : 0.f;
+                const unsigned char* src = a.kv.pool + (size_t)(at != NONE ? at : 0u) * d + half * (DP / 2);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    data[s][i] = at != NONE && half * (DP / 2) + 16 * i < d ? __ldg(reinterpret_cast<const uint4*>(src + 16 * i))
+                                                                              : make_uint4(0u, 0u, 0u, 0u);
+                if (flags) look();
+            };
+            look();
+#pragma unroll
+            for (int s = 0; s < DEPTH; ++s) fill(s);
+            while (alive) {
+#pragma unroll
+                for (int s = 0; s < DEPTH; ++s) {
+                    if (!(fl[s] & 1)) { alive = false; break; }
+                    const int wg = (fl[s] >> 1) & 1;
+                    if (!wait_free(wg)) { alive = false; break; }
+                    const uint32_t x = wg ? n1 : n0;
+                    const uint32_t buf = buf_of(wg, which, x & 1);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        const uint32_t c[4] = {data[s][i].x, data[s][i].y, data[s][i].z, data[s][i].w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) c8_halves<FORM>(c[k], h[2 * k], h[2 * k + 1]);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int ch = half * (DP / 16) + 2 * i + k;       // eight dimensions each
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                         ::"r"(tile_addr(buf + (ch >> 3) * KV_BLK, row, ch)), "r"(h[4 * k]), "r"(h[4 * k + 1]), "r"(h[4 * k + 2]),
+                                           "r"(h[4 * k + 3]) : "memory");
+                        }
+                    }
+                    meta(wg, scale[s], fl[s]);
+                    landed(wg, x);
+                    (wg ? n1 : n0) += 1;
+                    fill(s);
+                }
+            }
+        } else {
+            // copies of a tile are asked for as soon as its buffer is free; the tile before is announced when its own have landed
+            int before = -1;
+            uint32_t before_x = 0;
+            look();
+            while (alive && (flags & 1)) {
+                const int wg = (flags >> 1) & 1;
+                if (!wait_free(wg)) { alive = false; break; }
+                const uint32_t x = wg ? n1 : n0, buf = buf_of(wg, which, x & 1);
+                const unsigned char* src = a.kv.pool + ((size_t)(at != NONE ? at : 0u) * d + half * (DP / 2)) * 2;
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    const int ch = half * (DP / 16) + i;
+                    const bool in = at != NONE && ch * 8 < d;
+                    tc_cp16(tile_addr(buf + (ch >> 3) * KV_BLK, row, ch), in ? src + 16 * i : a.kv.pool, in);
+                }
+                tc_cp_commit();
+                meta(wg, 0.f, flags);
+                (wg ? n1 : n0) += 1;
+                look();
+                if (before >= 0) {
+                    tc_cp_wait<1>();
+                    landed(before, before_x);
+                }
+                before = wg;
+                before_x = x;
+            }
+            tc_cp_wait<0>();
+            if (alive && before >= 0) landed(before, before_x);
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_SOFTMAX));
+        // ---- softmax threads: thread `row` of a group has query row `row`, a lane of tensor memory
+        const int wg = warp >> 2, row = tid & 127, warp4 = warp & 3;
+        const uint32_t t_wg = tmem + wg * WG_COLS + ((uint32_t)(warp4 * 32) << 16);
+        const uint32_t mb_s = bar(wg, M_S), mb_o = bar(wg, M_O), mb_meta = bar(wg, M_META);
+        const RtMeta& meta = s_meta[wg];
+        bool alive = true;
+        uint32_t n = 0;                                  // tiles of this group so far
+        RowWalk walk;
+        walk.begin(a.plan, blockIdx.x);
+        RowPiece pc;
+        int k = 0;
+        for (; walk.next(a.plan, pc); ++k) {
+            const RtKeys keys = rt_keys(pc);
+            const int mine = rt_share(keys.n, wg), rows = pc.t.n_tok * g;
+            const int place = pc.t.first + row / g;
+            const int token = row < rows ? (a.plan.items ? a.plan.items[place] : place) : -1;
+            const int pos = token >= 0 ? a.positions[token] : -1;
+            const int head = pc.head * g + row % g;
+            float fac = a.scale_log2;
+            // ---- this piece's queries: the other buffer may still be read by the group that is behind.  A thread brings half a
+            // row, the groups a half each; the power of two comes from the whole row, alike in both.
+            {
+                const bf16* q = (const bf16*)a.q + (size_t)(pos >= 0 ? token : 0) * a.q_stride + (size_t)(pos >= 0 ? head : 0) * d;
+                float mul = 1.f;
+                if (HALF) {
+                    uint32_t amax = 0;
+                    if (pos >= 0)
+                        for (int c = 0; c < d; c += 8) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(q + c);
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                        }
+                    const int ex = min(max((int)(amax >> 7) - 127, -100), 127);
+                    mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+                    fac = ldexpf(a.scale_log2, ex - 14);
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    const int ch = wg * (DP / 16) + i;
+                    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                    if (pos >= 0 && ch * 8 < d) {
+                        u = *reinterpret_cast<const uint4*>(q + ch * 8);
+                        if (HALF) {
+                            uint32_t* w = &u.x;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * mul, __uint_as_float(w[j] & 0xffff0000u) * mul);
+                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                 ::"r"(tile_addr(sQ + (k & 1) * Q_BUF + (ch >> 3) * Q_BLK, row, ch)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+                }
+            }
+            tc_fence_async_smem();
+            tc_fence_before_sync();
+            __syncwarp();
+            rt_piece_sync();
+            if (wg == 1 && k > 0) rt_taken_sync();       // the first group has read this one's O of the piece before
+            const int hi = min(pos + 1, keys.k_end);
+            const int lo = max(pc.t.key_lo, a.window > 0 ? pos - a.window + 1 : 0);
+            float ref = -INFINITY, sum = 0.f;
+            for (int i = 0; i < mine; ++i) {
+                const uint32_t x = n + i;
+                const int key0 = keys.k0 + TC_BN * (wg + 2 * i), mt = x & (RT_META - 1);
+                if (alive) alive = tc_wait_warp(mb_s, x & 1, dead);
+                tc_fence_after_sync();
+                float s[TC_BN];
+                tc_ld32(t_wg, s);
+                tc_ld32(t_wg + 32, s + 32);
+                if (alive) alive = tc_wait_warp(mb_meta + 8 * mt, (x / RT_META) & 1, dead);
+                tc_ld_wait();
+                tc_fence_before_sync();
+                if (alive) rt_arrive(wg, 0);
+                else rt_sync(wg, 0);
+                float lead = 0.f;
+                if (HALF) {
+#pragma unroll
+                    for (int c = 0; c < TC_BN; c += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&meta.ks[mt][c]);
+                        s[c] *= f.x; s[c + 1] *= f.y; s[c + 2] *= f.z; s[c + 3] *= f.w;
+                    }
+                    const float4 f = *reinterpret_cast<const float4*>(meta.vmax[mt]);
+                    const float vmax = fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w));
+                    lead = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -90);
+                }
+                const bool edge = key0 + TC_BN > hi || key0 < lo;        // this row does not see all of the tile's keys
+                if (edge) {
+#pragma unroll
+                    for (int c = 0; c < TC_BN; ++c)
+                        if (key0 + c >= hi || key0 + c < lo) s[c] = -INFINITY;
+                }
+                {
+                    const int4 f = *reinterpret_cast<const int4*>(meta.hole[mt]);
+                    if (f.x | f.y | f.z | f.w) {
+#pragma unroll
+                        for (int c = 0; c < TC_BN; ++c)
+                            if (!meta.ok[mt][c]) s[c] = -INFINITY;
+                    }
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < TC_BN; c += 8) {
+                    mx4[0] = tc_max3(mx4[0], s[c], s[c + 1]); mx4[1] = tc_max3(mx4[1], s[c + 2], s[c + 3]);
+                    mx4[2] = tc_max3(mx4[2], s[c + 4], s[c + 5]); mx4[3] = tc_max3(mx4[3], s[c + 6], s[c + 7]);
+                }
+                float need = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), fac, lead);
+                if (HALF && edge) {
+                    // key by key: the scale of a key that the row does not see has no part in its unit
+                    need = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < TC_BN; ++c)
+                        need = fmaxf(need, fmaf(s[c], fac, (float)max((int)(__float_as_uint(meta.vs[mt][c]) >> 23) - 126, -90)));
+                }
+                // the reference moves when p vs could pass 2^15 (or from "no key yet"), and then to 11 below the largest
+                const bool move = need > ref + 15.f;
+                const float old = ref;
+                if (move) ref = need - 11.f;
+                const float neg = ref == -INFINITY ? 0.f : -ref;
+                float rs[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                uint32_t w[TC_BN / 2];
+#pragma unroll
+                for (int c = 0; c < TC_BN; c += 4) {
+                    float p[4];
+                    tc_fma2(p[0], p[1], s[c], s[c + 1], fac, neg);
+                    tc_fma2(p[2], p[3], s[c + 2], s[c + 3], fac, neg);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = tc_exp2(p[j]);
+                    tc_add2(rs[c & 4], rs[(c & 4) + 1], p[0], p[1]);
+                    tc_add2(rs[(c & 4) + 2], rs[(c & 4) + 3], p[2], p[3]);
+                    if (HALF) {
+                        // (a value row that is not finite has the scale NaN: hidden, its weight stays zero)
+                        const float4 f = *reinterpret_cast<const float4*>(&meta.vs[mt][c]);
+                        p[0] = p[0] == 0.f ? 0.f : p[0] * f.x; p[1] = p[1] == 0.f ? 0.f : p[1] * f.y;
+                        p[2] = p[2] == 0.f ? 0.f : p[2] * f.z; p[3] = p[3] == 0.f ? 0.f : p[3] * f.w;
+                        const __half2 h0 = __floats2half2_rn(p[0], p[1]), h1 = __floats2half2_rn(p[2], p[3]);
+                        w[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+                        w[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                    } else {
+                        const __nv_bfloat162 h0 = __floats2bfloat162_rn(p[0], p[1]), h1 = __floats2bfloat162_rn(p[2], p[3]);
+                        w[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+                        w[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                    }
+                }
+                if (i > 0) {                             // O += P V of tile i - 1: O may be scaled and P overwritten after it
+                    if (alive) alive = tc_wait_warp(mb_o, (x - 1) & 1, dead);
+                    tc_fence_after_sync();
+                }
+                if (__any_sync(0xffffffffu, move) && i > 0) {
+                    const float corr = move ? tc_exp2(old - ref) : 1.f;
+#pragma unroll
+                    for (int cb = 0; cb < DP / 32; ++cb) {
+                        float ov[32];
+                        tc_ld32(t_wg + T_O + cb * 32, ov);
+                        tc_ld_wait();
+#pragma unroll
+                        for (int kk = 0; kk < 32; ++kk) ov[kk] *= corr;
+                        tc_st32(t_wg + T_O + cb * 32, ov);
+                    }
+                    tc_st_wait();
+                    sum *= corr;
+                }
+                tc_st32(t_wg + T_P, reinterpret_cast<const float*>(w));
+                sum += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
+                tc_st_wait();
+                tc_fence_before_sync();
+                if (alive) rt_arrive(wg, 1);
+                else rt_sync(wg, 1);
+            }
+            if (mine > 0) {
+                if (alive) alive = tc_wait_warp(mb_o, (n + mine - 1) & 1, dead);
+                tc_fence_after_sync();
+            }
+            n += mine;
+            // ---- the groups' sums
+            if (wg == 1) {
+                s_mrg[0][row] = mine > 0 ? ref : -INFINITY;
+                s_mrg[1][row] = sum;
+                tc_fence_before_sync();
+                rt_share_arrive();
+            } else {
+                rt_share_sync();
+                tc_fence_after_sync();
+                const bool two = keys.n > 1;             // the second group has tiles
+                const float r1 = s_mrg[0][row], m = fmaxf(ref, r1);
+                const float a0 = ar_weight(ref, m), a1 = ar_weight(r1, m);
+                const float l = sum * a0 + s_mrg[1][row] * a1;
+                const bool direct = a.direct && pc.whole, mine_to_store = row < rows && pos >= 0 && alive;
+                const size_t slot = ((size_t)(pc.unit + blockIdx.x)) * AR_ROWS + row;
+                if (!direct && row < rows) { a.parts.r[slot] = m; a.parts.l[slot] = l; }
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                bf16* out = (bf16*)a.out + ((size_t)(token >= 0 ? token : 0) * a.plan.nh + head) * d;
+                float* part = a.parts.o + slot * d;
+#pragma unroll
+                for (int cb = 0; cb < DP / 16; ++cb) {
+                    float o[16], o1[16];
+                    uint32_t* r0 = reinterpret_cast<uint32_t*>(o);
+                    uint32_t* r1p = reinterpret_cast<uint32_t*>(o1);
+                    const uint32_t t0 = t_wg + T_O + cb * 16, t1 = t0 + WG_COLS;
+#define RT_LD16(r, t)                                                                                                              \
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"         \
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),     \
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(t) : "memory")
+                    __syncwarp();
+                    RT_LD16(r0, t0);
+                    if (two) RT_LD16(r1p, t1);
+                    tc_ld_wait();
+                    if (cb * 16 >= d) continue;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = o[e] * a0 + (two ? o1[e] * a1 : 0.f);
+                    if (mine_to_store && direct) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 8) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 b = __floats2bfloat162_rn(o[e + 2 * j] * inv, o[e + 2 * j + 1] * inv);
+                                h[j] = *reinterpret_cast<const uint32_t*>(&b);
+                            }
+                            *reinterpret_cast<uint4*>(out + cb * 16 + e) = make_uint4(h[0], h[1], h[2], h[3]);
+                        }
+                    } else if (mine_to_store) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) store4(part + cb * 16 + e, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                    }
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                rt_taken_arrive();
+            }
+        }
+        if (wg == 1 && k > 0) rt_taken_sync();
+    }
+    tc_fence_before_sync();
+    asm volatile("bar.sync 8, %0;\n" ::"n"(RT_THREADS) : "memory");
+    if (s_dead && tid == 0) atomicExch(a.kv.status, 3);
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <int FORM, int DP> static int rt_run(const RowArgs& a, cudaStream_t s) {
+    constexpr size_t smem = 2 * (DP / 64) * TC_BM * 128 + 8 * (DP / 64) * TC_BN * 128 + 1024;
+    auto kernel = attention_rows_tc_kernel<FORM, DP>;
+    AR_ALLOW_SMEM(kernel, smem);
+    // the redistribution of registers moves what the launch got, and waits for more for ever: only for a kernel compiled as assumed
+    static int regs[64] = {0};
+    int& have = regs[ar_device()];
+    if (!have) {
+        cudaFuncAttributes attr;
+        const cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+        if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+        have = attr.numRegs;
+    }
+    if (have * RT_THREADS < 256 * RT_REGS_SOFTMAX + 384 * RT_REGS_OTHER) return ST_ERR_TOO_LARGE;
+    kernel<<<a.plan.ctas, RT_THREADS, smem, s>>>(a);
+    return st_launch_status();
+}
+
+int ar_rows_tc(const RowArgs& a, int form, cudaStream_t s) {
+    if (form == C8_INT8) return a.d <= 64 ? rt_run<C8_INT8, 64>(a, s) : rt_run<C8_INT8, 128>(a, s);
+    if (form == C8_E4M3) return a.d <= 64 ? rt_run<C8_E4M3, 64>(a, s) : rt_run<C8_E4M3, 128>(a, s);
+    return a.d <= 64 ? rt_run<C8_BF16, 64>(a, s) : rt_run<C8_BF16, 128>(a, s);
+}
