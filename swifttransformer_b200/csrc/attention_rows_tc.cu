@@ -25,7 +25,7 @@
 #include "attention_rows.cuh"
 #include "tcgen05.cuh"
 
-#define RT_THREADS 640                   // 8 softmax warps, 4 for keys, 4 for values, 2 issuing products, 2 to fill the last four
+#define RT_THREADS 640                   // 8 softmax warps, 4 for keys, 4 for values, 2 issuing products, 2 for queries
 // Registers a thread keeps after the block has shared them out anew; the sum must not pass what the launch got, 640 x 96.
 #define RT_REGS_SOFTMAX 144
 #define RT_REGS_OTHER 64
@@ -36,8 +36,7 @@ __device__ __forceinline__ void rt_mbar_arrive(uint32_t mbar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(mbar) : "memory");
 }
 // Named barriers.  1-4: a softmax group and the warp that issues its products (160 threads): 0 "S has been read", 1 "P has been written".
-// 5: all softmax threads and both issuing warps, once per piece: its queries are in place.  6: the second group's share of a
-// piece is complete.  7: the first group has read it.  8: the whole block.  A softmax warp that has given up waiting meets the issuing
+// 5: the second group's share of a piece is complete.  6: the first group has read it.  7: the whole block.  A softmax warp that has given up waiting meets the issuing
 // warp at 1-4 instead of only arriving, so that it cannot come round twice.
 __device__ __forceinline__ void rt_arrive(int wg, int which) {
     const int id = 2 * wg + which;
@@ -53,11 +52,25 @@ __device__ __forceinline__ void rt_sync(int wg, int which) {
     else if (id == 2) asm volatile("bar.sync 3, 160;\n" ::: "memory");
     else asm volatile("bar.sync 4, 160;\n" ::: "memory");
 }
-__device__ __forceinline__ void rt_piece_sync() { asm volatile("bar.sync 5, 320;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_share_arrive() { asm volatile("bar.arrive 6, 256;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_share_sync() { asm volatile("bar.sync 6, 256;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_taken_arrive() { asm volatile("bar.arrive 7, 256;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_taken_sync() { asm volatile("bar.sync 7, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_share_arrive() { asm volatile("bar.arrive 5, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_share_sync() { asm volatile("bar.sync 5, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_taken_arrive() { asm volatile("bar.arrive 6, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void rt_taken_sync() { asm volatile("bar.sync 6, 256;\n" ::: "memory"); }
+
+__device__ __forceinline__ void rt_mul2(float& d0, float& d1, float b0, float b1) {       // d *= b
+    asm("{\n\t.reg .b64 b, d;\n\tmov.b64 b, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\tmul.rn.f32x2 d, d, b;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
+        : "+f"(d0), "+f"(d1) : "f"(b0), "f"(b1));
+}
+// what the softmax threads need to know of a row
+struct RtRows {
+    int pos[AR_ROWS], token[AR_ROWS];
+    float fac[AR_ROWS];
+};
+// bits lo .. hi - 1 of a word
+__device__ __forceinline__ uint32_t rt_bits(int lo, int hi) {
+    const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1;
+    return lo <= 0 ? below : lo >= 32 ? 0u : below & (0xffffffffu << lo);
+}
 
 // the keys of a piece: tiles of 64 from k0 on, below k_end
 struct RtKeys { int k0, k_end, n; };
@@ -73,27 +86,8 @@ __device__ __forceinline__ int rt_share(int n, int wg) { return (n - wg + 1) >> 
 // what the softmax threads need to know of a tile, beside S
 struct RtMeta {
     float ks[RT_META][TC_BN], vs[RT_META][TC_BN];
-    float vmax[RT_META][4];              // the largest value scale of each bringing warp's rows
-    int hole[RT_META][4];                // whether one of its keys has no page
-    unsigned char ok[RT_META][TC_BN];
-};
-
-// the line of tiles as a bringing warp sees it
-struct RtStream {
-    RowWalk walk;
-    RowPiece pc;
-    RtKeys keys;
-    const int* bt;
-    int i;
-    bool have;
-    __device__ __forceinline__ void piece(const RowArgs& a) {
-        have = walk.next(a.plan, pc);
-        i = 0;
-        if (!have) return;
-        keys = rt_keys(pc);
-        const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
-        bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
-    }
+    float vmax[RT_META][2];              // the largest value scale of each half of the keys
+    uint32_t seen[RT_META][2];           // bit c: key c of that half is one of the tile's and has a page
 };
 
 template <int FORM, int DP>
@@ -106,11 +100,14 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     constexpr int WG_COLS = 256, T_O = 64, T_P = 64 + DP;              // a group's columns: S, O, P
     extern __shared__ unsigned char rt_raw[];
     __shared__ __align__(16) RtMeta s_meta[2];
+    __shared__ RtRows s_rows[2];
     __shared__ float s_mrg[2][128];
-    // per group: S done, O done, "landed" for K0 K1 V0 V1, "free" for the same, and the scales of four tiles
-    __shared__ __align__(8) unsigned long long s_mbar[2][10 + RT_META];
+    // per group: S done, O done, "landed" for K0 K1 V0 V1, "free" for the same, and the scales of four tiles; of the two
+    // query buffers: "landed" and "free"
+    __shared__ __align__(8) unsigned long long s_mbar[2][10 + RT_META], s_qbar[2][2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
+    __shared__ RowWalk s_walk;
     const uint32_t base = (tc_smem(rt_raw) + 1023u) & ~1023u;
     const int tid = threadIdx.x, warp = tc_warp(), lane = tid & 31;
     const int d = a.d, g = a.plan.group;
@@ -129,11 +126,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     if (tid == 0) {
         for (int w = 0; w < 2; ++w) {
             for (int k = 0; k < 10 + RT_META; ++k)
-                tc_mbar_init(bar(w, k), k >= M_META ? (HALF ? 8 : 4) : k >= M_FULL && k < M_FREE ? 4 : 1);
+                tc_mbar_init(bar(w, k), k >= M_META ? (HALF ? 4 : 2) : k >= M_FULL && k < M_FREE ? 2 : 1);
+        }
+        for (int k = 0; k < 2; ++k) {
+            tc_mbar_init(tc_smem(&s_qbar[0][k]), 2);           // both bringing warps
+            tc_mbar_init(tc_smem(&s_qbar[1][k]), 2 + 8);       // both groups' last S, all softmax warps
         }
         tc_mbar_init_fence();
         s_dead = 0;
     }
+    if (tid == 32) s_walk.begin(a.plan, blockIdx.x);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -159,13 +161,12 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             const uint32_t mb_s = bar(wg, M_S), mb_o = bar(wg, M_O), mb_full = bar(wg, M_FULL), mb_free = bar(wg, M_FREE);
             bool alive = true;
             uint32_t n = 0;              // tiles of this group so far: buffer n & 1, phase (n >> 1) & 1
-            RowWalk walk;
-            walk.begin(a.plan, blockIdx.x);
+            RowWalk walk = s_walk;
             RowPiece pc;
             for (int k = 0; walk.next(a.plan, pc); ++k) {
                 const int mine = rt_share(rt_keys(pc).n, wg);
                 const uint64_t dq = tc_desc(sQ + (k & 1) * Q_BUF, 16, 1024);
-                auto issue_s = [&](uint32_t x) {
+                auto issue_s = [&](uint32_t x, bool last) {
                     const int b = x & 1;
                     if (alive) alive = tc_wait_warp(mb_full + 8 * b, (x >> 1) & 1, dead);
                     if (alive) {
@@ -177,17 +178,19 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                                        dk + ((b * BUF + (kk >> 2) * KV_BLK + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
                             tc_commit(mb_s);
                             tc_commit(mb_free + 8 * b);
+                            if (last) tc_commit(tc_smem(&s_qbar[1][k & 1]));
                         }
                     }
                     __syncwarp();
                 };
-                rt_piece_sync();
-                if (mine > 0) issue_s(n);
+                if (alive) alive = tc_wait_warp(tc_smem(&s_qbar[0][k & 1]), (k >> 1) & 1, dead);
+                if (mine > 0) issue_s(n, mine == 1);
+                else if (lane == 0) rt_mbar_arrive(tc_smem(&s_qbar[1][k & 1]));
                 for (int i = 0; i < mine; ++i) {
                     const uint32_t x = n + i;
                     const int b = x & 1;
                     rt_sync(wg, 0);      // S(i) is in the softmax threads' registers
-                    if (i + 1 < mine) issue_s(x + 1);
+                    if (i + 1 < mine) issue_s(x + 1, i + 2 == mine);
                     rt_sync(wg, 1);      // P(i) is written, O += P V of tile i - 1 has completed
                     if (alive) alive = tc_wait_warp(mb_full + 8 * (2 + b), (x >> 1) & 1, dead);
                     if (alive) {
@@ -204,147 +207,181 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                 }
                 n += mine;
             }
+        } else {
+            // ---- two warps bring the queries, a piece ahead: a thread has two rows
+            RowWalk walk = s_walk;
+            RowPiece pc;
+            for (int k = 0; walk.next(a.plan, pc); ++k) {
+                if (k >= 2 && !tc_wait_warp(tc_smem(&s_qbar[1][k & 1]), ((k - 2) >> 1) & 1, dead)) break;
+                const int rows = pc.t.n_tok * g;
+#pragma unroll 1
+                for (int row = (warp - 18) * 32 + lane; row < AR_ROWS; row += 64) {
+                    const int place = pc.t.first + row / g;
+                    const int token = row < rows ? (a.plan.items ? a.plan.items[place] : place) : -1;
+                    const int pos = token >= 0 ? a.positions[token] : -1;
+                    const bf16* q = (const bf16*)a.q + (size_t)(pos >= 0 ? token : 0) * a.q_stride + (size_t)(pos >= 0 ? pc.head * g + row % g : 0) * d;
+                    float mul = 1.f, fac = a.scale_log2;
+                    if (HALF) {
+                        // a power of two that brings the row's largest element to [2^14, 2^15)
+                        uint32_t amax = 0;
+#pragma unroll
+                        for (int c = 0; c < DP / 8; ++c) {
+                            if (pos < 0 || 8 * c >= d) continue;
+                            const uint4 u = __ldg(reinterpret_cast<const uint4*>(q) + c);
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                        }
+                        const int ex = min(max((int)(amax >> 7) - 127, -100), 127);
+                        mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+                        fac = ldexpf(a.scale_log2, ex - 14);
+                    }
+                    const uint32_t dst = sQ + (k & 1) * Q_BUF + row * 128, swz = (uint32_t)(row & 7) << 4;
+#pragma unroll
+                    for (int c = 0; c < DP / 8; ++c) {
+                        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                        if (pos >= 0 && 8 * c < d) u = __ldg(reinterpret_cast<const uint4*>(q) + c);
+                        if (HALF) {
+                            uint32_t* w = &u.x;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * mul, __uint_as_float(w[j] & 0xffff0000u) * mul);
+                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                     ::"r"(dst + (c >> 3) * Q_BLK + (((uint32_t)(c & 7) << 4) ^ swz)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+                    }
+                    s_rows[k & 1].pos[row] = pos;
+                    s_rows[k & 1].token[row] = token;
+                    s_rows[k & 1].fac[row] = fac;
+                }
+                tc_fence_async_smem();
+                __syncwarp();
+                if (lane == 0) rt_mbar_arrive(tc_smem(&s_qbar[0][k & 1]));
+            }
         }
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_OTHER));
-        // ---- four warps bring keys (which = 0), four bring values: two threads per row, half of its dimensions each
-        const int which = warp >= 12, p = (tid - 256) & 127, row = p >> 1, half = p & 1, w4 = p >> 5;
-        uint32_t n0 = 0, n1 = 0;         // tiles of each group so far
-        bool alive = true;
-        RtStream st;
-        st.walk.begin(a.plan, blockIdx.x);
-        st.piece(a);
-        // the next tile of the line: this thread's row of the pool (or none), and its flags
+        // ---- two warps per group bring its keys (which = 0), two its values: a thread per row
+        const int w8 = warp - 8, wg = w8 & 1, which = (w8 >> 1) & 1, half = w8 >> 2, row = half * 32 + lane;
+        const uint32_t mb_full = bar(wg, M_FULL + which * 2), mb_free = bar(wg, M_FREE + which * 2), mb_meta = bar(wg, M_META);
+        const uint32_t buf0 = buf_of(wg, which, 0) + row * 128, swz = (uint32_t)(row & 7) << 4;
+        RtMeta& meta = s_meta[wg];
         constexpr uint32_t NONE = 0xffffffffu;
-        uint32_t at = NONE;              // looked up a tile ahead of its loads
-        int flags = 0;                   // 1: there is a tile; 2: the group; 4: a key that a row may see has no page
+        const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
+        uint32_t n = 0;                  // this group's tiles so far
+        RowWalk walk = s_walk;
+        RowPiece pc;
+        RtKeys keys;
+        keys.n = 0;
+        const int* bt = nullptr;
+        int i = wg;                      // the next tile of the piece
+        bool have = true;
+        uint32_t at = NONE;              // its keys' row of this thread, looked up a tile ahead of the loads
+        bool hole = false;               // a key that a row may see has no page
         auto look = [&]() {
+            while (i >= keys.n) {
+                if (!walk.next(a.plan, pc)) { have = false; return; }
+                keys = rt_keys(pc);
+                const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
+                bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
+                i = wg;
+            }
+            const int key = keys.k0 + TC_BN * i + row;
             at = NONE;
-            flags = 0;
-            if (!st.have) return;
-            const int key = st.keys.k0 + TC_BN * st.i + row;
-            flags = 1 | (st.i & 1) << 1;
-            if (key >= st.pc.t.key_lo && key < st.keys.k_end) {
-                const int page = a.kv.page(st.bt, key);
-                if (page >= 0) at = a.kv.row0(page, which, st.pc.head) + a.kv.offset(key, a.kv.page_index(key));
-                else flags |= 4;
+            hole = false;
+            if (key >= pc.t.key_lo && key < keys.k_end) {
+                const int index = a.kv.page_index(key);
+                const int page = index < a.kv.max_pages ? __ldg(bt + index) : -1;
+                hole = (unsigned)page >= (unsigned)a.kv.num_pages;
+                if (!hole) at = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, index);
             }
-            if (++st.i >= st.keys.n) st.piece(a);
+            i += 2;
         };
-        auto wait_free = [&](int wg) -> bool {
-            const uint32_t x = wg ? n1 : n0;
-            if (x >= 2) return tc_wait_warp(bar(wg, M_FREE + which * 2 + (x & 1)), ((x - 2) >> 1) & 1, dead);
-            return true;
-        };
-        // scales and marks of a tile, into the place of its turn.  RT_META places: the tile four before in this group has been
-        // read when this one's buffer is free, because S of the tile two before was issued after the softmax threads were done with
-        // the one before that.
-        auto meta = [&](int wg, float scale, int fl) {
-            RtMeta& m = s_meta[wg];
-            const int x = (wg ? n1 : n0) & (RT_META - 1);
+        // Scales and marks of a tile, into the place of its turn.  RT_META places: the tile four before has been read when this one's
+        // buffer is free, because S of the tile two before was issued after the softmax threads were done with the one before that.
+        auto put_meta = [&](float ks, float vs, uint32_t row_at, bool no_page) {
+            const int x = n & (RT_META - 1);
             if (which == 0) {
-                const bool hole = (fl & 4) != 0;
-                if (half == 0) {
-                    if (HALF) m.ks[x][row] = scale;
-                    m.ok[x][row] = hole ? 0 : 1;
-                }
-                const bool any = __any_sync(0xffffffffu, hole);
-                if (lane == 0) {
-                    m.hole[x][w4] = any;
-                    if (any) *a.kv.status = 1;
-                }
+                // (a value row that is not finite has the scale NaN: with the key's it reaches those who see the key and nobody else)
+                if (HALF) meta.ks[x][row] = isnan(vs) ? vs : ks;
+                const uint32_t seen = __ballot_sync(0xffffffffu, row_at != NONE);
+                if (lane == 0) meta.seen[x][half] = seen;
+                if (no_page) *a.kv.status = 1;
             } else if (HALF) {
-                if (half == 0) m.vs[x][row] = scale;
-                float v = scale;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-                if (lane == 0) m.vmax[x][w4] = v;
+                vs = isnan(vs) ? 0.f : vs;
+                meta.vs[x][row] = vs;
+                const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(vs));
+                if (lane == 0) meta.vmax[x][half] = __uint_as_float(most);
             }
         };
-        auto landed = [&](int wg, uint32_t x) {
+        auto landed = [&](uint32_t x) {
             tc_fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-                rt_mbar_arrive(bar(wg, M_FULL + which * 2 + (x & 1)));
-                if (HALF || which == 0) rt_mbar_arrive(bar(wg, M_META + (x & (RT_META - 1))));
+                rt_mbar_arrive(mb_full + 8 * (x & 1));
+                if (HALF || which == 0) rt_mbar_arrive(mb_meta + 8 * (x & (RT_META - 1)));
             }
         };
+        auto wait_free = [&]() -> bool { return n < 2 || tc_wait_warp(mb_free + 8 * (n & 1), ((n - 2) >> 1) & 1, dead); };
+        look();
         if constexpr (HALF) {
-            constexpr int NB = DP / 32;                  // 16-byte pieces of a half row
-            constexpr int DEPTH = 8 / NB;                // tiles under way: 32 registers
-            uint4 data[DEPTH][NB];
-            float scale[DEPTH];
-            int fl[DEPTH];
-            auto fill = [&](int s) {                     // loads of the tile looked up before, and the next look
-                fl[s] = flags;
-                scale[s] = at != NONE ? __ldg(a.kv.scales + at) : 0.f;
-                const unsigned char* src = a.kv.pool + (size_t)(at != NONE ? at : 0u) * d + half * (DP / 2);
-#pragma unroll
-                for (int i = 0; i < NB; ++i)
-                    data[s][i] = at != NONE && half * (DP / 2) + 16 * i < d ? __ldg(reinterpret_cast<const uint4*>(src + 16 * i))
-                                                                              : make_uint4(0u, 0u, 0u, 0u);
-                if (flags) look();
-            };
-            look();
-#pragma unroll
-            for (int s = 0; s < DEPTH; ++s) fill(s);
-            while (alive) {
-#pragma unroll
-                for (int s = 0; s < DEPTH; ++s) {
-                    if (!(fl[s] & 1)) { alive = false; break; }
-                    const int wg = (fl[s] >> 1) & 1;
-                    if (!wait_free(wg)) { alive = false; break; }
-                    const uint32_t x = wg ? n1 : n0;
-                    const uint32_t buf = buf_of(wg, which, x & 1);
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        const uint32_t c[4] = {data[s][i].x, data[s][i].y, data[s][i].z, data[s][i].w};
-                        uint32_t h[8];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) c8_halves<FORM>(c[k], h[2 * k], h[2 * k + 1]);
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const int ch = half * (DP / 16) + 2 * i + k;       // eight dimensions each
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
-                                         ::"r"(tile_addr(buf + (ch >> 3) * KV_BLK, row, ch)), "r"(h[4 * k]), "r"(h[4 * k + 1]), "r"(h[4 * k + 2]),
-                                           "r"(h[4 * k + 3]) : "memory");
-                        }
-                    }
-                    meta(wg, scale[s], fl[s]);
-                    landed(wg, x);
-                    (wg ? n1 : n0) += 1;
-                    fill(s);
+            constexpr int NB = DP / 16;                  // 16-byte pieces of a row
+            while (have) {
+                uint4 data[NB];
+                const uint32_t mine = at;
+                const bool no_page = hole;
+                float ks = 0.f, vs = 0.f;
+                if (mine != NONE) {
+                    if (which == 0) ks = __ldg(a.kv.scales + mine);
+                    vs = __ldg(a.kv.scales + mine + to_values);
                 }
+                const unsigned char* src = a.kv.pool + (size_t)(mine != NONE ? mine + (which ? to_values : 0u) : 0u) * d;
+#pragma unroll
+                for (int k = 0; k < NB; ++k)
+                    data[k] = mine != NONE && 16 * k < d ? __ldg(reinterpret_cast<const uint4*>(src) + k) : make_uint4(0u, 0u, 0u, 0u);
+                look();
+                if (!wait_free()) break;
+                const uint32_t buf = buf0 + (n & 1) * BUF;
+#pragma unroll
+                for (int k = 0; k < NB; ++k) {
+                    uint32_t h[8];
+                    c8_halves<FORM>(data[k].x, h[0], h[1]);
+                    c8_halves<FORM>(data[k].y, h[2], h[3]);
+                    c8_halves<FORM>(data[k].z, h[4], h[5]);
+                    c8_halves<FORM>(data[k].w, h[6], h[7]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)              // eight dimensions each
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                     ::"r"(buf + (k >> 2) * KV_BLK + (((uint32_t)((2 * k + c) & 7) << 4) ^ swz)), "r"(h[4 * c]),
+                                       "r"(h[4 * c + 1]), "r"(h[4 * c + 2]), "r"(h[4 * c + 3]) : "memory");
+                }
+                put_meta(ks, vs, mine, no_page);
+                landed(n);
+                ++n;
             }
         } else {
             // copies of a tile are asked for as soon as its buffer is free; the tile before is announced when its own have landed
-            int before = -1;
-            uint32_t before_x = 0;
-            look();
-            while (alive && (flags & 1)) {
-                const int wg = (flags >> 1) & 1;
-                if (!wait_free(wg)) { alive = false; break; }
-                const uint32_t x = wg ? n1 : n0, buf = buf_of(wg, which, x & 1);
-                const unsigned char* src = a.kv.pool + ((size_t)(at != NONE ? at : 0u) * d + half * (DP / 2)) * 2;
+            bool alive = true;
+            while (have) {
+                if (!wait_free()) { alive = false; break; }
+                const uint32_t buf = buf0 + (n & 1) * BUF;
+                const unsigned char* src = a.kv.pool + (size_t)(at != NONE ? at + (which ? to_values : 0u) : 0u) * d * 2;
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    const int ch = half * (DP / 16) + i;
-                    const bool in = at != NONE && ch * 8 < d;
-                    tc_cp16(tile_addr(buf + (ch >> 3) * KV_BLK, row, ch), in ? src + 16 * i : a.kv.pool, in);
-                }
+                for (int k = 0; k < DP / 8; ++k)
+                    tc_cp16(buf + (k >> 3) * KV_BLK + (((uint32_t)(k & 7) << 4) ^ swz), 8 * k < d ? src + 16 * k : src, at != NONE && 8 * k < d);
                 tc_cp_commit();
-                meta(wg, 0.f, flags);
-                (wg ? n1 : n0) += 1;
+                put_meta(0.f, 0.f, at, hole);
+                ++n;
                 look();
-                if (before >= 0) {
+                if (n > 1) {
                     tc_cp_wait<1>();
-                    landed(before, before_x);
+                    landed(n - 2);
                 }
-                before = wg;
-                before_x = x;
             }
             tc_cp_wait<0>();
-            if (alive && before >= 0) landed(before, before_x);
+            if (alive && n > 0) landed(n - 1);
         }
         __syncwarp();
     } else {
@@ -356,59 +393,18 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         const RtMeta& meta = s_meta[wg];
         bool alive = true;
         uint32_t n = 0;                                  // tiles of this group so far
-        RowWalk walk;
-        walk.begin(a.plan, blockIdx.x);
+        RowWalk walk = s_walk;
         RowPiece pc;
         int k = 0;
         for (; walk.next(a.plan, pc); ++k) {
             const RtKeys keys = rt_keys(pc);
             const int mine = rt_share(keys.n, wg), rows = pc.t.n_tok * g;
-            const int place = pc.t.first + row / g;
-            const int token = row < rows ? (a.plan.items ? a.plan.items[place] : place) : -1;
-            const int pos = token >= 0 ? a.positions[token] : -1;
             const int head = pc.head * g + row % g;
-            float fac = a.scale_log2;
-            // ---- this piece's queries: the other buffer may still be read by the group that is behind.  A thread brings half a
-            // row, the groups a half each; the power of two comes from the whole row, alike in both.
-            {
-                const bf16* q = (const bf16*)a.q + (size_t)(pos >= 0 ? token : 0) * a.q_stride + (size_t)(pos >= 0 ? head : 0) * d;
-                float mul = 1.f;
-                if (HALF) {
-                    uint32_t amax = 0;
-                    if (pos >= 0)
-                        for (int c = 0; c < d; c += 8) {
-                            const uint4 u = *reinterpret_cast<const uint4*>(q + c);
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-                        }
-                    const int ex = min(max((int)(amax >> 7) - 127, -100), 127);
-                    mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-                    fac = ldexpf(a.scale_log2, ex - 14);
-                }
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    const int ch = wg * (DP / 16) + i;
-                    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                    if (pos >= 0 && ch * 8 < d) {
-                        u = *reinterpret_cast<const uint4*>(q + ch * 8);
-                        if (HALF) {
-                            uint32_t* w = &u.x;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * mul, __uint_as_float(w[j] & 0xffff0000u) * mul);
-                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
-                        }
-                    }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
-                                 ::"r"(tile_addr(sQ + (k & 1) * Q_BUF + (ch >> 3) * Q_BLK, row, ch)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
-                }
-            }
-            tc_fence_async_smem();
-            tc_fence_before_sync();
+            if (alive) alive = tc_wait_warp(tc_smem(&s_qbar[0][k & 1]), (k >> 1) & 1, dead);
+            const int pos = s_rows[k & 1].pos[row], token = s_rows[k & 1].token[row];
+            const float fac = s_rows[k & 1].fac[row];
             __syncwarp();
-            rt_piece_sync();
+            if (lane == 0) rt_mbar_arrive(tc_smem(&s_qbar[1][k & 1]));
             if (wg == 1 && k > 0) rt_taken_sync();       // the first group has read this one's O of the piece before
             const int hi = min(pos + 1, keys.k_end);
             const int lo = max(pc.t.key_lo, a.window > 0 ? pos - a.window + 1 : 0);
@@ -426,29 +422,34 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                 tc_fence_before_sync();
                 if (alive) rt_arrive(wg, 0);
                 else rt_sync(wg, 0);
-                float lead = 0.f;
                 if (HALF) {
 #pragma unroll
                     for (int c = 0; c < TC_BN; c += 4) {
                         const float4 f = *reinterpret_cast<const float4*>(&meta.ks[mt][c]);
-                        s[c] *= f.x; s[c + 1] *= f.y; s[c + 2] *= f.z; s[c + 3] *= f.w;
+                        rt_mul2(s[c], s[c + 1], f.x, f.y);
+                        rt_mul2(s[c + 2], s[c + 3], f.z, f.w);
                     }
-                    const float4 f = *reinterpret_cast<const float4*>(meta.vmax[mt]);
-                    const float vmax = fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w));
-                    lead = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -90);
                 }
-                const bool edge = key0 + TC_BN > hi || key0 < lo;        // this row does not see all of the tile's keys
-                if (edge) {
+                float vmax = HALF ? fmaxf(meta.vmax[mt][0], meta.vmax[mt][1]) : 0.f;
+                const uint2 seen = *reinterpret_cast<const uint2*>(meta.seen[mt]);
+                if ((seen.x & seen.y) != 0xffffffffu || key0 + TC_BN > hi || key0 < lo) {
+                    // this row does not see all 64 keys
+                    const uint32_t b0 = seen.x & rt_bits(lo - key0, hi - key0), b1 = seen.y & rt_bits(lo - key0 - 32, hi - key0 - 32);
 #pragma unroll
-                    for (int c = 0; c < TC_BN; ++c)
-                        if (key0 + c >= hi || key0 + c < lo) s[c] = -INFINITY;
-                }
-                {
-                    const int4 f = *reinterpret_cast<const int4*>(meta.hole[mt]);
-                    if (f.x | f.y | f.z | f.w) {
+                    for (int c = 0; c < 32; ++c) {
+                        if (!(b0 >> c & 1)) s[c] = -INFINITY;
+                        if (!(b1 >> c & 1)) s[c + 32] = -INFINITY;
+                    }
+                    if (HALF) {
+                        // the scale of a key that the row does not see has no part in its unit
+                        vmax = 0.f;
 #pragma unroll
-                        for (int c = 0; c < TC_BN; ++c)
-                            if (!meta.ok[mt][c]) s[c] = -INFINITY;
+                        for (int c = 0; c < TC_BN; c += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(&meta.vs[mt][c]);
+                            const uint32_t b = (c < 32 ? b0 : b1) >> (c & 31);
+                            vmax = tc_max3(vmax, b & 1 ? f.x : 0.f, b & 2 ? f.y : 0.f);
+                            vmax = tc_max3(vmax, b & 4 ? f.z : 0.f, b & 8 ? f.w : 0.f);
+                        }
                     }
                 }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -457,14 +458,8 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                     mx4[0] = tc_max3(mx4[0], s[c], s[c + 1]); mx4[1] = tc_max3(mx4[1], s[c + 2], s[c + 3]);
                     mx4[2] = tc_max3(mx4[2], s[c + 4], s[c + 5]); mx4[3] = tc_max3(mx4[3], s[c + 6], s[c + 7]);
                 }
-                float need = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), fac, lead);
-                if (HALF && edge) {
-                    // key by key: the scale of a key that the row does not see has no part in its unit
-                    need = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < TC_BN; ++c)
-                        need = fmaxf(need, fmaf(s[c], fac, (float)max((int)(__float_as_uint(meta.vs[mt][c]) >> 23) - 126, -90)));
-                }
+                const float lead = HALF ? (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -90) : 0.f;
+                const float need = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), fac, lead);
                 // the reference moves when p vs could pass 2^15 (or from "no key yet"), and then to 11 below the largest
                 const bool move = need > ref + 15.f;
                 const float old = ref;
@@ -482,10 +477,9 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                     tc_add2(rs[c & 4], rs[(c & 4) + 1], p[0], p[1]);
                     tc_add2(rs[(c & 4) + 2], rs[(c & 4) + 3], p[2], p[3]);
                     if (HALF) {
-                        // (a value row that is not finite has the scale NaN: hidden, its weight stays zero)
                         const float4 f = *reinterpret_cast<const float4*>(&meta.vs[mt][c]);
-                        p[0] = p[0] == 0.f ? 0.f : p[0] * f.x; p[1] = p[1] == 0.f ? 0.f : p[1] * f.y;
-                        p[2] = p[2] == 0.f ? 0.f : p[2] * f.z; p[3] = p[3] == 0.f ? 0.f : p[3] * f.w;
+                        rt_mul2(p[0], p[1], f.x, f.y);
+                        rt_mul2(p[2], p[3], f.z, f.w);
                         const __half2 h0 = __floats2half2_rn(p[0], p[1]), h1 = __floats2half2_rn(p[2], p[3]);
                         w[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
                         w[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
@@ -585,7 +579,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         if (wg == 1 && k > 0) rt_taken_sync();
     }
     tc_fence_before_sync();
-    asm volatile("bar.sync 8, %0;\n" ::"n"(RT_THREADS) : "memory");
+    asm volatile("bar.sync 7, %0;\n" ::"n"(RT_THREADS) : "memory");
     if (s_dead && tid == 0) atomicExch(a.kv.status, 3);
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
