@@ -256,28 +256,44 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
 }
 
 // ---- joining the parts of units that a cut goes through ------------------------------------------------------------
+// Block c looks at the cut in front of run c, and joins the unit there if it is the first cut through it.  Bound by latency: two to
+// a few parts per row, four dimensions per thread.
 template <typename QT>
 __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs a) {
-    const int tile = blockIdx.x / a.plan.nkv, head = blockIdx.x % a.plan.nkv, d = a.d, g = a.plan.group;
-    const RowTile t = ar_tile(a.plan, tile);
-    const int n = ar_chunks(t);
-    if (n == 0) return;
-    const int x0 = t.start + head * n, c0 = ar_owner(a.plan, x0), c1 = ar_owner(a.plan, x0 + n - 1);
-    if (c0 == c1) return;                                           // one block had it all and has stored it
+    const RowPlan& p = a.plan;
+    const int x = blockIdx.x * p.run, d = a.d, g = p.group;
+    if (x == 0 || x >= p.total) return;
+    RowWalk w;
+    w.begin(p, blockIdx.x);
+    RowPiece pc;
+    if (!w.next(p, pc) || pc.chunk0 == 0) return;                   // the run begins with a unit of its own
+    const int n = ar_chunks(pc.t), x0 = pc.t.start + pc.head * n, c0 = x0 / p.run, c1 = (x0 + n - 1) / p.run;
+    if (c0 != (int)blockIdx.x - 1) return;
     ST_PDL_WAIT();
-    const size_t unit = (size_t)tile * a.plan.nkv + head;
-    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < t.n_tok * g * d; i += gridDim.y * blockDim.x) {
-        const int r = i / d, e = i - r * d, token = a.plan.items ? a.plan.items[t.first + r / g] : t.first + r / g;
-        if (token < 0 || a.positions[token] < 0) continue;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(a.parts.r + (unit + c) * AR_ROWS + r));
+    const int pieces = (d + 3) / 4, total = pc.t.n_tok * g * pieces;
+    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < total; i += gridDim.y * blockDim.x) {
+        const int r = i / pieces, e = (i - r * pieces) * 4, place = pc.t.first + r / g, token = p.items ? p.items[place] : place;
+        if (a.positions[token] < 0) continue;
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(a.parts.r + (size_t)(pc.unit + c) * AR_ROWS + r));
         for (int c = c0; c <= c1; ++c) {
-            const size_t at = (unit + c) * AR_ROWS + r;
-            const float w = ar_weight(__ldcg(a.parts.r + at), m);
-            l += w * __ldcg(a.parts.l + at);
-            o += w * __ldcg(a.parts.o + at * d + e);
+            const size_t at = (size_t)(pc.unit + c) * AR_ROWS + r;
+            const float f = ar_weight(__ldcg(a.parts.r + at), m);
+            const float* part = a.parts.o + at * d + e;
+            l += f * __ldcg(a.parts.l + at);
+            if (d % 4 == 0) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(part));
+                o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (e + k < d) o[k] += f * __ldcg(part + k);
+            }
         }
-        ((QT*)a.out)[((size_t)token * a.plan.nh + head * g + r % g) * d + e] = from_f32<QT>(l == 0.f ? 0.f : o / l);
+        QT* out = (QT*)a.out + ((size_t)token * p.nh + pc.head * g + r % g) * d + e;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (e + k < d) out[k] = from_f32<QT>(l == 0.f ? 0.f : o[k] / l);
     }
 }
 
@@ -426,10 +442,11 @@ static int ar_rows(RowArgs a, int act, int form, int max_rows, cudaStream_t s) {
     return aa_rows<C8_F32, float>(a, max_rows, s);
 }
 
-// Blocks among which a plan's line of chunks is dealt out: as many as run at the same time, one per SM of the tensor-core kernel.
-static int ar_ctas(const RowArgs& a, int act, int form) {
+// The runs a plan's line of chunks is cut into: as many as blocks run at the same time, one per SM of the tensor-core kernel.
+static void ar_deal(RowArgs& a, int act, int form) {
     const int most = st_sm_count() * (ar_tc(a, act, form) ? 1 : a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
-    return a.plan.total < most ? (a.plan.total > 0 ? a.plan.total : 1) : most;
+    a.plan.run = a.plan.total > most ? (a.plan.total + most - 1) / most : 1;
+    a.plan.ctas = (a.plan.total + a.plan.run - 1) / a.plan.run;
 }
 static RowParts ar_parts(float* scratch, long long slots) {
     return RowParts{scratch, scratch + slots * AR_ROWS, scratch + 2 * slots * AR_ROWS};
@@ -481,8 +498,8 @@ static RowArgs ar_row_args(const RowCall& c) {
     a.q = c.q; a.out = c.out; a.q_stride = c.q_stride > 0 ? c.q_stride : (long long)c.nh * c.d; a.kv = ar_kv(c);
     a.positions = c.positions; a.seq_of_token = c.seq_of_token; a.slots = c.slots; a.d = c.d;
     a.scale_log2 = c.scale * AR_LOG2E; a.window = c.window;
-    a.plan = RowPlan{c.tiles, c.items, c.n_tiles, c.total, 1, c.nh, c.nkv, c.nh / c.nkv};
-    a.plan.ctas = ar_ctas(a, c.act, c.form);
+    a.plan = RowPlan{c.tiles, c.items, c.n_tiles, c.total, 0, 0, c.nh, c.nkv, c.nh / c.nkv};
+    ar_deal(a, c.act, c.form);
     return a;
 }
 
@@ -511,7 +528,7 @@ ST_EXPORT int st_attention_tiles8(const RowCall* c, void* stream) {
     const cudaStream_t s = (cudaStream_t)stream;
     const int r = ar_rows(a, c->act, c->form, c->max_rows, s);
     if (r || a.plan.ctas == 1) return r;
-    const dim3 grid(c->n_tiles * c->nkv, 4);
+    const dim3 grid(a.plan.ctas, 8);
     return c->act == 0 ? st_launch_pdl("rows_join", attention_rows_join_kernel<float>, grid, dim3(256), 0, s, a)
                        : st_launch_pdl("rows_join", attention_rows_join_kernel<bf16>, grid, dim3(256), 0, s, a);
 }

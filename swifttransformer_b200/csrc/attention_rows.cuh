@@ -3,9 +3,9 @@
 //
 // A row is one (token, query head).  A tile holds the rows of up to 128 / g tokens, for one key head, g = query heads per key
 // head: row r is head r % g of the group of token r / g.  The tile's keys [key_lo, key_hi) are walked in chunks of AR_CHUNK.
-// All chunks of all (tile, key head) pairs, one pair's behind the other's, form one line of `total` chunks which is cut
-// into `ctas` runs of equal length: every block gets the same work however unequal the tiles are, and a pair that a cut goes
-// through ("unit") is put together from parts.  Part (unit u, block c) has slot u + c: a new slot begins with every unit and with
+// All chunks of all (tile, key head) pairs ("units"), one unit's behind the other's, form one line of `total` chunks which is cut
+// into runs of `run` chunks, one per block: every block gets the same work however unequal the tiles are, and a unit that a cut
+// goes through is put together from parts.  Part (unit u, block c) has slot u + c: a new slot begins with every unit and with
 // every block, so no two parts share one.
 //
 // A part of a row is (R, l, O): p_j = 2^(s_j - R), s in units of log2, l = sum p_j, O = sum p_j v_j, all float; R is a number near
@@ -23,7 +23,7 @@ struct RowTile { int first, n_tok, seq, key_lo, key_hi, start; };   // start: th
 struct RowPlan {
     const int* tiles;        // [n_tiles][6]
     const int* items;        // tokens in the tiles' order, or null: tile tokens are first, first + 1, ...
-    int n_tiles, total, ctas;
+    int n_tiles, total, ctas, run;
     int nh, nkv, group;      // group = nh / nkv
 };
 // where parts lie: per slot AR_ROWS rows (R, l) and AR_ROWS x d of O
@@ -57,15 +57,6 @@ __device__ __forceinline__ RowTile ar_tile(const RowPlan& p, int i) {
 __device__ __forceinline__ int ar_chunks(const RowTile& t) {
     return t.key_hi > t.key_lo ? (t.key_hi - (t.key_lo & ~(AR_CHUNK - 1)) + AR_CHUNK - 1) / AR_CHUNK : 0;
 }
-// the first chunk of block c's run, and the block whose run holds chunk x
-__device__ __forceinline__ int ar_run(const RowPlan& p, int c) { return (int)((long long)p.total * c / p.ctas); }
-__device__ __forceinline__ int ar_owner(const RowPlan& p, int x) {
-    int c = (int)((long long)x * p.ctas / p.total);
-    while (c + 1 < p.ctas && ar_run(p, c + 1) <= x) ++c;
-    while (c > 0 && ar_run(p, c) > x) --c;
-    return c;
-}
-
 // A block's way along its run: pieces of one (tile, key head) pair.
 struct RowPiece {
     RowTile t;
@@ -77,8 +68,8 @@ struct RowWalk {
     int at, end, tile;
     RowTile t;
     __device__ __forceinline__ void begin(const RowPlan& p, int c) {
-        at = ar_run(p, c);
-        end = ar_run(p, c + 1);
+        at = c * p.run;
+        end = min(at + p.run, p.total);
         // the last tile that starts at or before `at` (tiles without chunks start where the next one does)
         int lo = 0, hi = p.n_tiles - 1;
         while (lo < hi) {
@@ -109,14 +100,14 @@ struct RowWalk {
     }
 };
 
-// Cut and joined parts of row `row` of unit (tile, head) -> sums over e0, e0 + step, ... of d: calls f(weight, O row, l) per part.
+// Calls f(slot) for every part of unit (tile, head).
 template <typename F>
 __device__ __forceinline__ void ar_each_part(const RowPlan& p, const RowTile& t, int tile, int head, F f) {
     const int n = ar_chunks(t);
     if (n == 0) return;
     const int x0 = t.start + head * n, unit = tile * p.nkv + head;
-    const int c1 = ar_owner(p, x0 + n - 1);
-    for (int c = ar_owner(p, x0); c <= c1; ++c) f(unit + c);
+    const int c1 = (x0 + n - 1) / p.run;
+    for (int c = x0 / p.run; c <= c1; ++c) f(unit + c);
 }
 
 __device__ __forceinline__ float ar_exp2(float x) {      // 2 ulp, exp2(-inf) = 0

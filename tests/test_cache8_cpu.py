@@ -11,7 +11,8 @@ from swifttransformer_b200.ops import KernelError
 def walk(plan, ctas):
     """The pieces every block gets, as the kernels cut the line of chunks."""
     tiles = plan.tiles.view(-1, 6).tolist()
-    bounds = [plan.total * c // ctas for c in range(ctas + 1)]
+    run = -(-plan.total // ctas)
+    bounds = [min(run * c, plan.total) for c in range(ctas + 1)]
     pieces = []
     for c in range(ctas):
         for x in range(bounds[c], bounds[c + 1]):
