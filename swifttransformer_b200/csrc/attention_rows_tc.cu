@@ -263,10 +263,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         }
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_OTHER));
-        // ---- two warps per group bring its keys (which = 0), two its values: a thread per row
+        // ---- two warps per group bring its keys (which = 0), two its values: 32 rows of every tile each
         const int w8 = warp - 8, wg = w8 & 1, which = (w8 >> 1) & 1, half = w8 >> 2, row = half * 32 + lane;
         const uint32_t mb_full = bar(wg, M_FULL + which * 2), mb_free = bar(wg, M_FREE + which * 2), mb_meta = bar(wg, M_META);
-        const uint32_t buf0 = buf_of(wg, which, 0) + row * 128, swz = (uint32_t)(row & 7) << 4;
+        const uint32_t buf0 = buf_of(wg, which, 0) + half * 32 * 128;
         RtMeta& meta = s_meta[wg];
         constexpr uint32_t NONE = 0xffffffffu;
         const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
@@ -326,51 +326,76 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         };
         auto wait_free = [&]() -> bool { return n < 2 || tc_wait_warp(mb_free + 8 * (n & 1), ((n - 2) >> 1) & 1, dead); };
         look();
+        const unsigned char* pool = a.kv.pool;
         if constexpr (HALF) {
-            constexpr int NB = DP / 16;                  // 16-byte pieces of a row
+            // NP neighbouring lanes read a row, 16 bytes each: load j has rows j RI .. j RI + RI - 1 of the warp's 32
+            constexpr int NP = DP / 16, RI = 32 / NP;
+            const int p = lane % NP, rl = lane / NP;
+            const bool in = 16 * p < d;
+            uint4 data[NP];
+            float ks = 0.f, vs = 0.f;
+            auto load = [&](int j) {
+                const uint32_t r = __shfl_sync(0xffffffffu, at, j * RI + rl);
+                data[j] = in && r != NONE ? __ldg(reinterpret_cast<const uint4*>(pool + (size_t)(which ? r + to_values : r) * d) + p)
+                                          : make_uint4(0u, 0u, 0u, 0u);
+            };
+            auto load_scales = [&]() {
+                ks = which == 0 && at != NONE ? __ldg(a.kv.scales + at) : 0.f;
+                vs = at != NONE ? __ldg(a.kv.scales + at + to_values) : 0.f;
+            };
+            if (have) {
+                load_scales();
+#pragma unroll
+                for (int j = 0; j < NP; ++j) load(j);
+            }
             while (have) {
-                uint4 data[NB];
                 const uint32_t mine = at;
                 const bool no_page = hole;
-                float ks = 0.f, vs = 0.f;
-                if (mine != NONE) {
-                    if (which == 0) ks = __ldg(a.kv.scales + mine);
-                    vs = __ldg(a.kv.scales + mine + to_values);
-                }
-                const unsigned char* src = a.kv.pool + (size_t)(mine != NONE ? mine + (which ? to_values : 0u) : 0u) * d;
-#pragma unroll
-                for (int k = 0; k < NB; ++k)
-                    data[k] = mine != NONE && 16 * k < d ? __ldg(reinterpret_cast<const uint4*>(src) + k) : make_uint4(0u, 0u, 0u, 0u);
-                look();
+                look();                                      // `at`: the next tile's (NONE behind the last one)
+                if (!have) at = NONE;
                 if (!wait_free()) break;
-                const uint32_t buf = buf0 + (n & 1) * BUF;
-#pragma unroll
-                for (int k = 0; k < NB; ++k) {
-                    uint32_t h[8];
-                    c8_halves<FORM>(data[k].x, h[0], h[1]);
-                    c8_halves<FORM>(data[k].y, h[2], h[3]);
-                    c8_halves<FORM>(data[k].z, h[4], h[5]);
-                    c8_halves<FORM>(data[k].w, h[6], h[7]);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)              // eight dimensions each
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
-                                     ::"r"(buf + (k >> 2) * KV_BLK + (((uint32_t)((2 * k + c) & 7) << 4) ^ swz)), "r"(h[4 * c]),
-                                       "r"(h[4 * c + 1]), "r"(h[4 * c + 2]), "r"(h[4 * c + 3]) : "memory");
-                }
+                const uint32_t buf = buf0 + (n & 1) * BUF + (p >> 2) * KV_BLK;
                 put_meta(ks, vs, mine, no_page);
+                load_scales();
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    uint32_t h[8];
+                    c8_halves<FORM>(data[j].x, h[0], h[1]);
+                    c8_halves<FORM>(data[j].y, h[2], h[3]);
+                    c8_halves<FORM>(data[j].z, h[4], h[5]);
+                    c8_halves<FORM>(data[j].w, h[6], h[7]);
+                    load(j);                                 // the next tile's, as soon as the registers are free
+                    const uint32_t r = j * RI + rl;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {            // eight dimensions each; the upper half of a row the other way round (banks)
+                        const bool flip = (p >> 2) & 1;
+                        const uint32_t c = (2 * p + (flip ? 1 - k : k)) & 7;
+                        const bool hi = flip ? k == 0 : k == 1;
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                     ::"r"(buf + r * 128 + ((c ^ (r & 7)) << 4)), "r"(hi ? h[4] : h[0]), "r"(hi ? h[5] : h[1]),
+                                       "r"(hi ? h[6] : h[2]), "r"(hi ? h[7] : h[3]) : "memory");
+                    }
+                }
                 landed(n);
                 ++n;
             }
         } else {
             // copies of a tile are asked for as soon as its buffer is free; the tile before is announced when its own have landed
+            constexpr int NP = DP / 8, RI = 32 / NP;         // lanes of a row, rows of a copy
+            const int p = lane % NP, rl = lane / NP;
+            const bool in = 8 * p < d;
             bool alive = true;
             while (have) {
                 if (!wait_free()) { alive = false; break; }
-                const uint32_t buf = buf0 + (n & 1) * BUF;
-                const unsigned char* src = a.kv.pool + (size_t)(at != NONE ? at + (which ? to_values : 0u) : 0u) * d * 2;
+                const uint32_t buf = buf0 + (n & 1) * BUF + (p >> 3) * KV_BLK;
 #pragma unroll
-                for (int k = 0; k < DP / 8; ++k)
-                    tc_cp16(buf + (k >> 3) * KV_BLK + (((uint32_t)(k & 7) << 4) ^ swz), 8 * k < d ? src + 16 * k : src, at != NONE && 8 * k < d);
+                for (int j = 0; j < NP; ++j) {
+                    const int row_j = j * RI + rl;
+                    const uint32_t r = __shfl_sync(0xffffffffu, at, row_j);
+                    const bool ok = in && r != NONE;
+                    tc_cp16(buf + row_j * 128 + (((p & 7) ^ (row_j & 7)) << 4),
+                            ok ? pool + (size_t)(which ? r + to_values : r) * d * 2 + 16 * p : pool, ok);
+                }
                 tc_cp_commit();
                 put_meta(0.f, 0.f, at, hole);
                 ++n;
