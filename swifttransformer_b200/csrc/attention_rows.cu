@@ -442,9 +442,10 @@ static int ar_rows(RowArgs a, int act, int form, int max_rows, cudaStream_t s) {
     return aa_rows<C8_F32, float>(a, max_rows, s);
 }
 
-// The runs a plan's line of chunks is cut into: as many as blocks run at the same time, one per SM of the tensor-core kernel.
+// The runs a plan's line of chunks is cut into: as many as are walked at the same time, two per SM by the tensor-core kernel, one by every
+// block of the float kernel.
 static void ar_deal(RowArgs& a, int act, int form) {
-    const int most = st_sm_count() * (ar_tc(a, act, form) ? 1 : a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
+    const int most = st_sm_count() * (ar_tc(a, act, form) ? 2 : a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
     a.plan.run = a.plan.total > most ? (a.plan.total + most - 1) / most : 1;
     a.plan.ctas = (a.plan.total + a.plan.run - 1) / a.plan.run;
 }

@@ -4,9 +4,9 @@
 // A row is one (token, query head).  A tile holds the rows of up to 128 / g tokens, for one key head, g = query heads per key
 // head: row r is head r % g of the group of token r / g.  The tile's keys [key_lo, key_hi) are walked in chunks of AR_CHUNK.
 // All chunks of all (tile, key head) pairs ("units"), one unit's behind the other's, form one line of `total` chunks which is cut
-// into runs of `run` chunks, one per block: every block gets the same work however unequal the tiles are, and a unit that a cut
-// goes through is put together from parts.  Part (unit u, block c) has slot u + c: a new slot begins with every unit and with
-// every block, so no two parts share one.
+// into runs of `run` chunks, one per walker (a block, or one of a block's two groups): every walker gets the same work however
+// unequal the tiles are, and a unit that a cut goes through is put together from parts.  Part (unit u, walker c) has slot u + c: a
+// new slot begins with every unit and with every run, so no two parts share one.
 //
 // A part of a row is (R, l, O): p_j = 2^(s_j - R), s in units of log2, l = sum p_j, O = sum p_j v_j, all float; R is a number near
 // the largest s_j (the exact maximum is not needed: only the common factor).  Parts are joined by 2^(R - max R).
@@ -57,7 +57,7 @@ __device__ __forceinline__ RowTile ar_tile(const RowPlan& p, int i) {
 __device__ __forceinline__ int ar_chunks(const RowTile& t) {
     return t.key_hi > t.key_lo ? (t.key_hi - (t.key_lo & ~(AR_CHUNK - 1)) + AR_CHUNK - 1) / AR_CHUNK : 0;
 }
-// A block's way along its run: pieces of one (tile, key head) pair.
+// A walker's way along its run: pieces of one (tile, key head) pair.  A walker behind the line's end has none.
 struct RowPiece {
     RowTile t;
     int tile, head;          // head: key head
@@ -68,7 +68,7 @@ struct RowWalk {
     int at, end, tile;
     RowTile t;
     __device__ __forceinline__ void begin(const RowPlan& p, int c) {
-        at = c * p.run;
+        at = min(c * p.run, p.total);
         end = min(at + p.run, p.total);
         // the last tile that starts at or before `at` (tiles without chunks start where the next one does)
         int lo = 0, hi = p.n_tiles - 1;

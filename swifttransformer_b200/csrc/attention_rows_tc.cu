@@ -6,38 +6,40 @@
 // bfloat16.  S = Q K^T of 128 rows x 64 keys and O += P V are tcgen05 products with their sums in tensor memory; P goes there
 // straight from the softmax threads' registers (the product's A operand).
 //
-// One block per SM walks its run of the plan's chunks.  Two groups of four softmax warps take every second tile of 64 keys of a
-// piece, each with its own S, O and P in tensor memory, key and value buffers (two each) and issuing warp; at the piece's end
-// the first group reads the second's O from tensor memory (the lanes are the same rows) and stores the sum.  Four warps bring
-// keys, four bring values, for both groups in turn, and run ahead across pieces:
-//   8-bit forms: 16-byte loads to registers, several tiles ahead (32 KB per SM under way: memory needs that), conversion to
-//   halves, stores into the 128-byte swizzled layout the matrix descriptors expect.  Conversion is the price of the format: about
-//   2.5 instructions per four codes against the softmax's 4 per score; with one row of 128 codes per thread, two warps each, it
-//   bounded the kernel, so there are four.
-//   bfloat16: asynchronous copies into that layout, as many tiles ahead as there are buffers.
-// Page sizes are arbitrary: every thread looks up its row's page, a tile ahead of its loads.
-// With the row's scales go their largest value scale per tile, from which the softmax threads take the power of two that keeps P in
-// a half's range (attention_single8.cuh), and a mark where a key has no page.
+// One block per SM, in it two groups that have nothing to do with one another: each walks its own run of the plan's chunks in tiles of
+// 64 keys, with four softmax warps (a thread per row), a warp that issues its products, two that bring keys and two that bring values
+// through two buffers each.  What one group waits for the other fills: a tile is a chain (codes landed, S, softmax, P V) whose
+// links are a few hundred to a thousand clocks each.  The next piece's queries are brought by the softmax warps while the last P V
+// of a piece is on the tensor cores; its first S then runs under their stores.
+//   8-bit forms: neighbouring lanes read a row in 16-byte loads, a tile ahead of the conversion to halves, which is stored in the 128-byte
+//   swizzled layout that the matrix descriptors expect.  At head size 128 the two halves of every 16 codes go to different blocks of
+//   64 dimensions (rt_dim): neighbouring lanes then store to different banks without sorting; queries are stored alike, results
+//   are put in order when they leave.
+//   bfloat16: asynchronous copies into that layout.
+// Page sizes are arbitrary: a lane looks up its row's page two tiles ahead of its loads.
+// The warps that bring keys also leave both scales of the rows, the largest value scale of a tile, from which the softmax threads take the
+// power of two that keeps P in a half's range (attention_single8.cuh), and a bit per key that has a page.
 //
-// Bound by the softmax (an exponential per score, 16 a clock and SM) at head size 64, by softmax and conversion together at 128, and by
-// memory for prefixes shared by few rows.  Waits are bounded; one that expires marks the block dead, the other waits end, `status`
-// gets 3, tensor memory is freed and the kernel returns.
+// Waits are bounded; one that expires marks the block dead, the other waits end, `status` gets 3, tensor memory is freed and the
+// kernel returns.
 #include "attention_rows.cuh"
 #include "tcgen05.cuh"
 
-#define RT_THREADS 640                   // 8 softmax warps, 4 for keys, 4 for values, 2 issuing products, 2 for queries
+#define RT_THREADS 640                   // 8 softmax warps, 8 bringing keys and values, 2 issuing products, 2 that fill the last four
 // Registers a thread keeps after the block has shared them out anew; the sum must not pass what the launch got, 640 x 96.
 #define RT_REGS_SOFTMAX 144
-#define RT_REGS_OTHER 64
-static_assert(256 * RT_REGS_SOFTMAX + 384 * RT_REGS_OTHER <= RT_THREADS * 96, "more registers than the block owns");
+#define RT_REGS_BRING 80
+#define RT_REGS_ISSUE 32
+#define RT_REGS_ALL (256 * RT_REGS_SOFTMAX + 256 * RT_REGS_BRING + 128 * RT_REGS_ISSUE)
+static_assert(RT_REGS_ALL <= RT_THREADS * 96, "more registers than the block owns");
 #define RT_META 4                        // tiles whose scales are kept: see below
 
 __device__ __forceinline__ void rt_mbar_arrive(uint32_t mbar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(mbar) : "memory");
 }
-// Named barriers.  1-4: a softmax group and the warp that issues its products (160 threads): 0 "S has been read", 1 "P has been written".
-// 5: the second group's share of a piece is complete.  6: the first group has read it.  7: the whole block.  A softmax warp that has given up waiting meets the issuing
-// warp at 1-4 instead of only arriving, so that it cannot come round twice.
+// Named barriers 1-4: a softmax group and the warp that issues its products (160 threads): 0 "S has been read", 1 "P has been
+// written".  5: the whole block.  A softmax warp without rows of its own, or one that has given up waiting, meets the issuing warp there
+// instead of only arriving, so that it cannot come round twice.
 __device__ __forceinline__ void rt_arrive(int wg, int which) {
     const int id = 2 * wg + which;
     if (id == 0) asm volatile("bar.arrive 1, 160;\n" ::: "memory");
@@ -52,20 +54,10 @@ __device__ __forceinline__ void rt_sync(int wg, int which) {
     else if (id == 2) asm volatile("bar.sync 3, 160;\n" ::: "memory");
     else asm volatile("bar.sync 4, 160;\n" ::: "memory");
 }
-__device__ __forceinline__ void rt_share_arrive() { asm volatile("bar.arrive 5, 256;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_share_sync() { asm volatile("bar.sync 5, 256;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_taken_arrive() { asm volatile("bar.arrive 6, 256;\n" ::: "memory"); }
-__device__ __forceinline__ void rt_taken_sync() { asm volatile("bar.sync 6, 256;\n" ::: "memory"); }
-
 __device__ __forceinline__ void rt_mul2(float& d0, float& d1, float b0, float b1) {       // d *= b
     asm("{\n\t.reg .b64 b, d;\n\tmov.b64 b, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\tmul.rn.f32x2 d, d, b;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
         : "+f"(d0), "+f"(d1) : "f"(b0), "f"(b1));
 }
-// what the softmax threads need to know of a row
-struct RtRows {
-    int pos[AR_ROWS], token[AR_ROWS];
-    float fac[AR_ROWS];
-};
 // bits lo .. hi - 1 of a word
 __device__ __forceinline__ uint32_t rt_bits(int lo, int hi) {
     const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1;
@@ -81,7 +73,8 @@ __device__ __forceinline__ RtKeys rt_keys(const RowPiece& p) {
     k.n = (k.k_end - k.k0 + TC_BN - 1) / TC_BN;
     return k;
 }
-__device__ __forceinline__ int rt_share(int n, int wg) { return (n - wg + 1) >> 1; }    // tiles of a group
+// where dimension 8 c + i of a row is kept: piece rt_place(c) + i, in blocks of 64
+template <bool HALF, int DP> __device__ __forceinline__ int rt_place(int c) { return HALF && DP == 128 ? (c & 1) * 8 + (c >> 1) : c; }
 
 // what the softmax threads need to know of a tile, beside S
 struct RtMeta {
@@ -98,16 +91,14 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     constexpr uint32_t Q_BUF = DB * Q_BLK, BUF = DB * KV_BLK;
     constexpr uint32_t ALL_BYTES = 2 * Q_BUF + 8 * BUF;
     constexpr int WG_COLS = 256, T_O = 64, T_P = 64 + DP;              // a group's columns: S, O, P
+    constexpr uint32_t NONE = 0xffffffffu;
     extern __shared__ unsigned char rt_raw[];
     __shared__ __align__(16) RtMeta s_meta[2];
-    __shared__ RtRows s_rows[2];
-    __shared__ float s_mrg[2][128];
-    // per group: S done, O done, "landed" for K0 K1 V0 V1, "free" for the same, and the scales of four tiles; of the two
-    // query buffers: "landed" and "free"
-    __shared__ __align__(8) unsigned long long s_mbar[2][10 + RT_META], s_qbar[2][2];
+    // per group: S done, O done, "landed" for K0 K1 V0 V1, "free" for the same, queries landed, the scales of four tiles
+    __shared__ __align__(8) unsigned long long s_mbar[2][11 + RT_META];
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
-    __shared__ RowWalk s_walk;
+    __shared__ RowWalk s_walk[2];
     const uint32_t base = (tc_smem(rt_raw) + 1023u) & ~1023u;
     const int tid = threadIdx.x, warp = tc_warp(), lane = tid & 31;
     const int d = a.d, g = a.plan.group;
@@ -119,23 +110,20 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             return;
         }
     }
-    const uint32_t sQ = base;                                          // two query buffers
-    auto buf_of = [&](int wg, int which, int b) { return base + 2 * Q_BUF + (uint32_t)((wg * 2 + which) * 2 + b) * BUF; };
-    auto bar = [&](int wg, int i) { return tc_smem(&s_mbar[wg][i]); };
-    constexpr int M_S = 0, M_O = 1, M_FULL = 2, M_FREE = 6, M_META = 10;
+    // the group: softmax warps 0-3 and 4-7, the others in turn
+    const int wg = warp < 8 ? warp >> 2 : warp & 1;
+    const uint32_t sQ = base + wg * Q_BUF;
+    auto buf_of = [&](int which) { return base + 2 * Q_BUF + (uint32_t)(wg * 2 + which) * 2 * BUF; };
+    auto bar = [&](int i) { return tc_smem(&s_mbar[wg][i]); };
+    constexpr int M_S = 0, M_O = 1, M_FULL = 2, M_FREE = 6, M_Q = 10, M_META = 11;
     if (tid == 0) {
-        for (int w = 0; w < 2; ++w) {
-            for (int k = 0; k < 10 + RT_META; ++k)
-                tc_mbar_init(bar(w, k), k >= M_META ? (HALF ? 4 : 2) : k >= M_FULL && k < M_FREE ? 2 : 1);
-        }
-        for (int k = 0; k < 2; ++k) {
-            tc_mbar_init(tc_smem(&s_qbar[0][k]), 2);           // both bringing warps
-            tc_mbar_init(tc_smem(&s_qbar[1][k]), 2 + 8);       // both groups' last S, all softmax warps
-        }
+        for (int w = 0; w < 2; ++w)
+            for (int k = 0; k < 11 + RT_META; ++k)
+                tc_mbar_init(tc_smem(&s_mbar[w][k]), k >= M_META || (k >= M_FULL && k < M_FREE) ? 2 : k == M_Q ? 4 : 1);
         tc_mbar_init_fence();
         s_dead = 0;
     }
-    if (tid == 32) s_walk.begin(a.plan, blockIdx.x);
+    if (tid == 32 || tid == 64) s_walk[(tid >> 5) - 1].begin(a.plan, 2 * blockIdx.x + (tid >> 5) - 1);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -146,27 +134,24 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     ST_PDL_TRIGGER();
     const uint32_t tmem = s_tmem;
     volatile int* dead = &s_dead;
-    auto tile_addr = [](uint32_t tile, int r, int c) -> uint32_t { return tile + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+    RowWalk walk = s_walk[wg];
+    RowPiece pc;
 
     if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_OTHER));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_ISSUE));
         if (warp < 18) {
-            // ---- the warp that issues a group's products
-            const int wg = warp - 16;
+            // ---- the warp that issues the group's products
             const uint32_t t_wg = tmem + wg * WG_COLS;
             constexpr uint32_t type = HALF ? 0u : (1u << 7) | (1u << 10);
             constexpr uint32_t idesc_s = (1u << 4) | type | ((TC_BN / 8) << 17) | ((TC_BM / 16) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((DP / 8) << 17) | ((TC_BM / 16) << 24);
-            const uint64_t dk = tc_desc(buf_of(wg, 0, 0), 16, 1024), dv = tc_desc(buf_of(wg, 1, 0), KV_BLK, 1024);
-            const uint32_t mb_s = bar(wg, M_S), mb_o = bar(wg, M_O), mb_full = bar(wg, M_FULL), mb_free = bar(wg, M_FREE);
+            const uint64_t dq = tc_desc(sQ, 16, 1024), dk = tc_desc(buf_of(0), 16, 1024), dv = tc_desc(buf_of(1), KV_BLK, 1024);
+            const uint32_t mb_s = bar(M_S), mb_o = bar(M_O), mb_full = bar(M_FULL), mb_free = bar(M_FREE);
             bool alive = true;
-            uint32_t n = 0;              // tiles of this group so far: buffer n & 1, phase (n >> 1) & 1
-            RowWalk walk = s_walk;
-            RowPiece pc;
+            uint32_t n = 0;              // tiles so far: buffer n & 1, phase (n >> 1) & 1
             for (int k = 0; walk.next(a.plan, pc); ++k) {
-                const int mine = rt_share(rt_keys(pc).n, wg);
-                const uint64_t dq = tc_desc(sQ + (k & 1) * Q_BUF, 16, 1024);
-                auto issue_s = [&](uint32_t x, bool last) {
+                const int tiles = rt_keys(pc).n;
+                auto issue_s = [&](uint32_t x) {
                     const int b = x & 1;
                     if (alive) alive = tc_wait_warp(mb_full + 8 * b, (x >> 1) & 1, dead);
                     if (alive) {
@@ -178,19 +163,17 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                                        dk + ((b * BUF + (kk >> 2) * KV_BLK + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
                             tc_commit(mb_s);
                             tc_commit(mb_free + 8 * b);
-                            if (last) tc_commit(tc_smem(&s_qbar[1][k & 1]));
                         }
                     }
                     __syncwarp();
                 };
-                if (alive) alive = tc_wait_warp(tc_smem(&s_qbar[0][k & 1]), (k >> 1) & 1, dead);
-                if (mine > 0) issue_s(n, mine == 1);
-                else if (lane == 0) rt_mbar_arrive(tc_smem(&s_qbar[1][k & 1]));
-                for (int i = 0; i < mine; ++i) {
+                if (alive) alive = tc_wait_warp(bar(M_Q), k & 1, dead);
+                issue_s(n);
+                for (int i = 0; i < tiles; ++i) {
                     const uint32_t x = n + i;
                     const int b = x & 1;
                     rt_sync(wg, 0);      // S(i) is in the softmax threads' registers
-                    if (i + 1 < mine) issue_s(x + 1, i + 2 == mine);
+                    if (i + 1 < tiles) issue_s(x + 1);
                     rt_sync(wg, 1);      // P(i) is written, O += P V of tile i - 1 has completed
                     if (alive) alive = tc_wait_warp(mb_full + 8 * (2 + b), (x >> 1) & 1, dead);
                     if (alive) {
@@ -205,158 +188,115 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                     }
                     __syncwarp();
                 }
-                n += mine;
-            }
-        } else {
-            // ---- two warps bring the queries, a piece ahead: a thread has two rows
-            RowWalk walk = s_walk;
-            RowPiece pc;
-            for (int k = 0; walk.next(a.plan, pc); ++k) {
-                if (k >= 2 && !tc_wait_warp(tc_smem(&s_qbar[1][k & 1]), ((k - 2) >> 1) & 1, dead)) break;
-                const int rows = pc.t.n_tok * g;
-#pragma unroll 1
-                for (int row = (warp - 18) * 32 + lane; row < AR_ROWS; row += 64) {
-                    const int place = pc.t.first + row / g;
-                    const int token = row < rows ? (a.plan.items ? a.plan.items[place] : place) : -1;
-                    const int pos = token >= 0 ? a.positions[token] : -1;
-                    const bf16* q = (const bf16*)a.q + (size_t)(pos >= 0 ? token : 0) * a.q_stride + (size_t)(pos >= 0 ? pc.head * g + row % g : 0) * d;
-                    float mul = 1.f, fac = a.scale_log2;
-                    if (HALF) {
-                        // a power of two that brings the row's largest element to [2^14, 2^15)
-                        uint32_t amax = 0;
-#pragma unroll
-                        for (int c = 0; c < DP / 8; ++c) {
-                            if (pos < 0 || 8 * c >= d) continue;
-                            const uint4 u = __ldg(reinterpret_cast<const uint4*>(q) + c);
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-                        }
-                        const int ex = min(max((int)(amax >> 7) - 127, -100), 127);
-                        mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-                        fac = ldexpf(a.scale_log2, ex - 14);
-                    }
-                    const uint32_t dst = sQ + (k & 1) * Q_BUF + row * 128, swz = (uint32_t)(row & 7) << 4;
-#pragma unroll
-                    for (int c = 0; c < DP / 8; ++c) {
-                        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                        if (pos >= 0 && 8 * c < d) u = __ldg(reinterpret_cast<const uint4*>(q) + c);
-                        if (HALF) {
-                            uint32_t* w = &u.x;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * mul, __uint_as_float(w[j] & 0xffff0000u) * mul);
-                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
-                                     ::"r"(dst + (c >> 3) * Q_BLK + (((uint32_t)(c & 7) << 4) ^ swz)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
-                    }
-                    s_rows[k & 1].pos[row] = pos;
-                    s_rows[k & 1].token[row] = token;
-                    s_rows[k & 1].fac[row] = fac;
-                }
-                tc_fence_async_smem();
-                __syncwarp();
-                if (lane == 0) rt_mbar_arrive(tc_smem(&s_qbar[0][k & 1]));
+                n += tiles;
             }
         }
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_OTHER));
-        // ---- two warps per group bring its keys (which = 0), two its values: 32 rows of every tile each
-        const int w8 = warp - 8, wg = w8 & 1, which = (w8 >> 1) & 1, half = w8 >> 2, row = half * 32 + lane;
-        const uint32_t mb_full = bar(wg, M_FULL + which * 2), mb_free = bar(wg, M_FREE + which * 2), mb_meta = bar(wg, M_META);
-        const uint32_t buf0 = buf_of(wg, which, 0) + half * 32 * 128;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_BRING));
+        // ---- two warps bring the group's keys (which = 0), two its values: 32 rows of every tile each
+        const int which = (warp >> 1) & 1, half = (warp - 8) >> 2, row = half * 32 + lane;
+        const uint32_t mb_full = bar(M_FULL + which * 2), mb_free = bar(M_FREE + which * 2), mb_meta = bar(M_META);
+        const uint32_t buf0 = buf_of(which) + half * 32 * 128;
         RtMeta& meta = s_meta[wg];
-        constexpr uint32_t NONE = 0xffffffffu;
         const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
-        uint32_t n = 0;                  // this group's tiles so far
-        RowWalk walk = s_walk;
-        RowPiece pc;
+        uint32_t n = 0;                  // tiles so far
         RtKeys keys;
         keys.n = 0;
         const int* bt = nullptr;
-        int i = wg;                      // the next tile of the piece
+        int i = 0;                       // the next tile of the piece
         bool have = true;
-        uint32_t at = NONE;              // its keys' row of this thread, looked up a tile ahead of the loads
-        bool hole = false;               // a key that a row may see has no page
-        auto look = [&]() {
-            while (i >= keys.n) {
+        // A lane looks up the page of its row two tiles ahead (ask), turns it into a row of the pool one tile ahead (resolve).
+        int page = -1, off = 0, head = 0;
+        bool wanted = false;
+        auto ask = [&]() {
+            wanted = false;
+            if (i >= keys.n) {
                 if (!walk.next(a.plan, pc)) { have = false; return; }
                 keys = rt_keys(pc);
                 const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
                 bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
-                i = wg;
+                head = pc.head;
+                i = 0;
             }
             const int key = keys.k0 + TC_BN * i + row;
-            at = NONE;
-            hole = false;
+            ++i;
             if (key >= pc.t.key_lo && key < keys.k_end) {
                 const int index = a.kv.page_index(key);
-                const int page = index < a.kv.max_pages ? __ldg(bt + index) : -1;
-                hole = (unsigned)page >= (unsigned)a.kv.num_pages;
-                if (!hole) at = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, index);
+                wanted = true;
+                off = a.kv.offset(key, index);
+                page = index < a.kv.max_pages ? __ldg(bt + index) : -1;
             }
-            i += 2;
         };
-        // Scales and marks of a tile, into the place of its turn.  RT_META places: the tile four before has been read when this one's
+        uint32_t at = NONE;              // the lane's row among the keys
+        bool hole = false;               // a key that a row may see has no page
+        auto resolve = [&]() {
+            const bool there = (unsigned)page < (unsigned)a.kv.num_pages;
+            at = wanted && there ? a.kv.row0(page, 0, head) + off : NONE;
+            hole = wanted && !there;
+        };
+        // Scales and marks of a tile, into the place of its turn.  RT_META places: the tile four before has been read when this one's key
         // buffer is free, because S of the tile two before was issued after the softmax threads were done with the one before that.
-        auto put_meta = [&](float ks, float vs, uint32_t row_at, bool no_page) {
+        auto put_meta = [&](float ks, float vs) {
             const int x = n & (RT_META - 1);
-            if (which == 0) {
+            if (HALF) {
                 // (a value row that is not finite has the scale NaN: with the key's it reaches those who see the key and nobody else)
-                if (HALF) meta.ks[x][row] = isnan(vs) ? vs : ks;
-                const uint32_t seen = __ballot_sync(0xffffffffu, row_at != NONE);
-                if (lane == 0) meta.seen[x][half] = seen;
-                if (no_page) *a.kv.status = 1;
-            } else if (HALF) {
+                meta.ks[x][row] = isnan(vs) ? vs : ks;
                 vs = isnan(vs) ? 0.f : vs;
                 meta.vs[x][row] = vs;
                 const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(vs));
                 if (lane == 0) meta.vmax[x][half] = __uint_as_float(most);
             }
+            const uint32_t seen = __ballot_sync(0xffffffffu, at != NONE);
+            __syncwarp();
+            if (lane == 0) {
+                meta.seen[x][half] = seen;
+                rt_mbar_arrive(mb_meta + 8 * x);
+            }
+            if (hole) *a.kv.status = 1;
         };
         auto landed = [&](uint32_t x) {
             tc_fence_async_smem();
             __syncwarp();
-            if (lane == 0) {
-                rt_mbar_arrive(mb_full + 8 * (x & 1));
-                if (HALF || which == 0) rt_mbar_arrive(mb_meta + 8 * (x & (RT_META - 1)));
-            }
+            if (lane == 0) rt_mbar_arrive(mb_full + 8 * (x & 1));
         };
         auto wait_free = [&]() -> bool { return n < 2 || tc_wait_warp(mb_free + 8 * (n & 1), ((n - 2) >> 1) & 1, dead); };
-        look();
-        const unsigned char* pool = a.kv.pool;
+        ask();
+        const unsigned char* pool = a.kv.pool + (which ? (size_t)to_values * d * c8_bytes(FORM) : 0);
         if constexpr (HALF) {
             // NP neighbouring lanes read a row, 16 bytes each: load j has rows j RI .. j RI + RI - 1 of the warp's 32
             constexpr int NP = DP / 16, RI = 32 / NP;
             const int p = lane % NP, rl = lane / NP;
             const bool in = 16 * p < d;
+            const unsigned char* mine = pool + 16 * p;
+            // the 16-byte pieces (eight halves) of a row's codes 16 p .. 16 p + 15, for even and odd j (at RI = 4 the rows' swizzle differs)
+            const int c0 = rt_place<true, DP>(2 * p), c1 = rt_place<true, DP>(2 * p + 1);
+            const uint32_t to0 = buf0 + rl * 128 + (c0 >> 3) * KV_BLK, to1 = buf0 + rl * 128 + (c1 >> 3) * KV_BLK;
+            const uint32_t even0 = to0 + (((c0 & 7) ^ (rl & 7)) << 4), even1 = to1 + (((c1 & 7) ^ (rl & 7)) << 4);
+            const uint32_t odd0 = to0 + (((c0 & 7) ^ ((rl + RI) & 7)) << 4), odd1 = to1 + (((c1 & 7) ^ ((rl + RI) & 7)) << 4);
             uint4 data[NP];
             float ks = 0.f, vs = 0.f;
-            auto load = [&](int j) {
-                const uint32_t r = __shfl_sync(0xffffffffu, at, j * RI + rl);
-                data[j] = in && r != NONE ? __ldg(reinterpret_cast<const uint4*>(pool + (size_t)(which ? r + to_values : r) * d) + p)
-                                          : make_uint4(0u, 0u, 0u, 0u);
-            };
-            auto load_scales = [&]() {
-                ks = which == 0 && at != NONE ? __ldg(a.kv.scales + at) : 0.f;
-                vs = at != NONE ? __ldg(a.kv.scales + at + to_values) : 0.f;
-            };
-            if (have) {
-                load_scales();
+            auto load = [&]() {
+                uint32_t r[NP];
 #pragma unroll
-                for (int j = 0; j < NP; ++j) load(j);
+                for (int j = 0; j < NP; ++j) r[j] = __shfl_sync(0xffffffffu, at, j * RI + rl);
+#pragma unroll
+                for (int j = 0; j < NP; ++j)
+                    data[j] = in && r[j] != NONE ? __ldg(reinterpret_cast<const uint4*>(mine + (size_t)r[j] * d)) : make_uint4(0u, 0u, 0u, 0u);
+                if (which == 0) {
+                    ks = at != NONE ? __ldg(a.kv.scales + at) : 0.f;
+                    vs = at != NONE ? __ldg(a.kv.scales + at + to_values) : 0.f;
+                }
+            };
+            bool now = have;                                 // there is a tile in the registers
+            if (now) {
+                resolve();
+                load();
+                ask();
             }
-            while (have) {
-                const uint32_t mine = at;
-                const bool no_page = hole;
-                look();                                      // `at`: the next tile's (NONE behind the last one)
-                if (!have) at = NONE;
+            while (now) {
                 if (!wait_free()) break;
-                const uint32_t buf = buf0 + (n & 1) * BUF + (p >> 2) * KV_BLK;
-                put_meta(ks, vs, mine, no_page);
-                load_scales();
+                if (which == 0) put_meta(ks, vs);
+                const uint32_t b = (n & 1) * BUF;
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
                     uint32_t h[8];
@@ -364,17 +304,16 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                     c8_halves<FORM>(data[j].y, h[2], h[3]);
                     c8_halves<FORM>(data[j].z, h[4], h[5]);
                     c8_halves<FORM>(data[j].w, h[6], h[7]);
-                    load(j);                                 // the next tile's, as soon as the registers are free
-                    const uint32_t r = j * RI + rl;
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {            // eight dimensions each; the upper half of a row the other way round (banks)
-                        const bool flip = (p >> 2) & 1;
-                        const uint32_t c = (2 * p + (flip ? 1 - k : k)) & 7;
-                        const bool hi = flip ? k == 0 : k == 1;
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
-                                     ::"r"(buf + r * 128 + ((c ^ (r & 7)) << 4)), "r"(hi ? h[4] : h[0]), "r"(hi ? h[5] : h[1]),
-                                       "r"(hi ? h[6] : h[2]), "r"(hi ? h[7] : h[3]) : "memory");
-                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                 ::"r"((j & 1 ? odd0 : even0) + b + j * RI * 128), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                 ::"r"((j & 1 ? odd1 : even1) + b + j * RI * 128), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                }
+                now = have;
+                if (now) {
+                    resolve();
+                    load();                                  // under way while this tile is announced and its successor's buffer waited for
+                    ask();
                 }
                 landed(n);
                 ++n;
@@ -386,20 +325,20 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             const bool in = 8 * p < d;
             bool alive = true;
             while (have) {
+                resolve();
+                ask();
                 if (!wait_free()) { alive = false; break; }
+                if (which == 0) put_meta(0.f, 0.f);
                 const uint32_t buf = buf0 + (n & 1) * BUF + (p >> 3) * KV_BLK;
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
                     const int row_j = j * RI + rl;
                     const uint32_t r = __shfl_sync(0xffffffffu, at, row_j);
                     const bool ok = in && r != NONE;
-                    tc_cp16(buf + row_j * 128 + (((p & 7) ^ (row_j & 7)) << 4),
-                            ok ? pool + (size_t)(which ? r + to_values : r) * d * 2 + 16 * p : pool, ok);
+                    tc_cp16(buf + row_j * 128 + (((p & 7) ^ (row_j & 7)) << 4), ok ? pool + (size_t)r * d * 2 + 16 * p : pool, ok);
                 }
                 tc_cp_commit();
-                put_meta(0.f, 0.f, at, hole);
                 ++n;
-                look();
                 if (n > 1) {
                     tc_cp_wait<1>();
                     landed(n - 2);
@@ -412,31 +351,89 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(RT_REGS_SOFTMAX));
         // ---- softmax threads: thread `row` of a group has query row `row`, a lane of tensor memory
-        const int wg = warp >> 2, row = tid & 127, warp4 = warp & 3;
+        const int row = tid & 127, warp4 = warp & 3;
         const uint32_t t_wg = tmem + wg * WG_COLS + ((uint32_t)(warp4 * 32) << 16);
-        const uint32_t mb_s = bar(wg, M_S), mb_o = bar(wg, M_O), mb_meta = bar(wg, M_META);
+        const uint32_t mb_s = bar(M_S), mb_o = bar(M_O), mb_meta = bar(M_META);
         const RtMeta& meta = s_meta[wg];
         bool alive = true;
-        uint32_t n = 0;                                  // tiles of this group so far
-        RowWalk walk = s_walk;
-        RowPiece pc;
-        int k = 0;
-        for (; walk.next(a.plan, pc); ++k) {
+        uint32_t n = 0;                                  // tiles so far
+        // ---- queries.  A piece's tokens and positions are looked up a piece ahead.
+        RowPiece nx;
+        int token_n = -1, pos_n = -1;
+        auto look = [&]() -> bool {
+            if (!walk.next(a.plan, nx)) return false;
+            const int place = nx.t.first + row / g;
+            token_n = row < nx.t.n_tok * g ? (a.plan.items ? __ldg(a.plan.items + place) : place) : -1;
+            pos_n = token_n >= 0 ? __ldg(a.positions + token_n) : -1;
+            return true;
+        };
+        // The warp's 32 rows of `nx` into shared memory: NP neighbouring lanes have a row, RI rows to a load.  All S over the queries
+        // that were there are complete.  Returns the factor of this thread's row.
+        auto bring = [&]() -> float {
+            constexpr int NP = DP / 8, RI = 32 / NP;
+            float fac = a.scale_log2;
+            if (warp4 * 32 < nx.t.n_tok * g) {
+                const int p = lane % NP, rl = lane / NP;
+                const int r_own = pos_n >= 0 ? row % g : 0;
+                const long long at_own = pos_n >= 0 ? (long long)token_n * a.q_stride + (nx.head * g + r_own) * d : -1;
+                uint4 u[NP];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    const long long at = __shfl_sync(0xffffffffu, at_own, j * RI + rl);
+                    u[j] = at >= 0 && 8 * p < d ? __ldg(reinterpret_cast<const uint4*>((const bf16*)a.q + at) + p) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                const int place = rt_place<HALF, DP>(p);
+                const uint32_t dst = sQ + (place >> 3) * Q_BLK;
+                int ex_own = 0;
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    const int r = warp4 * 32 + j * RI + rl;
+                    uint32_t* w = &u[j].x;
+                    if (HALF) {
+                        // a power of two that brings the row's largest element to [2^14, 2^15)
+                        uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+                        for (int o = NP / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const int ex = min(max((int)(max(m & 0xffffu, m >> 16) >> 7) - 127, -100), 127);
+                        const int theirs = __shfl_sync(0xffffffffu, ex, (lane % RI) * NP);
+                        if (lane / RI == j) ex_own = theirs;
+                        const float mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * mul, __uint_as_float(w[i] & 0xffff0000u) * mul);
+                            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                 ::"r"(dst + r * 128 + (((place & 7) ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                }
+                if (HALF) fac = ldexpf(a.scale_log2, ex_own - 14);
+                tc_fence_async_smem();
+                __syncwarp();
+            }
+            if (lane == 0) rt_mbar_arrive(bar(M_Q));
+            return fac;
+        };
+        bool more = look();
+        float fac_n = more ? bring() : 0.f;
+        while (more) {
+            pc = nx;
             const RtKeys keys = rt_keys(pc);
-            const int mine = rt_share(keys.n, wg), rows = pc.t.n_tok * g;
-            const int head = pc.head * g + row % g;
-            if (alive) alive = tc_wait_warp(tc_smem(&s_qbar[0][k & 1]), (k >> 1) & 1, dead);
-            const int pos = s_rows[k & 1].pos[row], token = s_rows[k & 1].token[row];
-            const float fac = s_rows[k & 1].fac[row];
-            __syncwarp();
-            if (lane == 0) rt_mbar_arrive(tc_smem(&s_qbar[1][k & 1]));
-            if (wg == 1 && k > 0) rt_taken_sync();       // the first group has read this one's O of the piece before
+            const int rows = pc.t.n_tok * g, pos = pos_n, token = token_n;
+            const float fac = fac_n;
+            more = look();
+            if (warp4 * 32 >= rows) {                    // no row of this warp's is one of the tile's
+                for (int i = 0; i < keys.n; ++i) { rt_sync(wg, 0); rt_sync(wg, 1); }
+                n += keys.n;
+                if (more) fac_n = bring();
+                continue;
+            }
             const int hi = min(pos + 1, keys.k_end);
             const int lo = max(pc.t.key_lo, a.window > 0 ? pos - a.window + 1 : 0);
             float ref = -INFINITY, sum = 0.f;
-            for (int i = 0; i < mine; ++i) {
+            for (int i = 0; i < keys.n; ++i) {
                 const uint32_t x = n + i;
-                const int key0 = keys.k0 + TC_BN * (wg + 2 * i), mt = x & (RT_META - 1);
+                const int key0 = keys.k0 + TC_BN * i, mt = x & (RT_META - 1);
                 if (alive) alive = tc_wait_warp(mb_s, x & 1, dead);
                 tc_fence_after_sync();
                 float s[TC_BN];
@@ -539,72 +536,49 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                 if (alive) rt_arrive(wg, 1);
                 else rt_sync(wg, 1);
             }
-            if (mine > 0) {
-                if (alive) alive = tc_wait_warp(mb_o, (n + mine - 1) & 1, dead);
-                tc_fence_after_sync();
-            }
-            n += mine;
-            // ---- the groups' sums
-            if (wg == 1) {
-                s_mrg[0][row] = mine > 0 ? ref : -INFINITY;
-                s_mrg[1][row] = sum;
-                tc_fence_before_sync();
-                rt_share_arrive();
-            } else {
-                rt_share_sync();
-                tc_fence_after_sync();
-                const bool two = keys.n > 1;             // the second group has tiles
-                const float r1 = s_mrg[0][row], m = fmaxf(ref, r1);
-                const float a0 = ar_weight(ref, m), a1 = ar_weight(r1, m);
-                const float l = sum * a0 + s_mrg[1][row] * a1;
-                const bool direct = a.direct && pc.whole, mine_to_store = row < rows && pos >= 0 && alive;
-                const size_t slot = ((size_t)(pc.unit + blockIdx.x)) * AR_ROWS + row;
-                if (!direct && row < rows) { a.parts.r[slot] = m; a.parts.l[slot] = l; }
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                bf16* out = (bf16*)a.out + ((size_t)(token >= 0 ? token : 0) * a.plan.nh + head) * d;
-                float* part = a.parts.o + slot * d;
+            if (more) fac_n = bring();
+            if (alive) alive = tc_wait_warp(mb_o, (n + keys.n - 1) & 1, dead);
+            tc_fence_after_sync();
+            n += keys.n;
+            // ---- the piece's sums: out, or into its slot
+            const bool direct = a.direct && pc.whole, store = row < rows && pos >= 0 && alive;
+            const size_t slot = ((size_t)(pc.unit + 2 * blockIdx.x + wg)) * AR_ROWS + row;
+            if (!direct && row < rows) { a.parts.r[slot] = ref; a.parts.l[slot] = sum; }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            bf16* out = (bf16*)a.out + ((size_t)(token >= 0 ? token : 0) * a.plan.nh + pc.head * g + row % g) * d;
+            float* part = a.parts.o + slot * d;
 #pragma unroll
-                for (int cb = 0; cb < DP / 16; ++cb) {
-                    float o[16], o1[16];
-                    uint32_t* r0 = reinterpret_cast<uint32_t*>(o);
-                    uint32_t* r1p = reinterpret_cast<uint32_t*>(o1);
-                    const uint32_t t0 = t_wg + T_O + cb * 16, t1 = t0 + WG_COLS;
-#define RT_LD16(r, t)                                                                                                              \
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"         \
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),     \
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(t) : "memory")
-                    __syncwarp();
-                    RT_LD16(r0, t0);
-                    if (two) RT_LD16(r1p, t1);
-                    tc_ld_wait();
-                    if (cb * 16 >= d) continue;
+            for (int cb = 0; cb < DP / 32; ++cb) {
+                float o[32];
+                __syncwarp();
+                tc_ld32(t_wg + T_O + cb * 32, o);
+                tc_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = o[e] * a0 + (two ? o1[e] * a1 : 0.f);
-                    if (mine_to_store && direct) {
+                for (int c = 0; c < 4; ++c) {
+                    // the piece of eight dimensions that is kept at place 4 cb + c
+                    const int at = 4 * cb + c, e = 8 * (HALF && DP == 128 ? (at & 7) * 2 + (at >> 3) : at);
+                    if (!store || e >= d) continue;
+                    const float* v = o + 8 * c;
+                    if (direct) {
+                        uint32_t h[4];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 8) {
-                            uint32_t h[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const __nv_bfloat162 b = __floats2bfloat162_rn(o[e + 2 * j] * inv, o[e + 2 * j + 1] * inv);
-                                h[j] = *reinterpret_cast<const uint32_t*>(&b);
-                            }
-                            *reinterpret_cast<uint4*>(out + cb * 16 + e) = make_uint4(h[0], h[1], h[2], h[3]);
+                        for (int j = 0; j < 4; ++j) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j] * inv, v[2 * j + 1] * inv);
+                            h[j] = *reinterpret_cast<const uint32_t*>(&b);
                         }
-                    } else if (mine_to_store) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) store4(part + cb * 16 + e, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                        *reinterpret_cast<uint4*>(out + e) = make_uint4(h[0], h[1], h[2], h[3]);
+                    } else {
+                        store4(part + e, make_float4(v[0], v[1], v[2], v[3]));
+                        store4(part + e + 4, make_float4(v[4], v[5], v[6], v[7]));
                     }
                 }
-                tc_fence_before_sync();
-                __syncwarp();
-                rt_taken_arrive();
             }
+            tc_fence_before_sync();
         }
-        if (wg == 1 && k > 0) rt_taken_sync();
     }
     tc_fence_before_sync();
-    asm volatile("bar.sync 7, %0;\n" ::"n"(RT_THREADS) : "memory");
+    __syncwarp();
+    asm volatile("bar.sync 5, %0;\n" ::"n"(RT_THREADS) : "memory");
     if (s_dead && tid == 0) atomicExch(a.kv.status, 3);
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
@@ -622,8 +596,8 @@ template <int FORM, int DP> static int rt_run(const RowArgs& a, cudaStream_t s) 
         if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
         have = attr.numRegs;
     }
-    if (have * RT_THREADS < 256 * RT_REGS_SOFTMAX + 384 * RT_REGS_OTHER) return ST_ERR_TOO_LARGE;
-    kernel<<<a.plan.ctas, RT_THREADS, smem, s>>>(a);
+    if (have * RT_THREADS < RT_REGS_ALL) return ST_ERR_TOO_LARGE;
+    kernel<<<(a.plan.ctas + 1) / 2, RT_THREADS, smem, s>>>(a);
     return st_launch_status();
 }
 
