@@ -1,23 +1,28 @@
 // Attention of single query tokens over paged caches in 8 and 16 bits (and, in 16 bits, of the keys behind a shared prefix): one
-// block per (token, key head, up to 8 or 16 of its query heads, share of the keys).
+// block per (token, key head, up to eight of its query heads, share of the keys).
 //
 // Mathematics: s_j = (q . c_j) ks_j, o = sum_j p_j vs_j c'_j / sum_j p_j with the codes c, c' and the rows' scales ks, vs: the
 // scales leave both products, whose operands are then exact in 16 bits: codes of either 8-bit form are halves; a bfloat16 query
 // is scaled by a power of two per row, so that its largest element lies in [2^14, 2^15), and is a half unless an element is
 // 2^-29 of that or less; a float query is the sum of two halves (22 bits; the rest, 2^-23 of an element, is below what 32-bit
-// sums round away).  Products go to mma.sync (m16n8k16: 8 or 16 query rows on the row side, eight keys or eight dimensions on
-// the other), sums are float.  The weights are p_j vs_j in a half of 2^-11 (for float queries and bfloat16 caches in two
-// numbers, the lower one in the row operand's other eight rows, which costs no instruction).
+// sums round away).  The weights are p_j vs_j in a half of 2^-11, for float queries and for up to four heads over bfloat16 caches in
+// two numbers.  Sums are float.
+//
+// Products are mma.sync (m16n8k16) with sixteen keys, then sixteen dimensions, on the row side, whose operand takes four
+// registers, all of them data, and the query heads as the eight columns: S^T = K Q^T, O^T += V^T P^T.  (With the heads on the row side
+// half of that operand is zeros, which have to be moved into place: 630 instructions for 16 keys of 128 dimensions; this
+// way 300.)  Two numbers of a head are columns h and h + 4.
 //
 // p_j = 2^(s_j - R): R follows the largest of s_j + log2 vs_j in steps: it moves when that exceeds R + 15, and then to 11 below, so
-// that p_j vs_j stays below 2^15 and what is 2^-24 of the largest still has a half's full precision.  Sums of 32 (16) keys are formed
-// in fresh accumulators and added to the running ones with a float add each: tensor cores cut what they add to a large sum.
+// that p_j vs_j stays below 2^15 and what is 2^-24 of the largest still has a half's full precision.  For float queries the values' sums
+// of 32 (16) keys are formed in fresh accumulators and added to the running ones with a float add each: tensor cores cut
+// what they add to a large sum.
 //
 // Layout: no shared memory on the way in.  A warp walks every n-th run of KT = 32 keys (16 where rows are longer than 64 bytes).
-// Lane (g, t) = (lane / 4, lane % 4) reads of each key row that is its column g of a product a quarter in pieces of 16 bytes
-// (the order of the summed dimensions is free, the query's is the same), and of the values of KT/4 neighbouring keys an
-// eighth of the row.  Keys are dealt to columns so that the KT/4 keys of lane t's scores are those whose values it reads:
-// scores, weights and values meet without an exchange between lanes, and each lane looks up two pages per run.
+// Lane (g, t) = (lane / 4, lane % 4) reads of the key rows that are rows g and g + 8 of a product a quarter in pieces of 16
+// bytes (the order of the summed dimensions is free, the query's is the same), and of the values of KT/4 neighbouring keys an
+// eighth of the row.  Keys are dealt to rows so that a lane's values are of neighbouring keys and each lane looks up one page per run;
+// the weights change lanes in one transposition (movmatrix) per 8 x 8.
 //
 // Bound by memory.  What the loads in flight need is covered by many warps: keys of the next run are asked for as soon as this run's
 // products have taken theirs, values likewise.
@@ -120,13 +125,17 @@ __device__ __forceinline__ void sg_finish(const SingleArgs& a, float* smem, int 
     if (a.splits > 1) sg_cluster_sync();               // nobody leaves while others read here
 }
 
-__device__ __forceinline__ void sg_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1, bool half) {
-    if (half)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c = a b (+ c)
+template <bool HALF, bool ADD> __device__ __forceinline__ void sg_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    const float z0 = ADD ? c[0] : 0.f, z1 = ADD ? c[1] : 0.f, z2 = ADD ? c[2] : 0.f, z3 = ADD ? c[3] : 0.f;
+    if (HALF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
 }
 template <bool HALF> __device__ __forceinline__ uint32_t sg_pack(float a, float b) {
     if (HALF) {
@@ -154,16 +163,22 @@ template <int N> __device__ __forceinline__ void sg_load(const unsigned char* p,
     }
 }
 
-// FORM: the cache's; QT: query and output type; D: head size; WIDE: 16 query rows instead of 8 (bfloat16 queries, 8-bit forms and
-// bfloat16).  Pages hold a multiple of 8 positions.
-template <int FORM, typename QT, int D, bool WIDE>
+__device__ __forceinline__ uint32_t sg_transpose(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// FORM: the cache's; QT: query and output type; D: head size; TWO: weights (and float queries) in two numbers, four heads to a block
+// instead of eight.  Pages hold a multiple of 8 positions.
+template <int FORM, typename QT, int D, bool TWO>
 __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(const SingleArgs a) {
     constexpr bool HALF = FORM != C8_BF16;
-    constexpr bool TWO = sizeof(QT) == 4 || (!HALF && !WIDE);    // the weights in two numbers
-    constexpr bool FLOATQ = sizeof(QT) == 4;                     // the query in two numbers
+    constexpr bool FLOATQ = sizeof(QT) == 4;
+    static_assert(TWO || !FLOATQ, "");
     constexpr int B = c8_bytes(FORM), ROW = D * B;
-    constexpr int KT = ROW <= 64 ? 32 : 16, NK = KT / 4, JT = KT / 8;   // keys of a run, keys of a lane, columns of eight
-    constexpr int R = WIDE ? 16 : 8;                             // query rows
+    constexpr int KT = ROW <= 64 ? 32 : 16, NK = KT / 4, MT = KT / 16;   // keys of a run, keys of a lane, products over 16 keys
+    constexpr int R = TWO ? 4 : 8;                               // query heads
     constexpr int NS = D / 16;                                   // products over 16 dimensions
     constexpr int KW = ROW / 16;                                 // words of a key row a lane reads: a quarter
     constexpr int VW = (D / 8 * B + 3) / 4;                      // words of a value row a lane reads: an eighth (D = 80: 2.5 or 5)
@@ -185,279 +200,314 @@ __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(co
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    // ---- the query's fragments: dimension of summand k of product s, as the key rows are read
-    // pieces of 16 bytes per lane while the row lasts, then 8, then 4
-    auto key_byte = [&](int w) -> int {                          // offset of this lane's word w in a key row
+    // offset of this lane's word w in a key row: pieces of 16 bytes per lane while the row lasts, then 8, then 4
+    auto key_byte = [&](int w) -> int {
         constexpr int full = KW / 4 * 4, two = KW % 4 / 2 * 2;
         if (w < full) return (w / 4) * 64 + t * 16 + (w % 4) * 4;
         if (w < full + two) return full * 16 + t * 8 + (w - full) * 4;
         return (full + two) * 16 + t * 4;
     };
-    uint32_t qa[NS][4];
-    float fac[WIDE ? 2 : 1];
-    {
-        const QT* q = (const QT*)a.q + ((size_t)token * a.nh + head0) * D;
-#pragma unroll
-        for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
-            const int r = g + 8 * half;
-            const bool ok = r < rows;
-            float mul = 1.f;
-            float v[NS][4];
-            uint32_t amax = 0;
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // element 4 s + k of the lane's quarter row: a word holds 4 / B of them
-                    const int e = 4 * s + k, dim = key_byte(e * B / 4) / B + e % (4 / B);
-                    v[s][k] = ok ? to_f32(q[(size_t)r * D + dim]) : 0.f;
-                    amax = max(amax, __float_as_uint(v[s][k]) & 0x7fffffffu);
-                }
-            fac[half] = a.scale_log2;
-            if (HALF) {
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int ex = min(max((int)(amax >> 23) - 127, -100), 127);
-                mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-                fac[half] = ldexpf(a.scale_log2, ex - 14);
-            }
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const float x = v[s][2 * p] * mul, y = v[s][2 * p + 1] * mul;
-                    const uint32_t w = sg_pack<HALF>(x, y);
-                    qa[s][2 * p + half] = w;
-                    if (!WIDE) {
-                        const float2 f = sg_unpack<HALF>(w);
-                        qa[s][2 * p + 1] = FLOATQ ? sg_pack<HALF>(x - f.x, y - f.y) : 0u;
-                    }
-                }
-        }
-    }
-    constexpr int H = WIDE ? 2 : 1;
-    float ref[H], sum[H], acc[NT][2 * H];
-#pragma unroll
-    for (int h = 0; h < H; ++h) { ref[h] = -INFINITY; sum[h] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int k = 0; k < 2 * H; ++k) acc[i][k] = 0.f;
-
     const int base0 = lo & ~7, runs = hi > base0 ? (hi - base0 + KT - 1) / KT : 0, stride = W * a.splits;
-    // the page and place of this lane's column g (keys) and of its own keys (values, scales) in run i: the first position of
-    // an aligned block of eight or four keys, which one page holds
-    auto look = [&](int i, int& kpage, int& koff, int& vpage, int& voff) {
-        kpage = vpage = -1;
-        koff = voff = 0;
-        if (i >= runs) return;
-        const int b = base0 + i * KT, kk = b + (g >> 1) * NK, vk = b + t * NK;
-        if (kk < hi) { kpage = a.kv.page(bt, kk); koff = a.kv.offset(kk, a.kv.page_index(kk)); }
-        if (vk < hi) {
-            vpage = a.kv.page(bt, vk);
-            voff = a.kv.offset(vk, a.kv.page_index(vk));
-            if (vpage < 0 && vk + NK > lo && a.kv.status) *a.kv.status = 1;
+    // A run's keys are four aligned blocks of NK, each within a page.  Lane (g, t) looks up block t, two runs ahead (ask), and
+    // turns the page into a row of the pool one run ahead (resolve); its rows' keys are in block g / 2, whose row lane g / 2 has.
+    constexpr uint32_t NONE = 0xffffffffu;
+    const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
+    int page = -1, off = 0;
+    auto ask = [&](int i) {
+        const int key = base0 + i * KT + t * NK;
+        page = -1;
+        if (key < hi) {
+            const int index = a.kv.page_index(key);
+            off = a.kv.offset(key, index);
+            if (index < a.kv.max_pages) page = __ldg(bt + index);
         }
     };
-    uint32_t kw[JT][KW], vw[NK][VW];
-    float ks[NK], vs[NK];
-    auto load_keys = [&](int page, int off) {
-        const uint32_t row = page < 0 ? 0u : a.kv.row0(page, 0, key_head) + off + (g & 1);
-        const unsigned char* p = a.kv.pool + (size_t)row * ROW;
+    auto resolve = [&](int i) -> uint32_t {
+        const int key = base0 + i * KT + t * NK;
+        if (key >= hi) return NONE;
+        if ((unsigned)page >= (unsigned)a.kv.num_pages) {
+            if (key + NK > lo && a.kv.status) *a.kv.status = 1;
+            return NONE;
+        }
+        return a.kv.row0(page, 0, key_head) + off;
+    };
+    uint32_t kw[2 * MT][KW], vw[NK][VW];
+    float ks[2 * MT], vs[2 * MT];                                // of the keys of this lane's scores
+    const unsigned char* const key_pool = a.kv.pool + (g & 1) * ROW;
+    const unsigned char* const value_pool = a.kv.pool + (size_t)to_values * ROW;
+    auto load_keys = [&](uint32_t r) {                           // the row of block g / 2
+        const unsigned char* p = key_pool + (size_t)(r != NONE ? r : 0u) * ROW;
+        if (r != NONE) {
 #pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            constexpr int full = KW / 4 * 4, two = KW % 4 / 2 * 2;
-            if (page >= 0) {
+            for (int j = 0; j < 2 * MT; ++j) {
+                constexpr int full = KW / 4 * 4, two = KW % 4 / 2 * 2;
                 const unsigned char* pj = p + 2 * j * ROW;
 #pragma unroll
                 for (int w = 0; w < full; w += 4) sg_load<4>(pj + key_byte(w), kw[j] + w);
                 if constexpr (two > 0) sg_load<2>(pj + key_byte(full), kw[j] + full);
                 if constexpr (full + two < KW) sg_load<1>(pj + key_byte(full + two), kw[j] + full + two);
-            } else {
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * MT; ++j)
 #pragma unroll
                 for (int w = 0; w < KW; ++w) kw[j][w] = 0u;
-            }
         }
     };
-    // an eighth of a value row: of every 64 dimensions eight neighbours, then of 32 four, of 16 two
-    constexpr int V8 = D / 64, V4 = D % 64 / 32, V2 = D % 32 / 16;
-    auto value_dim = [&](int n, int i) -> int {                 // dimension of column n of the i-th product of values
-        if (i < 8 * V8) return (i >> 3) * 64 + n * 8 + (i & 7);
-        if (i < 8 * V8 + 4 * V4) return 64 * V8 + n * 4 + (i - 8 * V8);
-        return 64 * V8 + 32 * V4 + n * 2 + (i - 8 * V8 - 4 * V4);
+    auto load_scales = [&](uint32_t r) {
+        if (HALF) {
+            const float* sc = a.kv.scales + (r != NONE ? r : 0u) + (g & 1);
+#pragma unroll
+            for (int j = 0; j < 2 * MT; ++j) { ks[j] = __ldg(sc + 2 * j); vs[j] = __ldg(sc + to_values + 2 * j); }
+        }
     };
-    auto load_values = [&](int page, int off, int key) {        // key: the first of the lane's keys
-        const uint32_t row = page < 0 ? 0u : a.kv.row0(page, 1, key_head) + off;
+    // an eighth of a value row: of every 128 (8-bit forms) or 64 dimensions 16 or 8 neighbours, of 32 four, of 16 two
+    constexpr int V16 = B == 1 ? D / 128 : 0, V8 = (D - 128 * V16) / 64, V4 = D % 64 / 32, V2 = D % 32 / 16;
+    auto value_dim = [&](int n, int i) -> int {                 // the i-th dimension that lanes of g = n read
+        if (i < 16 * V16) return n * 16 + i;
+        if (i < 16 * V16 + 8 * V8) return 128 * V16 + ((i - 16 * V16) >> 3) * 64 + n * 8 + (i & 7);
+        if (i < 16 * V16 + 8 * V8 + 4 * V4) return 128 * V16 + 64 * V8 + n * 4 + (i - 16 * V16 - 8 * V8);
+        return 128 * V16 + 64 * V8 + 32 * V4 + n * 2 + (i - 16 * V16 - 8 * V8 - 4 * V4);
+    };
+    auto load_value = [&](const unsigned char* p, int k) {
+        if constexpr (V16) sg_load<4>(p + g * 16, vw[k]);
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const unsigned char* p = a.kv.pool + (size_t)(row + k) * ROW;
-            if (page >= 0 && key + k >= lo && key + k < hi) {
+        for (int c = 0; c < V8; ++c) {
+            if constexpr (B == 1) sg_load<2>(p + V16 * 128 + c * 64 + g * 8, vw[k] + 4 * V16 + 2 * c);
+            else sg_load<4>(p + c * 128 + g * 16, vw[k] + 4 * c);
+        }
+        if constexpr (V4) {
+            if constexpr (B == 1) sg_load<1>(p + V8 * 64 + g * 4, vw[k] + 2 * V8);
+            else sg_load<2>(p + V8 * 128 + g * 8, vw[k] + 4 * V8);
+        }
+        if constexpr (V2) {
+            if constexpr (B == 1) vw[k][VW - 1] = __ldg(reinterpret_cast<const unsigned short*>(p + V8 * 64 + V4 * 32 + g * 2));
+            else sg_load<1>(p + V8 * 128 + V4 * 64 + g * 4, vw[k] + VW - 1);
+        }
+    };
+    auto load_values = [&](uint32_t at, int key, bool all) {    // key: the first of block t's; all: none of the warp's is hidden
+        const unsigned char* p = value_pool + (size_t)(at != NONE ? at : 0u) * ROW;
+        if (all) {
 #pragma unroll
-                for (int c = 0; c < V8; ++c) {
-                    if constexpr (B == 1) sg_load<2>(p + c * 64 + g * 8, vw[k] + 2 * c);
-                    else sg_load<4>(p + c * 128 + g * 16, vw[k] + 4 * c);
-                }
-                if constexpr (V4) {
-                    if constexpr (B == 1) sg_load<1>(p + V8 * 64 + g * 4, vw[k] + 2 * V8);
-                    else sg_load<2>(p + V8 * 128 + g * 8, vw[k] + 4 * V8);
-                }
-                if constexpr (V2) {
-                    if constexpr (B == 1) vw[k][VW - 1] = __ldg(reinterpret_cast<const unsigned short*>(p + V8 * 64 + V4 * 32 + g * 2));
-                    else sg_load<1>(p + V8 * 128 + V4 * 64 + g * 4, vw[k] + VW - 1);
-                }
-            } else {
+            for (int k = 0; k < NK; ++k) load_value(p + k * ROW, k);
+        } else {
+            // hidden rows may hold anything: zeros in their place
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
 #pragma unroll
                 for (int w = 0; w < VW; ++w) vw[k][w] = 0u;
+                if (at != NONE && key + k >= lo && key + k < hi) load_value(p + k * ROW, k);
             }
         }
     };
-    auto load_scales = [&](int page, int off) {
-        if (!HALF || page < 0) {
-#pragma unroll
-            for (int k = 0; k < NK; ++k) ks[k] = vs[k] = 1.f;
-            return;
-        }
-        const float* k0 = a.kv.scales + a.kv.row0(page, 0, key_head) + off;
-        const float* v0 = a.kv.scales + a.kv.row0(page, 1, key_head) + off;
-#pragma unroll
-        for (int k = 0; k < NK; k += 4) {
-            const float4 x = __ldg(reinterpret_cast<const float4*>(k0 + k)), y = __ldg(reinterpret_cast<const float4*>(v0 + k));
-            ks[k] = x.x; ks[k + 1] = x.y; ks[k + 2] = x.z; ks[k + 3] = x.w;
-            vs[k] = y.x; vs[k + 1] = y.y; vs[k + 2] = y.z; vs[k + 3] = y.w;
-        }
-    };
+    auto sees_all = [&](uint32_t at, int key) -> bool { return __all_sync(0xffffffffu, at != NONE && key >= lo && key + NK <= hi); };
 
+    // the first run's loads leave before the query's
     int i = split * W + warp;
-    int kpage, koff, vpage, voff, kpage1, koff1, vpage1, voff1;
-    look(i, kpage, koff, vpage, voff);
-    load_keys(kpage, koff);
-    load_values(vpage, voff, base0 + i * KT + t * NK);
-    load_scales(vpage, voff);
-    look(i + stride, kpage1, koff1, vpage1, voff1);
-    for (; i < runs; i += stride) {
-        const int key0 = base0 + i * KT + t * NK;                // the lane's keys: key0 .. key0 + NK - 1
-        // ---- scores: column n of product j is key (n / 2) NK + 2 j + n % 2 of the run
-        float s[JT][4];
+    ask(i);
+    uint32_t at = resolve(i), at_k = __shfl_sync(0xffffffffu, at, g >> 1);
+    bool all = sees_all(at, base0 + i * KT + t * NK);
+    load_keys(at_k);
+    load_scales(at_k);
+    load_values(at, base0 + i * KT + t * NK, all);
+    ask(i + stride);
+
+    // ---- the query's fragments: column g is head g (TWO: head g % 4, its second number from column 4 on)
+    uint32_t qb[NS][2];
+    float fac[2] = {a.scale_log2, a.scale_log2};                 // of the heads of columns 2 t and 2 t + 1
+    {
+        const int r = TWO ? g & 3 : g;
+        const bool ok = r < rows;
+        const QT* q = (const QT*)a.q + ((size_t)token * a.nh + head0 + (ok ? r : 0)) * D;
+        float v[NS][4];
+        uint32_t amax = 0;
 #pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        for (int x = 0; x < NS; ++x)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // element 4 x + k of the lane's quarter row: a word holds 4 / B of them
+                const int e = 4 * x + k, dim = key_byte(e * B / 4) / B + e % (4 / B);
+                v[x][k] = ok ? to_f32(q[dim]) : 0.f;
+                amax = max(amax, __float_as_uint(v[x][k]) & 0x7fffffffu);
+            }
+        float mul = 1.f;
+        if (HALF) {
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int ex = min(max((int)(amax >> 23) - 127, -100), 127);
+            mul = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+            const float f = ldexpf(a.scale_log2, ex - 14);
+            fac[0] = __shfl_sync(0xffffffffu, f, 8 * t);
+            fac[1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+        }
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const float y = v[x][2 * p] * mul, z = v[x][2 * p + 1] * mul;
+                uint32_t w = sg_pack<HALF>(y, z);
+                if (FLOATQ) {
+                    const float2 f = sg_unpack<HALF>(w);
+                    if (g >= 4) w = sg_pack<HALF>(y - f.x, z - f.y);
+                }
+                qb[x][p] = w;
+            }
+    }
+    float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[NT / 2][4];
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[j][k] = 0.f;
+
+    for (; i < runs; i += stride) {
+        const int next0 = base0 + (i + stride) * KT + t * NK;
+        const uint32_t at1 = resolve(i + stride), at1_k = __shfl_sync(0xffffffffu, at1, g >> 1);
+        // ---- scores: rows g and g + 8 of product m are keys 4 m + g % 2 and 4 m + g % 2 + 2 of block g / 2
+        float s[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int x = 0; x < NS; ++x) {
-                uint32_t b0, b1;
-                if constexpr (HALF) c8_halves<FORM>(kw[j][x], b0, b1);
-                else { b0 = kw[j][2 * x]; b1 = kw[j][2 * x + 1]; }
-                sg_mma(s[j], qa[x], b0, b1, HALF);
+                uint32_t f[4];
+                if constexpr (HALF) {
+                    c8_halves<FORM>(kw[2 * m][x], f[0], f[2]);
+                    c8_halves<FORM>(kw[2 * m + 1][x], f[1], f[3]);
+                } else {
+                    f[0] = kw[2 * m][2 * x]; f[2] = kw[2 * m][2 * x + 1];
+                    f[1] = kw[2 * m + 1][2 * x]; f[3] = kw[2 * m + 1][2 * x + 1];
+                }
+                if (x == 0) sg_mma<HALF, false>(s[m], f, qb[x][0], qb[x][1]);
+                else sg_mma<HALF, true>(s[m], f, qb[x][0], qb[x][1]);
             }
-        }
-        load_keys(kpage1, koff1);
-        // ---- their softmax's numbers: this lane's NK keys of row g (and g + 8)
-        float lead = 0.f;                                        // log2 of the largest value scale, rounded up
-        if (HALF) {
-            float vmax = 0.f;
+        load_keys(at1_k);
+        ask(i + 2 * stride);
+        // ---- softmax's numbers: s[m][c], s[m][2 + c] are column 2 t + c at keys 2 m and 2 m + 1 of ks and vs
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                if (vpage < 0 || key0 + k < lo || key0 + k >= hi) vs[k] = 0.f;
-                vmax = fmaxf(vmax, vs[k]);
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (FLOATQ) s[m][k] += __shfl_xor_sync(0xffffffffu, s[m][k], 2);
+                if (HALF) s[m][k] *= ks[2 * m + (k >> 1)];
             }
-            lead = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -90);
-        }
-        float corr[H];
-        uint32_t pa[KT / 16][4];
+        if (!all) {
+            const int key = base0 + i * KT + (g >> 1) * NK + (g & 1);
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            float z[NK], mx = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                float v = s[k >> 1][2 * h + (k & 1)];
-                if (FLOATQ) v += s[k >> 1][2 + (k & 1)];
-                if (HALF) v *= ks[k];
-                v *= fac[h];
-                if (vpage < 0 || key0 + k < lo || key0 + k >= hi) v = -INFINITY;
-                z[k] = v;
-                mx = fmaxf(mx, v);
-            }
-            mx += lead;
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            corr[h] = 1.f;
-            if (mx > ref[h] + 15.f) {
-                const float r = mx - 11.f;
-                corr[h] = ar_exp2(ref[h] - r);                   // 0 from "no key yet"
-                ref[h] = r;
-            }
-            const float use = ref[h] == -INFINITY ? 0.f : ref[h];
-            float l = 0.f;
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                const float p = ar_exp2(z[k] - use);
-                l += p;
-                z[k] = HALF ? p * vs[k] : p;
-            }
-            // (a row that is not finite has the scale NaN; where it is masked its weight is zero, not NaN: vs is 0 there)
-            sum[h] = sum[h] * corr[h] + l;
-#pragma unroll
-            for (int m = 0; m < KT / 16; ++m)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const float x = z[4 * m + 2 * p], y = z[4 * m + 2 * p + 1];
-                    const uint32_t w = sg_pack<HALF>(x, y);
-                    pa[m][2 * p + h] = w;
-                    if (!WIDE) {
-                        const float2 f = sg_unpack<HALF>(w);
-                        pa[m][2 * p + 1] = TWO ? sg_pack<HALF>(x - f.x, y - f.y) : 0u;
-                    }
+            for (int j = 0; j < 2 * MT; ++j)
+                if (at_k == NONE || key + 2 * j < lo || key + 2 * j >= hi) {
+                    vs[j] = 0.f;                                 // (a row that is not finite has the scale NaN)
+                    s[j >> 1][2 * (j & 1)] = s[j >> 1][2 * (j & 1) + 1] = -INFINITY;
                 }
         }
-        // ---- weights times values
+        float lead = 0.f;                                        // log2 of the largest value scale, rounded up
+        if (HALF) {
+            float vmax = vs[0];
+#pragma unroll
+            for (int j = 1; j < 2 * MT; ++j) vmax = fmaxf(vmax, vs[j]);
+            lead = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -90);
+        }
+        float corr[2];
+        bool move = false;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(s[0][c], s[0][2 + c]);
+            if constexpr (MT == 2) mx = fmaxf(mx, fmaxf(s[MT - 1][c], s[MT - 1][2 + c]));
+            mx = fmaf(mx, fac[c], lead);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            corr[c] = 1.f;
+            if (mx > ref[c] + 15.f) {
+                const float r = mx - 11.f;
+                corr[c] = ar_exp2(ref[c] - r);                   // 0 from "no key yet"
+                ref[c] = r;
+                move = true;
+            }
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                sum[c] *= corr[c];
+#pragma unroll
+                for (int j = 0; j < NT / 2; ++j) { acc[j][c] *= corr[c]; acc[j][2 + c] *= corr[c]; }
+            }
+        }
+        uint32_t pb[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                        // keys of rows g, of rows g + 8
+                float z[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float neg = ref[c] == -INFINITY ? 0.f : -ref[c];
+                    const float p = ar_exp2(fmaf(s[m][2 * h + c], fac[c], neg));
+                    sum[c] += p;
+                    z[c] = HALF ? p * vs[2 * m + h] : p;
+                }
+                uint32_t w = sg_pack<HALF>(z[0], z[1]);
+                if (TWO) {
+                    const float2 f = sg_unpack<HALF>(w);
+                    if (t >= 2) w = sg_pack<HALF>(z[0] - f.x, z[1] - f.y);
+                }
+                pb[m][h] = sg_transpose(w);
+            }
+        load_scales(at1_k);
+        // ---- values times weights: rows g and g + 8 of product j are this lane's dimensions 2 j and 2 j + 1
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
             constexpr int PER = 4 / B;                           // dimensions of a word
-            uint32_t b[KT / 16][2][4];
+            uint32_t b[MT][2][4];
 #pragma unroll
-            for (int m = 0; m < KT / 16; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint32_t x = vw[4 * m + 2 * p][w], y = vw[4 * m + 2 * p + 1][w];
-                    if constexpr (HALF) c8_pairs<FORM>(x, y, b[m][p]);
-                    else { b[m][p][0] = __byte_perm(x, y, 0x5410); b[m][p][1] = __byte_perm(x, y, 0x7632); }
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x = vw[4 * m + 2 * h][w], y = vw[4 * m + 2 * h + 1][w];
+                    if constexpr (HALF) c8_pairs<FORM>(x, y, b[m][h]);
+                    else { b[m][h][0] = __byte_perm(x, y, 0x5410); b[m][h][1] = __byte_perm(x, y, 0x7632); }
                 }
 #pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                const int n = w * PER + c;
-                if (n < NT) {
-                    float o[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < PER; c += 2) {
+                const int j = (w * PER + c) / 2;
+                if (2 * j < NT) {
+                    float o[4];
 #pragma unroll
-                    for (int m = 0; m < KT / 16; ++m) sg_mma(o, pa[m], b[m][0][c], b[m][1][c], HALF);
+                    for (int m = 0; m < MT; ++m) {
+                        const uint32_t f[4] = {b[m][0][c], b[m][0][c + 1], b[m][1][c], b[m][1][c + 1]};
+                        if (!FLOATQ) sg_mma<HALF, true>(acc[j], f, pb[m][0], pb[m][1]);
+                        else if (m == 0) sg_mma<HALF, false>(o, f, pb[m][0], pb[m][1]);
+                        else sg_mma<HALF, true>(o, f, pb[m][0], pb[m][1]);
+                    }
+                    if (FLOATQ) {
 #pragma unroll
-                    for (int h = 0; h < H; ++h)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            acc[n][2 * h + k] = acc[n][2 * h + k] * corr[h] + (TWO ? o[k] + o[2 + k] : o[2 * h + k]);
+                        for (int k = 0; k < 4; ++k) acc[j][k] += o[k];
+                    }
                 }
             }
         }
-        const int next0 = base0 + (i + stride) * KT + t * NK;
-        load_values(vpage1, voff1, next0);
-        load_scales(vpage1, voff1);
-        vpage = vpage1;
-        look(i + 2 * stride, kpage1, koff1, vpage1, voff1);
+        at = at1;
+        at_k = at1_k;
+        all = sees_all(at, next0);
+        load_values(at, next0, all);
     }
     // ---- parts to shared memory
     float* s_ref = smem;
     float* s_sum = s_ref + W * R;
     float* s_acc = s_sum + W * R;
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        float l = sum[h];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const int r = g + 8 * h;
-        if (t == 0) { s_ref[warp * R + r] = ref[h]; s_sum[warp * R + r] = l; }
-        if (r < rows) {
-            float* o = s_acc + ((size_t)warp * R + r) * D;
+    for (int c = 0; c < 2; ++c) {
+        float l = sum[c];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) { o[value_dim(2 * t, n)] = acc[n][2 * h]; o[value_dim(2 * t + 1, n)] = acc[n][2 * h + 1]; }
-        }
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int r = 2 * t + c;
+        if (g == 0 && r < R) { s_ref[warp * R + r] = ref[c]; s_sum[warp * R + r] = l; }
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float o = acc[j][2 * h + c];
+                if (TWO) o += __shfl_xor_sync(0xffffffffu, o, 2);
+                if (r < rows) s_acc[((size_t)warp * R + r) * D + value_dim(g, 2 * j + h)] = o;
+            }
     }
     sg_finish<QT>(a, smem, W, R, rows, D, token, item, head0, key_head);
 }
@@ -494,36 +544,23 @@ static inline int sg_launch(const char* tag, K kernel, const SingleArgs& a, int 
     return st_launch_status();
 }
 
-template <int FORM, typename QT, int D, bool WIDE>
+template <int FORM, typename QT, int D, bool TWO>
 static int sg_run(SingleArgs a, int max_keys, cudaStream_t s) {
-    constexpr int R = WIDE ? 16 : 8, KT = D * c8_bytes(FORM) <= 64 ? 32 : 16;
+    constexpr int R = TWO ? 4 : 8, KT = D * c8_bytes(FORM) <= 64 ? 32 : 16;
     a.row_blocks = (a.group + R - 1) / R;
     const int grid_y = a.row_blocks * a.kv.nkv;
     const SingleShape shape = sg_shape((long long)a.n_items * grid_y, max_keys, KT);
     a.splits = shape.splits;
     const size_t smem = (size_t)shape.warps * R * (D + 2) * 4;
-    AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, WIDE>), smem);
-    return sg_launch("single8", attention_single8_kernel<FORM, QT, D, WIDE>, a, shape.warps, smem, grid_y, s);
+    AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO>), smem);
+    return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO>, a, shape.warps, smem, grid_y, s);
 }
-template <int FORM, typename QT>
-static int sg_run(const SingleArgs& a, int max_keys, cudaStream_t s) {
-    // 16 rows where a key head has more than eight query heads; a float query needs the other eight for its lower half
-    const bool wide = sizeof(QT) == 2 && a.group > 8;
-    if constexpr (sizeof(QT) == 2) {
-        if (wide) {
-            if (a.d == 32) return sg_run<FORM, QT, 32, true>(a, max_keys, s);
-            if (a.d == 64) return sg_run<FORM, QT, 64, true>(a, max_keys, s);
-            if (a.d == 80) return sg_run<FORM, QT, 80, true>(a, max_keys, s);
-            if (a.d == 96) return sg_run<FORM, QT, 96, true>(a, max_keys, s);
-            if (a.d == 128) return sg_run<FORM, QT, 128, true>(a, max_keys, s);
-            return ST_ERR_BAD_SIZE;
-        }
-    }
-    if (a.d == 32) return sg_run<FORM, QT, 32, false>(a, max_keys, s);
-    if (a.d == 64) return sg_run<FORM, QT, 64, false>(a, max_keys, s);
-    if (a.d == 80) return sg_run<FORM, QT, 80, false>(a, max_keys, s);
-    if (a.d == 96) return sg_run<FORM, QT, 96, false>(a, max_keys, s);
-    if (a.d == 128) return sg_run<FORM, QT, 128, false>(a, max_keys, s);
+template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a, int max_keys, cudaStream_t s) {
+    if (a.d == 32) return sg_run<FORM, QT, 32, TWO>(a, max_keys, s);
+    if (a.d == 64) return sg_run<FORM, QT, 64, TWO>(a, max_keys, s);
+    if (a.d == 80) return sg_run<FORM, QT, 80, TWO>(a, max_keys, s);
+    if (a.d == 96) return sg_run<FORM, QT, 96, TWO>(a, max_keys, s);
+    if (a.d == 128) return sg_run<FORM, QT, 128, TWO>(a, max_keys, s);
     return ST_ERR_BAD_SIZE;
 }
 

@@ -2,5 +2,5 @@
 #include "attention_single8.cuh"
 
 int sg_int8(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s) {
-    return float_q ? sg_run<C8_INT8, float>(a, max_keys, s) : sg_run<C8_INT8, bf16>(a, max_keys, s);
+    return float_q ? sg_run<C8_INT8, float, true>(a, max_keys, s) : sg_run<C8_INT8, bf16, false>(a, max_keys, s);
 }
