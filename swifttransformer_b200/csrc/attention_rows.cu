@@ -418,10 +418,11 @@ template <int FORM, typename QT> static int aa_rows(const RowArgs& a, int max_ro
 static bool ar_types(int act, int form) {
     return form == C8_INT8 || form == C8_E4M3 ? act == 0 || act == 1 : form == C8_BF16 ? act == 1 : form == C8_F32 && act == 0;
 }
+static bool ar_single_fast(int page_size, int d, int form) {
+    return page_size % 8 == 0 && (d == 32 || d == 64 || d == 80 || d == 96 || d == 128) && form != C8_F32;
+}
 static int ar_single(const SingleArgs& a, int act, int form, int max_keys, cudaStream_t s) {
-    const bool fast = a.kv.page_size % 8 == 0 && (a.d == 32 || a.d == 64 || a.d == 80 || a.d == 96 || a.d == 128) &&
-                      form != C8_F32;
-    if (fast) {
+    if (ar_single_fast(a.kv.page_size, a.d, form)) {
         if (form == C8_INT8) return sg_int8(a, act == 0, max_keys, s);
         if (form == C8_E4M3) return sg_e4m3(a, act == 0, max_keys, s);
         return sg_bf16(a, max_keys, s);
@@ -506,12 +507,33 @@ static RowArgs ar_row_args(const RowCall& c) {
 
 ST_EXPORT int st_attention_rows_per_tile() { return AR_ROWS; }
 ST_EXPORT int st_attention_rows_chunk() { return AR_CHUNK; }
+// floats of scratch that st_attention_single8 wants for this call (0: none)
+static long long ar_line(const RowCall& c, SingleArgs* a) {
+    if (c.form >= C8_BF16 || !ar_single_fast(c.page_size, c.d, c.form) || c.nkv <= 0) return 0;
+    const int group = c.nh / c.nkv, R = c.act == 0 ? 4 : 8, walkers = sg_walkers(c.n_items, group, c.nkv, c.d, c.max_keys, c.act == 0);
+    if (!walkers) return 0;
+    const long long slots = (long long)c.n_items * c.nkv * ((group + R - 1) / R) + walkers, rows = slots * R;
+    if (a) {
+        a->walkers = walkers;
+        a->line = RowParts{c.scratch, c.scratch + rows, c.scratch + 2 * rows};
+        a->span = reinterpret_cast<int*>(c.scratch + rows * (2 + c.d));
+    }
+    return rows * (2 + c.d) + 2 * (slots - walkers);
+}
+ST_EXPORT long long st_attention_single8_scratch(int n_items, int nh, int nkv, int d, int page_size, int max_keys, int act, int form) {
+    RowCall c{};
+    c.n_items = n_items; c.nh = nh; c.nkv = nkv; c.d = d; c.page_size = page_size; c.max_keys = max_keys; c.act = act; c.form = form;
+    return ar_line(c, nullptr);
+}
+
 // single tokens; max_keys: about the longest of them (it decides how the work is spread, nothing else)
 ST_EXPORT int st_attention_single8(const RowCall* c, void* stream) {
     const int bad = ar_check(*c);
     if (bad) return bad;
     if (c->n_items <= 0) return 0;
-    return ar_single(ar_single_args(*c), c->act, c->form, c->max_keys, (cudaStream_t)stream);
+    SingleArgs a = ar_single_args(*c);
+    if (c->scratch && c->scratch_floats >= ar_line(*c, nullptr) && aligned16(c->out) && aligned16(c->scratch)) ar_line(*c, &a);
+    return ar_single(a, c->act, c->form, c->max_keys, (cudaStream_t)stream);
 }
 
 // tiles of tokens that follow one another in a request

@@ -30,6 +30,9 @@
 #include "attention_rows.cuh"
 
 #define SG_MAX_WARPS 16
+#define SG_LINE_ITEMS 1024           // tokens of a call that is dealt out as one line
+#define SG_LINE_WARPS 4              // warps of its blocks
+#define SG_LINE_BLOCKS 4             // of these blocks on an SM: what 128 registers a thread allow
 
 // what the finished row goes through, for all kernels of single tokens
 struct SingleArgs {
@@ -46,6 +49,11 @@ struct SingleArgs {
     int nh, group, d, n_items, splits, row_blocks;
     float scale_log2;
     int window;
+    // calls dealt out as one line: its walkers' parts (as in RowParts, R rows to a slot), and the first and last walker of every
+    // (key head and row block, token)
+    RowParts line;
+    int* span;
+    int walkers;
 };
 
 __device__ __forceinline__ void sg_cluster_sync() {
@@ -163,6 +171,96 @@ template <int N> __device__ __forceinline__ void sg_load(const unsigned char* p,
     }
 }
 
+// Calls of many keys are dealt out as one line: the runs of all tokens one behind the other, once per key head and row block, cut into
+// equal parts, one per warp, however unequal the tokens are (blocks that each had one token's keys left the device a third
+// empty at 64 requests of 500 to 1500 tokens).  Every block adds up the tokens' runs itself.
+template <bool LINE> struct SingleLine {
+    int length, total, run;
+    int before[LINE ? SG_LINE_ITEMS + 1 : 1];
+};
+template <int KT> __device__ __forceinline__ void sg_line_begin(const SingleArgs& a, SingleLine<true>& s) {
+    for (int i = threadIdx.x; i < a.n_items; i += blockDim.x) {
+        const int token = a.items ? a.items[i] : i, pos = token >= 0 ? a.positions[token] : -1;
+        const int base = a.window > 0 ? max(0, pos - a.window + 1) & ~7 : 0;
+        s.before[i + 1] = pos >= 0 ? (pos + 1 - base + KT - 1) / KT : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int i = 0; i < a.n_items; i += 32) {
+            int v = i + threadIdx.x < a.n_items ? s.before[i + threadIdx.x + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (threadIdx.x >= o) v += u;
+            }
+            v += sum;
+            if (i + threadIdx.x < a.n_items) s.before[i + threadIdx.x + 1] = v;
+            sum = __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (threadIdx.x == 0) {
+            s.before[0] = 0;
+            s.length = sum;
+            s.total = sum * a.row_blocks * a.kv.nkv;
+            s.run = max(1, (s.total + a.walkers - 1) / a.walkers);
+        }
+    }
+    __syncthreads();
+}
+// the item whose runs hold run r of the line
+__device__ __forceinline__ int sg_line_find(const SingleLine<true>& s, int n_items, int r) {
+    int lo = 0, hi = n_items - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s.before[mid] <= r) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+// A block per (unit, row): the parts that several walkers left, four dimensions a thread, the parts dealt out to the threads that remain.
+template <typename QT>
+__global__ void __launch_bounds__(128) attention_single8_join_kernel(const SingleArgs a, int R) {
+    __shared__ float s_max[4], s_l[128];
+    __shared__ float4 s_o[128];
+    const int unit = blockIdx.x, part = unit / a.n_items, item = unit - part * a.n_items, d = a.d, r = blockIdx.y;
+    const int key_head = part / a.row_blocks, head = key_head * a.group + (part % a.row_blocks) * R + r;
+    if (head >= (key_head + 1) * a.group) return;
+    const int token = a.items ? a.items[item] : item;
+    if (token < 0 || a.positions[token] < 0) return;
+    ST_PDL_WAIT();
+    const int c0 = __ldcg(a.span + 2 * unit), c1 = __ldcg(a.span + 2 * unit + 1);
+    if (c0 == c1) return;                                        // one walker had it all and has stored it
+    const int lanes = d / 4, groups = 128 / lanes, mine = threadIdx.x / lanes, e = threadIdx.x % lanes * 4;
+    float m = -INFINITY;
+    for (int c = c0 + threadIdx.x; c <= c1; c += 128) m = fmaxf(m, __ldcg(a.line.r + (size_t)(unit + c) * R + r));
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine < groups) {
+#pragma unroll 4
+        for (int c = c0 + mine; c <= c1; c += groups) {
+            const size_t at = (size_t)(unit + c) * R + r;
+            const float w = ar_weight(__ldcg(a.line.r + at), m);
+            const float4 v = load4_cg(a.line.o + at * d + e);
+            l += w * __ldcg(a.line.l + at);
+            o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
+        }
+    }
+    s_l[threadIdx.x] = l;
+    s_o[threadIdx.x] = o;
+    __syncthreads();
+    if (mine == 0) {
+        for (int k = 1; k < groups; ++k) {
+            l += s_l[k * lanes + threadIdx.x];
+            o = add4(o, s_o[k * lanes + threadIdx.x]);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        store4((QT*)a.out + ((size_t)token * a.nh + head) * d + e, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+}
+
 __device__ __forceinline__ uint32_t sg_transpose(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
@@ -171,8 +269,9 @@ __device__ __forceinline__ uint32_t sg_transpose(uint32_t a) {
 
 // FORM: the cache's; QT: query and output type; D: head size; TWO: weights (and float queries) in two numbers, four heads to a block
 // instead of eight.  Pages hold a multiple of 8 positions.
-template <int FORM, typename QT, int D, bool TWO>
-__global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(const SingleArgs a) {
+// LINE: see SingleLine below.
+template <int FORM, typename QT, int D, bool TWO, bool LINE>
+__global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS, LINE ? SG_LINE_BLOCKS : 1) attention_single8_kernel(const SingleArgs a) {
     constexpr bool HALF = FORM != C8_BF16;
     constexpr bool FLOATQ = sizeof(QT) == 4;
     static_assert(TWO || !FLOATQ, "");
@@ -184,22 +283,45 @@ __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(co
     constexpr int VW = (D / 8 * B + 3) / 4;                      // words of a value row a lane reads: an eighth (D = 80: 2.5 or 5)
     constexpr int NT = D / 8;                                    // dimensions of a value row a lane reads
     extern __shared__ float smem[];
-
-    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits;
-    const int key_head = blockIdx.y / a.row_blocks, head0 = key_head * a.group + (blockIdx.y % a.row_blocks) * R;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    __shared__ SingleLine<LINE> line;
+    int walker = 0, x = 0, x_end = 1;                            // LINE: this warp's part of the line
+    if constexpr (LINE) {
+        walker = blockIdx.x * SG_LINE_WARPS + warp;
+        sg_line_begin<KT>(a, line);
+        x = (int)min((long long)walker * line.run, (long long)line.total);
+        x_end = (int)min((long long)x + line.run, (long long)line.total);
+    }
+    while (x < x_end) {
+    int item, part, i, i_end, stride;                            // part: key head and row block; runs i, i + stride, ... below i_end
+    if constexpr (LINE) {
+        part = x / line.length;
+        const int r = x - part * line.length;
+        item = sg_line_find(line, a.n_items, r);
+        const int first = line.before[item], n = line.before[item + 1] - first;
+        i = r - first;
+        i_end = min(n, i + x_end - x);
+        stride = 1;
+    } else {
+        item = blockIdx.x / a.splits;
+        part = blockIdx.y;
+        i = blockIdx.x % a.splits * W + warp;
+        stride = W * a.splits;
+        i_end = 1 << 30;
+    }
+    const int key_head = part / a.row_blocks, head0 = key_head * a.group + (part % a.row_blocks) * R;
     const int rows = min(R, (key_head + 1) * a.group - head0);
     const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
-    if (pos < 0) {                                               // (the same for all blocks of a cluster)
+    if (!LINE && pos < 0) {                                      // (the same for all blocks of a cluster)
         if (a.info) ST_PDL_WAIT();                               // this kernel never ends before the one it was let in by
         return;
     }
     const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (a.info) lo = max(lo, a.info[3 * item]);
+    if (!LINE && a.info) lo = max(lo, a.info[3 * item]);
     const int hi = pos + 1;
-
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-    const int g = lane >> 2, t = lane & 3;
+    const int i0 = i;
     // offset of this lane's word w in a key row: pieces of 16 bytes per lane while the row lasts, then 8, then 4
     auto key_byte = [&](int w) -> int {
         constexpr int full = KW / 4 * 4, two = KW % 4 / 2 * 2;
@@ -207,7 +329,7 @@ __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(co
         if (w < full + two) return full * 16 + t * 8 + (w - full) * 4;
         return (full + two) * 16 + t * 4;
     };
-    const int base0 = lo & ~7, runs = hi > base0 ? (hi - base0 + KT - 1) / KT : 0, stride = W * a.splits;
+    const int base0 = lo & ~7, runs = min(i_end, hi > base0 ? (hi - base0 + KT - 1) / KT : 0);
     // A run's keys are four aligned blocks of NK, each within a page.  Lane (g, t) looks up block t, two runs ahead (ask), and
     // turns the page into a row of the pool one run ahead (resolve); its rows' keys are in block g / 2, whose row lane g / 2 has.
     constexpr uint32_t NONE = 0xffffffffu;
@@ -303,7 +425,6 @@ __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(co
     auto sees_all = [&](uint32_t at, int key) -> bool { return __all_sync(0xffffffffu, at != NONE && key >= lo && key + NK <= hi); };
 
     // the first run's loads leave before the query's
-    int i = split * W + warp;
     ask(i);
     uint32_t at = resolve(i), at_k = __shfl_sync(0xffffffffu, at, g >> 1);
     bool all = sees_all(at, base0 + i * KT + t * NK);
@@ -489,7 +610,10 @@ __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(co
         all = sees_all(at, next0);
         load_values(at, next0, all);
     }
-    // ---- parts to shared memory
+    // ---- the columns' sums
+    const int unit = LINE ? part * a.n_items + item : 0;
+    const bool whole = LINE && i0 == 0 && i_end == line.before[item + 1] - line.before[item];
+    const size_t slot = LINE ? (size_t)(unit + walker) * R : 0;
     float* s_ref = smem;
     float* s_sum = s_ref + W * R;
     float* s_acc = s_sum + W * R;
@@ -499,17 +623,39 @@ __global__ void __launch_bounds__(32 * SG_MAX_WARPS) attention_single8_kernel(co
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const int r = 2 * t + c;
-        if (g == 0 && r < R) { s_ref[warp * R + r] = ref[c]; s_sum[warp * R + r] = l; }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (g == 0 && r < R) {
+            if constexpr (LINE) {
+                if (!whole) { a.line.r[slot + r] = ref[c]; a.line.l[slot + r] = l; }
+            } else {
+                s_ref[warp * R + r] = ref[c];
+                s_sum[warp * R + r] = l;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < NT / 2; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float o = acc[j][2 * h + c];
                 if (TWO) o += __shfl_xor_sync(0xffffffffu, o, 2);
-                if (r < rows) s_acc[((size_t)warp * R + r) * D + value_dim(g, 2 * j + h)] = o;
+                const int e = value_dim(g, 2 * j + h);
+                if (r < rows) {
+                    if constexpr (!LINE) s_acc[((size_t)warp * R + r) * D + e] = o;
+                    else if (whole) ((QT*)a.out)[((size_t)token * a.nh + head0 + r) * D + e] = from_f32<QT>(o * inv);
+                    else a.line.o[(slot + r) * D + e] = o;
+                }
             }
     }
-    sg_finish<QT>(a, smem, W, R, rows, D, token, item, head0, key_head);
+    if constexpr (!LINE) {
+        sg_finish<QT>(a, smem, W, R, rows, D, token, item, head0, key_head);
+        return;
+    }
+    if (i0 == 0 && lane == 0) {
+        a.span[2 * unit] = walker;
+        a.span[2 * unit + 1] = (x + line.before[item + 1] - line.before[item] - 1) / line.run;
+    }
+    x += i_end - i0;
+    }
 }
 
 // Blocks, warps and the cluster: n_pairs = items x row blocks of all key heads, each over up to max_keys keys.
@@ -549,11 +695,20 @@ static int sg_run(SingleArgs a, int max_keys, cudaStream_t s) {
     constexpr int R = TWO ? 4 : 8, KT = D * c8_bytes(FORM) <= 64 ? 32 : 16;
     a.row_blocks = (a.group + R - 1) / R;
     const int grid_y = a.row_blocks * a.kv.nkv;
+    if constexpr (FORM != C8_BF16) {
+        if (a.walkers) {
+            attention_single8_kernel<FORM, QT, D, TWO, true><<<a.walkers / SG_LINE_WARPS, 32 * SG_LINE_WARPS, 0, s>>>(a);
+            const int rc = st_launch_status();
+            if (rc) return rc;
+            return st_launch_pdl("single8_join", attention_single8_join_kernel<QT>, dim3(a.n_items * grid_y, a.group < R ? a.group : R), dim3(128),
+                                 0, s, a, R);
+        }
+    }
     const SingleShape shape = sg_shape((long long)a.n_items * grid_y, max_keys, KT);
     a.splits = shape.splits;
     const size_t smem = (size_t)shape.warps * R * (D + 2) * 4;
-    AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO>), smem);
-    return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO>, a, shape.warps, smem, grid_y, s);
+    AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, false>), smem);
+    return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, false>, a, shape.warps, smem, grid_y, s);
 }
 template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a, int max_keys, cudaStream_t s) {
     if (a.d == 32) return sg_run<FORM, QT, 32, TWO>(a, max_keys, s);
@@ -562,6 +717,14 @@ template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a
     if (a.d == 96) return sg_run<FORM, QT, 96, TWO>(a, max_keys, s);
     if (a.d == 128) return sg_run<FORM, QT, 128, TWO>(a, max_keys, s);
     return ST_ERR_BAD_SIZE;
+}
+
+// Walkers of a call that is dealt out as one line, or 0: it pays (two launches, parts through memory) from four runs a warp on.
+static inline int sg_walkers(int n_items, int group, int nkv, int d, int max_keys, bool float_q) {
+    const int R = float_q ? 4 : 8, kt = d <= 64 ? 32 : 16;
+    const int walkers = st_sm_count() * SG_LINE_BLOCKS * SG_LINE_WARPS;
+    const long long parts = (long long)n_items * nkv * ((group + R - 1) / R), runs = parts * ((max_keys + kt - 1) / kt);
+    return n_items <= SG_LINE_ITEMS && runs >= 4ll * walkers && runs < (1 << 30) ? walkers : 0;
 }
 
 int sg_int8(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);

@@ -246,6 +246,10 @@ def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_tok
         stride = 0
     st = status if status is not None else _tc_status_word(q.device)
     scratch = None
+    if plan is None:
+        size = lib().st_attention_single8_scratch(n_items, nh, nkv, d, page_size, max_keys, _ACTS[q.dtype], _FORMS[pool.dtype])
+        if size:
+            scratch = torch.empty(size, dtype=torch.float32, device=q.device)
     n_tiles = total = max_rows = 0
     tiles = info = None
     if plan is not None:
