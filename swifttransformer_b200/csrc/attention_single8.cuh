@@ -15,24 +15,29 @@
 //
 // p_j = 2^(s_j - R): R follows the largest of s_j + log2 vs_j in steps: it moves when that exceeds R + 15, and then to 11 below, so
 // that p_j vs_j stays below 2^15 and what is 2^-24 of the largest still has a half's full precision.  For float queries the values' sums
-// of 32 (16) keys are formed in fresh accumulators and added to the running ones with a float add each: tensor cores cut
+// of a run are formed in fresh accumulators and added to the running ones with a float add each: tensor cores cut
 // what they add to a large sum.
 //
-// Layout: no shared memory on the way in.  A warp walks every n-th run of KT = 32 keys (16 where rows are longer than 64 bytes).
-// Lane (g, t) = (lane / 4, lane % 4) reads of the key rows that are rows g and g + 8 of a product a quarter in pieces of 16
-// bytes (the order of the summed dimensions is free, the query's is the same), and of the values of KT/4 neighbouring keys an
-// eighth of the row.  Keys are dealt to rows so that a lane's values are of neighbouring keys and each lane looks up one page per run;
-// the weights change lanes in one transposition (movmatrix) per 8 x 8.
+// Layout.  A warp walks runs of KT = 32 keys (16 where rows are longer than 128 bytes), each four aligned blocks of KT / 4 keys within a
+// page, which come by 16-byte asynchronous copies into a ring of its own in shared memory, one or two runs ahead: 8 KB a warp
+// under way, 100 to 140 KB an SM.  Lane (g, t) = (lane / 4, lane % 4) takes of the key rows that are rows g and g + 8 of a product a
+// quarter in pieces of 16 bytes (the order of the summed dimensions is free, the query's is the same), and of the values of KT/4
+// neighbouring keys an eighth of the row.  Keys are dealt to rows so that lane t's values are block t's and each lane looks up
+// one page per run; the weights change lanes in one transposition (movmatrix) per 8 x 8.  Rows are kept permuted (sg_key_at,
+// sg_value_at) so that lanes that read together hit different banks.
 //
-// Bound by memory.  What the loads in flight need is covered by many warps: keys of the next run are asked for as soon as this run's
-// products have taken theirs, values likewise.
+// Bound by memory where there are many keys.
 #pragma once
 #include "attention_rows.cuh"
 
 #define SG_MAX_WARPS 16
 #define SG_LINE_ITEMS 1024           // tokens of a call that is dealt out as one line
 #define SG_LINE_WARPS 4              // warps of its blocks
-#define SG_LINE_BLOCKS 4             // of these blocks on an SM: what 128 registers a thread allow
+// by the bytes of a row: keys of a run, runs of a warp's ring, and blocks of four warps on an SM, as their registers and rings allow
+__host__ __device__ constexpr int sg_run_keys(int row) { return row <= 128 ? 32 : 16; }
+__host__ __device__ constexpr int sg_stages(int row) { return row <= 80 ? 3 : 2; }
+__host__ __device__ constexpr int sg_line_blocks(int row) { return row <= 64 ? 4 : 3; }
+#define SG_JOIN 256                  // the most threads that join a row's parts
 
 // what the finished row goes through, for all kernels of single tokens
 struct SingleArgs {
@@ -158,17 +163,33 @@ template <bool HALF> __device__ __forceinline__ float2 sg_unpack(uint32_t w) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
-// N words from an address that is a multiple of 4 N bytes
-template <int N> __device__ __forceinline__ void sg_load(const unsigned char* p, uint32_t* w) {
-    if constexpr (N == 4) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else if constexpr (N == 2) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = u.x; w[1] = u.y;
-    } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    }
+// N words of shared memory from an address that is a multiple of 4 N bytes
+template <int N> __device__ __forceinline__ void sg_load(uint32_t p, uint32_t* w) {
+    if constexpr (N == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(p));
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(p));
+    else
+        asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(w[0]) : "r"(p));
+}
+__device__ __forceinline__ uint32_t sg_load2(uint32_t p) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(p));
+    return v;
+}
+__device__ __forceinline__ void sg_copy16(uint32_t dst, const void* src, bool ok) {      // zeros where not ok
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+// Where byte b (the first of 16) of row k of block t is kept, in blocks of N rows.  Keys: eight lanes read 64 bytes each of two
+// neighbouring rows; with rows of 128 bytes or more every second row has its halves of 128 bytes exchanged.  Values: lanes
+// of all four blocks read the same bytes of row k of theirs; the blocks' rows lie a multiple of 128 bytes apart, so block t's
+// pieces are moved by t.
+template <int ROW> __device__ __forceinline__ uint32_t sg_key_at(int row, int b) {
+    return row * ROW + (ROW % 128 == 0 ? b ^ ((row & 1) << 6) : b);
+}
+template <int ROW, int N> __device__ __forceinline__ uint32_t sg_value_at(int t, int k, int b) {
+    if (ROW == 64) return (t * N + (k ^ (t & 1))) * ROW + (b ^ ((t >> 1) << 5));
+    return (t * N + k) * ROW + (ROW % 128 == 0 ? b ^ (t << 5) : b);
 }
 
 // Calls of many keys are dealt out as one line: the runs of all tokens one behind the other, once per key head and row block, cut into
@@ -218,9 +239,9 @@ __device__ __forceinline__ int sg_line_find(const SingleLine<true>& s, int n_ite
 }
 // A block per (unit, row): the parts that several walkers left, four dimensions a thread, the parts dealt out to the threads that remain.
 template <typename QT>
-__global__ void __launch_bounds__(128) attention_single8_join_kernel(const SingleArgs a, int R) {
-    __shared__ float s_max[4], s_l[128];
-    __shared__ float4 s_o[128];
+__global__ void __launch_bounds__(SG_JOIN) attention_single8_join_kernel(const SingleArgs a, int R) {
+    __shared__ float s_max[SG_JOIN / 32], s_l[SG_JOIN];
+    __shared__ float4 s_o[SG_JOIN];
     const int unit = blockIdx.x, part = unit / a.n_items, item = unit - part * a.n_items, d = a.d, r = blockIdx.y;
     const int key_head = part / a.row_blocks, head = key_head * a.group + (part % a.row_blocks) * R + r;
     if (head >= (key_head + 1) * a.group) return;
@@ -229,13 +250,13 @@ __global__ void __launch_bounds__(128) attention_single8_join_kernel(const Singl
     ST_PDL_WAIT();
     const int c0 = __ldcg(a.span + 2 * unit), c1 = __ldcg(a.span + 2 * unit + 1);
     if (c0 == c1) return;                                        // one walker had it all and has stored it
-    const int lanes = d / 4, groups = 128 / lanes, mine = threadIdx.x / lanes, e = threadIdx.x % lanes * 4;
+    const int lanes = d / 4, groups = blockDim.x / lanes, mine = threadIdx.x / lanes, e = threadIdx.x % lanes * 4;
     float m = -INFINITY;
-    for (int c = c0 + threadIdx.x; c <= c1; c += 128) m = fmaxf(m, __ldcg(a.line.r + (size_t)(unit + c) * R + r));
+    for (int c = c0 + threadIdx.x; c <= c1; c += blockDim.x) m = fmaxf(m, __ldcg(a.line.r + (size_t)(unit + c) * R + r));
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    for (int i = 0; i < blockDim.x / 32; ++i) m = fmaxf(m, s_max[i]);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (mine < groups) {
@@ -271,23 +292,27 @@ __device__ __forceinline__ uint32_t sg_transpose(uint32_t a) {
 // instead of eight.  Pages hold a multiple of 8 positions.
 // LINE: see SingleLine below.
 template <int FORM, typename QT, int D, bool TWO, bool LINE>
-__global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS, LINE ? SG_LINE_BLOCKS : 1) attention_single8_kernel(const SingleArgs a) {
+__global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS, LINE ? sg_line_blocks(D * c8_bytes(FORM)) : 1) attention_single8_kernel(const SingleArgs a) {
     constexpr bool HALF = FORM != C8_BF16;
     constexpr bool FLOATQ = sizeof(QT) == 4;
     static_assert(TWO || !FLOATQ, "");
     constexpr int B = c8_bytes(FORM), ROW = D * B;
-    constexpr int KT = ROW <= 64 ? 32 : 16, NK = KT / 4, MT = KT / 16;   // keys of a run, keys of a lane, products over 16 keys
+    constexpr int KT = sg_run_keys(ROW), NK = KT / 4, MT = KT / 16;      // keys of a run, keys of a lane, products over 16 keys
+    constexpr int STAGES = sg_stages(ROW);
     constexpr int R = TWO ? 4 : 8;                               // query heads
     constexpr int NS = D / 16;                                   // products over 16 dimensions
     constexpr int KW = ROW / 16;                                 // words of a key row a lane reads: a quarter
     constexpr int VW = (D / 8 * B + 3) / 4;                      // words of a value row a lane reads: an eighth (D = 80: 2.5 or 5)
     constexpr int NT = D / 8;                                    // dimensions of a value row a lane reads
-    extern __shared__ float smem[];
+    constexpr int BLOCK = NK * ROW;                              // bytes of a block of keys or values
+    constexpr int STAGE = 8 * BLOCK + 8 * KT;                    // a run: keys, values, both scales
+    extern __shared__ __align__(128) float smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     __shared__ SingleLine<LINE> line;
     int walker = 0, x = 0, x_end = 1;                            // LINE: this warp's part of the line
     if constexpr (LINE) {
+        ST_PDL_TRIGGER();
         walker = blockIdx.x * SG_LINE_WARPS + warp;
         sg_line_begin<KT>(a, line);
         x = (int)min((long long)walker * line.run, (long long)line.total);
@@ -346,41 +371,44 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
     };
     auto resolve = [&](int i) -> uint32_t {
         const int key = base0 + i * KT + t * NK;
-        if (key >= hi) return NONE;
+        if (i >= runs || key >= hi) return NONE;
         if ((unsigned)page >= (unsigned)a.kv.num_pages) {
             if (key + NK > lo && a.kv.status) *a.kv.status = 1;
             return NONE;
         }
         return a.kv.row0(page, 0, key_head) + off;
     };
-    uint32_t kw[2 * MT][KW], vw[NK][VW];
-    float ks[2 * MT], vs[2 * MT];                                // of the keys of this lane's scores
-    const unsigned char* const key_pool = a.kv.pool + (g & 1) * ROW;
-    const unsigned char* const value_pool = a.kv.pool + (size_t)to_values * ROW;
-    auto load_keys = [&](uint32_t r) {                           // the row of block g / 2
-        const unsigned char* p = key_pool + (size_t)(r != NONE ? r : 0u) * ROW;
-        if (r != NONE) {
+    // ---- a run's copies: lane t has block t's row of the pool.  A lane's places are the same in every block but for bits of the address
+    // that the block's number turns over (the stages and blocks lie on multiples of 128 bytes).
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (STAGES * STAGE);
+    constexpr int CHUNKS = (BLOCK + 511) / 512;
+    const unsigned char* const keys_of = a.kv.pool + lane * 16;
+    const unsigned char* const values_of = keys_of + (size_t)to_values * ROW;
+    const int w_lane = lane / (NK / 4), c_lane = lane % (NK / 4);    // NK / 4 pieces of the keys' scales, as many of the values'
+    const float* const scales_of = a.kv.scales + (HALF && lane < NK / 2 ? w_lane * to_values + c_lane * 4 : 0u);
+    uint32_t key_to[CHUNKS], value_to[CHUNKS];
 #pragma unroll
-            for (int j = 0; j < 2 * MT; ++j) {
-                constexpr int full = KW / 4 * 4, two = KW % 4 / 2 * 2;
-                const unsigned char* pj = p + 2 * j * ROW;
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int b = c * 512 + lane * 16, k = b / ROW, e = b % ROW;
+        key_to[c] = sg_key_at<ROW>(k, e);
+        value_to[c] = 4 * BLOCK + sg_value_at<ROW, NK>(0, k, e);
+    }
+    const uint32_t scale_to = 8 * BLOCK + (w_lane * KT + c_lane * 4) * 4;
+    auto copy = [&](uint32_t at, uint32_t stage) {
 #pragma unroll
-                for (int w = 0; w < full; w += 4) sg_load<4>(pj + key_byte(w), kw[j] + w);
-                if constexpr (two > 0) sg_load<2>(pj + key_byte(full), kw[j] + full);
-                if constexpr (full + two < KW) sg_load<1>(pj + key_byte(full + two), kw[j] + full + two);
+        for (int b = 0; b < 4; ++b) {
+            const uint32_t r = __shfl_sync(0xffffffffu, at, b);
+            const bool ok = r != NONE;
+            const uint32_t row = ok ? r : 0u;
+            constexpr uint32_t turn = ROW == 64 ? 1 : 0;             // block b's values: (b & 1) << 6 | (b >> 1) << 5, or b << 5
+            const uint32_t bits = turn ? (uint32_t)((b & 1) << 6 | (b >> 1) << 5) : ROW % 128 == 0 ? (uint32_t)(b << 5) : 0u;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                if (c * 512 + lane * 16 >= BLOCK) continue;
+                sg_copy16(stage + key_to[c] + b * BLOCK, keys_of + (size_t)row * ROW + c * 512, ok);
+                sg_copy16(((stage + value_to[c]) ^ bits) + b * BLOCK, values_of + (size_t)row * ROW + c * 512, ok);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2 * MT; ++j)
-#pragma unroll
-                for (int w = 0; w < KW; ++w) kw[j][w] = 0u;
-        }
-    };
-    auto load_scales = [&](uint32_t r) {
-        if (HALF) {
-            const float* sc = a.kv.scales + (r != NONE ? r : 0u) + (g & 1);
-#pragma unroll
-            for (int j = 0; j < 2 * MT; ++j) { ks[j] = __ldg(sc + 2 * j); vs[j] = __ldg(sc + to_values + 2 * j); }
+            if (HALF && lane < NK / 2) sg_copy16(stage + scale_to + b * NK * 4, scales_of + row, ok);
         }
     };
     // an eighth of a value row: of every 128 (8-bit forms) or 64 dimensions 16 or 8 neighbours, of 32 four, of 16 two
@@ -391,47 +419,18 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
         if (i < 16 * V16 + 8 * V8 + 4 * V4) return 128 * V16 + 64 * V8 + n * 4 + (i - 16 * V16 - 8 * V8);
         return 128 * V16 + 64 * V8 + 32 * V4 + n * 2 + (i - 16 * V16 - 8 * V8 - 4 * V4);
     };
-    auto load_value = [&](const unsigned char* p, int k) {
-        if constexpr (V16) sg_load<4>(p + g * 16, vw[k]);
-#pragma unroll
-        for (int c = 0; c < V8; ++c) {
-            if constexpr (B == 1) sg_load<2>(p + V16 * 128 + c * 64 + g * 8, vw[k] + 4 * V16 + 2 * c);
-            else sg_load<4>(p + c * 128 + g * 16, vw[k] + 4 * c);
-        }
-        if constexpr (V4) {
-            if constexpr (B == 1) sg_load<1>(p + V8 * 64 + g * 4, vw[k] + 2 * V8);
-            else sg_load<2>(p + V8 * 128 + g * 8, vw[k] + 4 * V8);
-        }
-        if constexpr (V2) {
-            if constexpr (B == 1) vw[k][VW - 1] = __ldg(reinterpret_cast<const unsigned short*>(p + V8 * 64 + V4 * 32 + g * 2));
-            else sg_load<1>(p + V8 * 128 + V4 * 64 + g * 4, vw[k] + VW - 1);
-        }
-    };
-    auto load_values = [&](uint32_t at, int key, bool all) {    // key: the first of block t's; all: none of the warp's is hidden
-        const unsigned char* p = value_pool + (size_t)(at != NONE ? at : 0u) * ROW;
-        if (all) {
-#pragma unroll
-            for (int k = 0; k < NK; ++k) load_value(p + k * ROW, k);
-        } else {
-            // hidden rows may hold anything: zeros in their place
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {
-#pragma unroll
-                for (int w = 0; w < VW; ++w) vw[k][w] = 0u;
-                if (at != NONE && key + k >= lo && key + k < hi) load_value(p + k * ROW, k);
-            }
-        }
-    };
     auto sees_all = [&](uint32_t at, int key) -> bool { return __all_sync(0xffffffffu, at != NONE && key >= lo && key + NK <= hi); };
 
-    // the first run's loads leave before the query's
+    // the first runs' copies leave before the query's loads
+    uint32_t at[STAGES];                                      // block t's row of runs i, i + stride, ...
     ask(i);
-    uint32_t at = resolve(i), at_k = __shfl_sync(0xffffffffu, at, g >> 1);
-    bool all = sees_all(at, base0 + i * KT + t * NK);
-    load_keys(at_k);
-    load_scales(at_k);
-    load_values(at, base0 + i * KT + t * NK, all);
-    ask(i + stride);
+#pragma unroll
+    for (int j = 0; j + 1 < STAGES; ++j) {
+        at[j] = resolve(i + j * stride);
+        ask(i + (j + 1) * stride);
+        copy(at[j], ring + j * STAGE);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
 
     // ---- the query's fragments: column g is head g (TWO: head g % 4, its second number from column 4 on)
     uint32_t qb[NS][2];
@@ -480,28 +479,57 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[j][k] = 0.f;
 
+    uint32_t now = 0;                                            // the stage of run i
     for (; i < runs; i += stride) {
-        const int next0 = base0 + (i + stride) * KT + t * NK;
-        const uint32_t at1 = resolve(i + stride), at1_k = __shfl_sync(0xffffffffu, at1, g >> 1);
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();                                            // run i has landed, and every lane is done with the run before it
+        const uint32_t stage = ring + now * STAGE;
+        {
+            const uint32_t last = now == 0 ? STAGES - 1 : now - 1;
+            at[STAGES - 1] = resolve(i + (STAGES - 1) * stride);
+            ask(i + STAGES * stride);
+            copy(at[STAGES - 1], ring + last * STAGE);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+        const uint32_t at_k = __shfl_sync(0xffffffffu, at[0], g >> 1);
+        const bool all = sees_all(at[0], base0 + i * KT + t * NK);
         // ---- scores: rows g and g + 8 of product m are keys 4 m + g % 2 and 4 m + g % 2 + 2 of block g / 2
         float s[MT][4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m) {
+            uint32_t kw[2][KW];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                constexpr int full = KW / 4 * 4, two = KW % 4 / 2 * 2;
+                const int row = (g >> 1) * NK + 4 * m + 2 * h + (g & 1);
+#pragma unroll
+                for (int w = 0; w < full; w += 4) sg_load<4>(stage + sg_key_at<ROW>(row, key_byte(w)), kw[h] + w);
+                if constexpr (two > 0) sg_load<2>(stage + sg_key_at<ROW>(row, key_byte(full)), kw[h] + full);
+                if constexpr (full + two < KW) sg_load<1>(stage + sg_key_at<ROW>(row, key_byte(full + two)), kw[h] + full + two);
+            }
 #pragma unroll
             for (int x = 0; x < NS; ++x) {
                 uint32_t f[4];
                 if constexpr (HALF) {
-                    c8_halves<FORM>(kw[2 * m][x], f[0], f[2]);
-                    c8_halves<FORM>(kw[2 * m + 1][x], f[1], f[3]);
+                    c8_halves<FORM>(kw[0][x], f[0], f[2]);
+                    c8_halves<FORM>(kw[1][x], f[1], f[3]);
                 } else {
-                    f[0] = kw[2 * m][2 * x]; f[2] = kw[2 * m][2 * x + 1];
-                    f[1] = kw[2 * m + 1][2 * x]; f[3] = kw[2 * m + 1][2 * x + 1];
+                    f[0] = kw[0][2 * x]; f[2] = kw[0][2 * x + 1];
+                    f[1] = kw[1][2 * x]; f[3] = kw[1][2 * x + 1];
                 }
                 if (x == 0) sg_mma<HALF, false>(s[m], f, qb[x][0], qb[x][1]);
                 else sg_mma<HALF, true>(s[m], f, qb[x][0], qb[x][1]);
             }
-        load_keys(at1_k);
-        ask(i + 2 * stride);
+        }
+        float ks[2 * MT], vs[2 * MT];                            // of the keys of this lane's scores
+        if (HALF) {
+#pragma unroll
+            for (int j = 0; j < 2 * MT; ++j) {
+                const uint32_t p = stage + 8 * BLOCK + ((g >> 1) * NK + (g & 1) + 2 * j) * 4;
+                asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(ks[j]) : "r"(p));
+                asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(vs[j]) : "r"(p + KT * 4));
+            }
+        }
         // ---- softmax's numbers: s[m][c], s[m][2 + c] are column 2 t + c at keys 2 m and 2 m + 1 of ks and vs
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -572,8 +600,40 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
                 }
                 pb[m][h] = sg_transpose(w);
             }
-        load_scales(at1_k);
         // ---- values times weights: rows g and g + 8 of product j are this lane's dimensions 2 j and 2 j + 1
+        uint32_t vw[NK][VW];
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const uint32_t v = stage + 4 * BLOCK;
+            if constexpr (V16) sg_load<4>(v + sg_value_at<ROW, NK>(t, k, g * 16), vw[k]);
+#pragma unroll
+            for (int c = 0; c < V8; ++c) {
+                if constexpr (B == 1) sg_load<2>(v + sg_value_at<ROW, NK>(t, k, (V16 * 128 + c * 64 + g * 8) & ~15) + (g & 1) * 8, vw[k] + 4 * V16 + 2 * c);
+                else sg_load<4>(v + sg_value_at<ROW, NK>(t, k, c * 128 + g * 16), vw[k] + 4 * c);
+            }
+            if constexpr (V4) {
+                constexpr int from = V8 * 64 * B;
+                const int b = from + g * 4 * B;
+                if constexpr (B == 1) sg_load<1>(v + sg_value_at<ROW, NK>(t, k, b & ~15) + (b & 15), vw[k] + 2 * V8);
+                else sg_load<2>(v + sg_value_at<ROW, NK>(t, k, b & ~15) + (b & 15), vw[k] + 4 * V8);
+            }
+            if constexpr (V2) {
+                constexpr int from = (V8 * 64 + V4 * 32) * B;
+                const int b = from + g * 2 * B;
+                if constexpr (B == 1) vw[k][VW - 1] = sg_load2(v + sg_value_at<ROW, NK>(t, k, b & ~15) + (b & 15));
+                else sg_load<1>(v + sg_value_at<ROW, NK>(t, k, b & ~15) + (b & 15), vw[k] + VW - 1);
+            }
+        }
+        if (!all) {
+            // hidden rows may hold anything: zeros in their place
+            const int key = base0 + i * KT + t * NK;
+#pragma unroll
+            for (int k = 0; k < NK; ++k)
+                if (key + k < lo || key + k >= hi) {
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) vw[k][w] = 0u;
+                }
+        }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
             constexpr int PER = 4 / B;                           // dimensions of a word
@@ -605,11 +665,13 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
                 }
             }
         }
-        at = at1;
-        at_k = at1_k;
-        all = sees_all(at, next0);
-        load_values(at, next0, all);
+#pragma unroll
+        for (int j = 0; j + 1 < STAGES; ++j) at[j] = at[j + 1];
+        now = now + 1 == STAGES ? 0 : now + 1;
     }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    __syncwarp();                                                // the ring is free
+    if constexpr (!LINE) __syncthreads();                        // the parts lie where the rings were
     // ---- the columns' sums
     const int unit = LINE ? part * a.n_items + item : 0;
     const bool whole = LINE && i0 == 0 && i_end == line.before[item + 1] - line.before[item];
@@ -692,21 +754,26 @@ static inline int sg_launch(const char* tag, K kernel, const SingleArgs& a, int 
 
 template <int FORM, typename QT, int D, bool TWO>
 static int sg_run(SingleArgs a, int max_keys, cudaStream_t s) {
-    constexpr int R = TWO ? 4 : 8, KT = D * c8_bytes(FORM) <= 64 ? 32 : 16;
+    constexpr int R = TWO ? 4 : 8, ROW = D * c8_bytes(FORM), KT = sg_run_keys(ROW);
     a.row_blocks = (a.group + R - 1) / R;
     const int grid_y = a.row_blocks * a.kv.nkv;
+    constexpr size_t RING = sg_stages(ROW) * (2 * KT * ROW + 8 * KT);       // bytes per warp
     if constexpr (FORM != C8_BF16) {
         if (a.walkers) {
-            attention_single8_kernel<FORM, QT, D, TWO, true><<<a.walkers / SG_LINE_WARPS, 32 * SG_LINE_WARPS, 0, s>>>(a);
+            AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, true>), SG_LINE_WARPS * RING);
+            attention_single8_kernel<FORM, QT, D, TWO, true><<<a.walkers / SG_LINE_WARPS, 32 * SG_LINE_WARPS, SG_LINE_WARPS * RING, s>>>(a);
             const int rc = st_launch_status();
             if (rc) return rc;
-            return st_launch_pdl("single8_join", attention_single8_join_kernel<QT>, dim3(a.n_items * grid_y, a.group < R ? a.group : R), dim3(128),
-                                 0, s, a, R);
+            // few units have many parts each (150 for four long caches: 16 us with 128 threads, 3 with 256), many units two or three
+            const int units = a.n_items * grid_y;
+            return st_launch_pdl("single8_join", attention_single8_join_kernel<QT>, dim3(units, a.group < R ? a.group : R),
+                                 dim3(units < a.walkers / 8 ? SG_JOIN : 64), 0, s, a, R);
         }
     }
-    const SingleShape shape = sg_shape((long long)a.n_items * grid_y, max_keys, KT);
+    SingleShape shape = sg_shape((long long)a.n_items * grid_y, max_keys, KT);
+    while (shape.warps * RING > 200 * 1024) shape.warps /= 2;     // a block's shared memory
     a.splits = shape.splits;
-    const size_t smem = (size_t)shape.warps * R * (D + 2) * 4;
+    const size_t parts = (size_t)shape.warps * R * (D + 2) * 4, rings = shape.warps * RING, smem = parts > rings ? parts : rings;
     AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, false>), smem);
     return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, false>, a, shape.warps, smem, grid_y, s);
 }
@@ -721,8 +788,8 @@ template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a
 
 // Walkers of a call that is dealt out as one line, or 0: it pays (two launches, parts through memory) from four runs a warp on.
 static inline int sg_walkers(int n_items, int group, int nkv, int d, int max_keys, bool float_q) {
-    const int R = float_q ? 4 : 8, kt = d <= 64 ? 32 : 16;
-    const int walkers = st_sm_count() * SG_LINE_BLOCKS * SG_LINE_WARPS;
+    const int R = float_q ? 4 : 8, kt = sg_run_keys(d);          // (8-bit forms: rows of d bytes)
+    const int walkers = st_sm_count() * sg_line_blocks(d) * SG_LINE_WARPS;
     const long long parts = (long long)n_items * nkv * ((group + R - 1) / R), runs = parts * ((max_keys + kt - 1) / kt);
     return n_items <= SG_LINE_ITEMS && runs >= 4ll * walkers && runs < (1 << 30) ? walkers : 0;
 }

@@ -72,10 +72,9 @@ __device__ __forceinline__ uint32_t c8_hsub2(uint32_t a, uint32_t b) {
     asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-__device__ __forceinline__ uint32_t c8_e4m3x2(uint32_t two) {       // the low two bytes
-    uint32_t d;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}\n" : "=r"(d) : "r"(two));
-    return d;
+__device__ __forceinline__ void c8_e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {       // the low two bytes, the high two
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n"
+        : "=r"(lo), "=r"(hi) : "r"(w));
 }
 // int8: the byte c + 128 behind the exponent of 1024 is the half 1024 + 128 + c; 1152 less is c
 #define C8_BIAS 0x64806480u               // (half 1152) twice, which is also 0x6400 with the sign bit of the byte flipped
@@ -86,22 +85,23 @@ template <int FORM> __device__ __forceinline__ void c8_halves(uint32_t w, uint32
         lo = c8_hsub2(__byte_perm(u, 0x64646464u, 0x4140), C8_BIAS);
         hi = c8_hsub2(__byte_perm(u, 0x64646464u, 0x4342), C8_BIAS);
     } else {
-        lo = c8_e4m3x2(w);
-        hi = c8_e4m3x2(w >> 16);
+        c8_e4m3x4(w, lo, hi);
     }
+}
+__device__ __forceinline__ uint32_t c8_biased(uint32_t bytes) {      // bytes 0 and 2 behind the exponent of 1024, sign bits flipped
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n" : "=r"(d) : "r"(bytes), "r"(0x00ff00ffu), "r"(C8_BIAS));      // (bytes & mask) ^ bias in one
+    return d;
 }
 // words a and b of two rows -> the pairs (a_i, b_i), i = 0..3
 template <int FORM> __device__ __forceinline__ void c8_pairs(uint32_t a, uint32_t b, uint32_t* out) {
     if (FORM == C8_INT8) {
-        out[0] = c8_hsub2((__byte_perm(a, b, 0x0400) & 0x00ff00ffu) ^ C8_BIAS, C8_BIAS);
-        out[1] = c8_hsub2((__byte_perm(a, b, 0x0501) & 0x00ff00ffu) ^ C8_BIAS, C8_BIAS);
-        out[2] = c8_hsub2((__byte_perm(a, b, 0x0602) & 0x00ff00ffu) ^ C8_BIAS, C8_BIAS);
-        out[3] = c8_hsub2((__byte_perm(a, b, 0x0703) & 0x00ff00ffu) ^ C8_BIAS, C8_BIAS);
+        out[0] = c8_hsub2(c8_biased(__byte_perm(a, b, 0x0400)), C8_BIAS);
+        out[1] = c8_hsub2(c8_biased(__byte_perm(a, b, 0x0501)), C8_BIAS);
+        out[2] = c8_hsub2(c8_biased(__byte_perm(a, b, 0x0602)), C8_BIAS);
+        out[3] = c8_hsub2(c8_biased(__byte_perm(a, b, 0x0703)), C8_BIAS);
     } else {
-        const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
-        out[0] = c8_e4m3x2(x);
-        out[1] = c8_e4m3x2(x >> 16);
-        out[2] = c8_e4m3x2(y);
-        out[3] = c8_e4m3x2(y >> 16);
+        c8_e4m3x4(__byte_perm(a, b, 0x5140), out[0], out[1]);
+        c8_e4m3x4(__byte_perm(a, b, 0x7362), out[2], out[3]);
     }
 }
