@@ -393,7 +393,8 @@ template <int FORM, typename QT> static int aa_single(SingleArgs a, int max_keys
     a.splits = shape.splits;
     a.row_blocks = 1;
     const int warps = shape.warps < 4 ? shape.warps : 4;
-    return sg_launch("single_any", attention_single_any_kernel<FORM, QT>, a, warps, (size_t)warps * (a.d + 2) * 4, a.nh, s);
+    return sg_launch("single_any", attention_single_any_kernel<FORM, QT>, a, dim3((unsigned)a.n_items * a.splits, a.nh), warps,
+                     (size_t)warps * (a.d + 2) * 4, s);
 }
 
 template <int FORM, typename QT, int ROWS> static int aa_rows(const RowArgs& a, cudaStream_t s) {
@@ -507,23 +508,23 @@ static RowArgs ar_row_args(const RowCall& c) {
 
 ST_EXPORT int st_attention_rows_per_tile() { return AR_ROWS; }
 ST_EXPORT int st_attention_rows_chunk() { return AR_CHUNK; }
-// floats of scratch that st_attention_single8 wants for this call (0: none)
-static long long ar_line(const RowCall& c, SingleArgs* a) {
-    if (c.form >= C8_BF16 || !ar_single_fast(c.page_size, c.d, c.form) || c.nkv <= 0) return 0;
-    const int group = c.nh / c.nkv, R = c.act == 0 ? 4 : 8, walkers = sg_walkers(c.n_items, group, c.nkv, c.d, c.max_keys, c.act == 0);
-    if (!walkers) return 0;
-    const long long slots = (long long)c.n_items * c.nkv * ((group + R - 1) / R) + walkers, rows = slots * R;
+// floats of scratch that single tokens want for this call (0: none), laid out at `from`
+static long long ar_line(const RowCall& c, SingleArgs* a, float* from) {
+    if (c.nkv <= 0 || c.d <= 0 || !ar_single_fast(c.page_size, c.d, c.form)) return 0;
+    const LineShape s = sg_line_shape(c.n_items, c.nh / c.nkv, c.nkv, c.d, c.max_keys, c.act == 0, c.form);
+    if (!s.walkers) return 0;
+    const long long rows = s.slots * s.R, units = s.slots - s.walkers;
     if (a) {
-        a->walkers = walkers;
-        a->line = RowParts{c.scratch, c.scratch + rows, c.scratch + 2 * rows};
-        a->span = reinterpret_cast<int*>(c.scratch + rows * (2 + c.d));
+        a->walkers = s.walkers;
+        a->line = RowParts{from, from + rows, from + 2 * rows};
+        a->span = reinterpret_cast<int*>(from + rows * (2 + c.d));
     }
-    return rows * (2 + c.d) + 2 * (slots - walkers);
+    return rows * (2 + c.d) + 2 * units;
 }
 ST_EXPORT long long st_attention_single8_scratch(int n_items, int nh, int nkv, int d, int page_size, int max_keys, int act, int form) {
     RowCall c{};
     c.n_items = n_items; c.nh = nh; c.nkv = nkv; c.d = d; c.page_size = page_size; c.max_keys = max_keys; c.act = act; c.form = form;
-    return ar_line(c, nullptr);
+    return ar_line(c, nullptr, nullptr);
 }
 
 // single tokens; max_keys: about the longest of them (it decides how the work is spread, nothing else)
@@ -532,7 +533,7 @@ ST_EXPORT int st_attention_single8(const RowCall* c, void* stream) {
     if (bad) return bad;
     if (c->n_items <= 0) return 0;
     SingleArgs a = ar_single_args(*c);
-    if (c->scratch && c->scratch_floats >= ar_line(*c, nullptr) && aligned16(c->out) && aligned16(c->scratch)) ar_line(*c, &a);
+    if (c->scratch && c->scratch_floats >= ar_line(*c, nullptr, nullptr) && aligned16(c->out) && aligned16(c->scratch)) ar_line(*c, &a, c->scratch);
     return ar_single(a, c->act, c->form, c->max_keys, (cudaStream_t)stream);
 }
 
@@ -564,6 +565,7 @@ ST_EXPORT int st_attention_shared(const RowCall* c, void* stream) {
     if (c->nh / c->nkv > AR_ROWS || c->q_stride > 0) return ST_ERR_BAD_ARG;
     const cudaStream_t s = (cudaStream_t)stream;
     SingleArgs single = ar_single_args(*c);
+    long long used = 0;                     // floats of scratch
     if (c->total > 0) {
         RowArgs a = ar_row_args(*c);
         const long long slots = (long long)c->n_tiles * c->nkv + a.plan.ctas;
@@ -576,6 +578,9 @@ ST_EXPORT int st_attention_shared(const RowCall* c, void* stream) {
         single.info = c->info;
         single.plan = a.plan;
         single.parts = a.parts;
+        used = slots * (long long)ar_part_floats(c->d);
     }
+    if (c->scratch && c->scratch_floats >= used + ar_line(*c, nullptr, nullptr) && aligned16(c->out) && aligned16(c->scratch))
+        ar_line(*c, &single, c->scratch + used);
     return ar_single(single, c->act, c->form, c->max_keys, s);
 }

@@ -100,16 +100,6 @@ struct RowWalk {
     }
 };
 
-// Calls f(slot) for every part of unit (tile, head).
-template <typename F>
-__device__ __forceinline__ void ar_each_part(const RowPlan& p, const RowTile& t, int tile, int head, F f) {
-    const int n = ar_chunks(t);
-    if (n == 0) return;
-    const int x0 = t.start + head * n, unit = tile * p.nkv + head;
-    const int c1 = (x0 + n - 1) / p.run;
-    for (int c = x0 / p.run; c <= c1; ++c) f(unit + c);
-}
-
 __device__ __forceinline__ float ar_exp2(float x) {      // 2 ulp, exp2(-inf) = 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));

@@ -58,7 +58,7 @@ struct SingleArgs {
     // (key head and row block, token)
     RowParts line;
     int* span;
-    int walkers;
+    int walkers;                 // 0: no line
 };
 
 __device__ __forceinline__ void sg_cluster_sync() {
@@ -70,6 +70,18 @@ __device__ __forceinline__ float sg_remote(const float* local, uint32_t rank) { 
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
     return v;
+}
+
+// The parts of a token's shared keys: rows row, row + AR_ROWS, ... (n of them) of a.parts, for the key head's first query head.
+struct SharedParts { size_t row; int n; };
+__device__ __forceinline__ SharedParts sg_shared_parts(const SingleArgs& a, int item, int key_head) {
+    if (!a.info) return SharedParts{0, 0};
+    const int tile = a.info[3 * item + 1], place = a.info[3 * item + 2];
+    const RowTile t = ar_tile(a.plan, tile);
+    const int n = ar_chunks(t);
+    if (n == 0) return SharedParts{0, 0};
+    const int x0 = t.start + key_head * n, c0 = x0 / a.plan.run;
+    return SharedParts{(size_t)(tile * a.plan.nkv + key_head + c0) * AR_ROWS + place * a.group, (x0 + n - 1) / a.plan.run - c0 + 1};
 }
 
 // The warps' parts of R rows x D, then the cluster's, then the prefix's, to the output.  smem: W x R x (D + 2) floats: (R, l) of each
@@ -106,33 +118,28 @@ __device__ __forceinline__ void sg_finish(const SingleArgs& a, float* smem, int 
     } else {
         __syncthreads();
     }
-    RowTile t{};
-    int tile = 0, place = 0;
-    if (a.info) {
-        ST_PDL_WAIT();                                 // the prefix's parts are complete
-        tile = a.info[3 * item + 1];
-        place = a.info[3 * item + 2];
-        t = ar_tile(a.plan, tile);
-    }
+    SharedParts shared = sg_shared_parts(a, item, key_head);
+    if (a.info) ST_PDL_WAIT();                         // the prefix's parts are complete
     QT* out = (QT*)a.out + ((size_t)token * a.nh + head0) * D;
     for (int i = threadIdx.x + rank * blockDim.x; i < rows * D; i += blockDim.x * a.splits) {
         const int r = i / D;
+        const size_t row = shared.row + (head0 - key_head * a.group) + r;
         float m = -INFINITY, l = 0.f, o = 0.f;
         for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.splits > 1 ? sg_remote(ref + r, s) : ref[r]);
-        const int row = place * a.group + (head0 - key_head * a.group) + r;
-        if (a.info) ar_each_part(a.plan, t, tile, key_head, [&](int slot) { m = fmaxf(m, __ldcg(a.parts.r + (size_t)slot * AR_ROWS + row)); });
+#pragma unroll 4
+        for (int p = 0; p < shared.n; ++p) m = fmaxf(m, __ldcg(a.parts.r + row + (size_t)p * AR_ROWS));
         for (int s = 0; s < a.splits; ++s) {
             const float w = ar_weight(a.splits > 1 ? sg_remote(ref + r, s) : ref[r], m);
             l += w * (a.splits > 1 ? sg_remote(sum + r, s) : sum[r]);
             o += w * (a.splits > 1 ? sg_remote(acc + i, s) : acc[i]);
         }
-        if (a.info)
-            ar_each_part(a.plan, t, tile, key_head, [&](int slot) {
-                const size_t at = (size_t)slot * AR_ROWS + row;
-                const float w = ar_weight(__ldcg(a.parts.r + at), m);
-                l += w * __ldcg(a.parts.l + at);
-                o += w * __ldcg(a.parts.o + at * D + (i - r * D));
-            });
+#pragma unroll 4
+        for (int p = 0; p < shared.n; ++p) {
+            const size_t at = row + (size_t)p * AR_ROWS;
+            const float w = ar_weight(__ldcg(a.parts.r + at), m);
+            l += w * __ldcg(a.parts.l + at);
+            o += w * __ldcg(a.parts.o + at * D + (i - r * D));
+        }
         out[i] = from_f32<QT>(l == 0.f ? 0.f : o / l);   // no key at all: zeros
     }
     if (a.splits > 1) sg_cluster_sync();               // nobody leaves while others read here
@@ -199,11 +206,15 @@ template <bool LINE> struct SingleLine {
     int length, total, run;
     int before[LINE ? SG_LINE_ITEMS + 1 : 1];
 };
+template <int KT> __device__ __forceinline__ int sg_runs(const SingleArgs& a, int item, int pos) {     // of a token's own keys
+    int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    if (a.info) lo = max(lo, a.info[3 * item]);
+    return pos >= lo ? (pos + 1 - (lo & ~7) + KT - 1) / KT : 0;
+}
 template <int KT> __device__ __forceinline__ void sg_line_begin(const SingleArgs& a, SingleLine<true>& s) {
     for (int i = threadIdx.x; i < a.n_items; i += blockDim.x) {
         const int token = a.items ? a.items[i] : i, pos = token >= 0 ? a.positions[token] : -1;
-        const int base = a.window > 0 ? max(0, pos - a.window + 1) & ~7 : 0;
-        s.before[i + 1] = pos >= 0 ? (pos + 1 - base + KT - 1) / KT : 0;
+        s.before[i + 1] = sg_runs<KT>(a, i, pos);
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -237,22 +248,28 @@ __device__ __forceinline__ int sg_line_find(const SingleLine<true>& s, int n_ite
     }
     return lo;
 }
-// A block per (unit, row): the parts that several walkers left, four dimensions a thread, the parts dealt out to the threads that remain.
-template <typename QT>
+// A block per (unit, row): the parts that several walkers left, and those of shared keys, four dimensions a thread, the parts dealt out
+// to the threads that remain.
+template <typename QT, int KT>
 __global__ void __launch_bounds__(SG_JOIN) attention_single8_join_kernel(const SingleArgs a, int R) {
     __shared__ float s_max[SG_JOIN / 32], s_l[SG_JOIN];
     __shared__ float4 s_o[SG_JOIN];
     const int unit = blockIdx.x, part = unit / a.n_items, item = unit - part * a.n_items, d = a.d, r = blockIdx.y;
     const int key_head = part / a.row_blocks, head = key_head * a.group + (part % a.row_blocks) * R + r;
     if (head >= (key_head + 1) * a.group) return;
-    const int token = a.items ? a.items[item] : item;
-    if (token < 0 || a.positions[token] < 0) return;
+    const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
+    if (pos < 0) return;
+    const SharedParts shared = sg_shared_parts(a, item, key_head);
+    const size_t shared_row = shared.row + (head - key_head * a.group);
+    const bool own = sg_runs<KT>(a, item, pos) > 0;
     ST_PDL_WAIT();
-    const int c0 = __ldcg(a.span + 2 * unit), c1 = __ldcg(a.span + 2 * unit + 1);
-    if (c0 == c1) return;                                        // one walker had it all and has stored it
+    const int c0 = own ? __ldcg(a.span + 2 * unit) : 0, c1 = own ? __ldcg(a.span + 2 * unit + 1) : -1;
+    if (!a.info && c0 == c1) return;                             // one walker had it all and has stored it
     const int lanes = d / 4, groups = blockDim.x / lanes, mine = threadIdx.x / lanes, e = threadIdx.x % lanes * 4;
+    const int n_own = c1 - c0 + 1, n = n_own + shared.n;
     float m = -INFINITY;
-    for (int c = c0 + threadIdx.x; c <= c1; c += blockDim.x) m = fmaxf(m, __ldcg(a.line.r + (size_t)(unit + c) * R + r));
+    for (int p = threadIdx.x; p < n; p += blockDim.x)
+        m = fmaxf(m, p < n_own ? __ldcg(a.line.r + (size_t)(unit + c0 + p) * R + r) : __ldcg(a.parts.r + shared_row + (size_t)(p - n_own) * AR_ROWS));
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -261,11 +278,12 @@ __global__ void __launch_bounds__(SG_JOIN) attention_single8_join_kernel(const S
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (mine < groups) {
 #pragma unroll 4
-        for (int c = c0 + mine; c <= c1; c += groups) {
-            const size_t at = (size_t)(unit + c) * R + r;
-            const float w = ar_weight(__ldcg(a.line.r + at), m);
-            const float4 v = load4_cg(a.line.o + at * d + e);
-            l += w * __ldcg(a.line.l + at);
+        for (int p = mine; p < n; p += groups) {
+            const RowParts& from = p < n_own ? a.line : a.parts;
+            const size_t at = p < n_own ? (size_t)(unit + c0 + p) * R + r : shared_row + (size_t)(p - n_own) * AR_ROWS;
+            const float w = ar_weight(__ldcg(from.r + at), m);
+            const float4 v = load4_cg(from.o + at * d + e);
+            l += w * __ldcg(from.l + at);
             o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
         }
     }
@@ -344,7 +362,7 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
     }
     const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (!LINE && a.info) lo = max(lo, a.info[3 * item]);
+    if (a.info) lo = max(lo, a.info[3 * item]);
     const int hi = pos + 1;
     const int i0 = i;
     // offset of this lane's word w in a key row: pieces of 16 bytes per lane while the row lasts, then 8, then 4
@@ -674,7 +692,7 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
     if constexpr (!LINE) __syncthreads();                        // the parts lie where the rings were
     // ---- the columns' sums
     const int unit = LINE ? part * a.n_items + item : 0;
-    const bool whole = LINE && i0 == 0 && i_end == line.before[item + 1] - line.before[item];
+    const bool whole = LINE && !a.info && i0 == 0 && i_end == line.before[item + 1] - line.before[item];
     const size_t slot = LINE ? (size_t)(unit + walker) * R : 0;
     float* s_ref = smem;
     float* s_sum = s_ref + W * R;
@@ -718,6 +736,7 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
     }
     x += i_end - i0;
     }
+    if (LINE && a.info) ST_PDL_WAIT();                           // this kernel never ends before the one it was let in by
 }
 
 // Blocks, warps and the cluster: n_pairs = items x row blocks of all key heads, each over up to max_keys keys.
@@ -725,9 +744,9 @@ struct SingleShape { int splits, warps; };
 SingleShape sg_shape(long long n_pairs, int max_keys, int keys_per_run);
 
 template <typename K>
-static inline int sg_launch(const char* tag, K kernel, const SingleArgs& a, int warps, size_t smem, int grid_y, cudaStream_t s) {
+static inline int sg_launch(const char* tag, K kernel, const SingleArgs& a, dim3 grid, int warps, size_t smem, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.n_items * a.splits, grid_y);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(32 * warps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -758,24 +777,23 @@ static int sg_run(SingleArgs a, int max_keys, cudaStream_t s) {
     a.row_blocks = (a.group + R - 1) / R;
     const int grid_y = a.row_blocks * a.kv.nkv;
     constexpr size_t RING = sg_stages(ROW) * (2 * KT * ROW + 8 * KT);       // bytes per warp
-    if constexpr (FORM != C8_BF16) {
-        if (a.walkers) {
-            AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, true>), SG_LINE_WARPS * RING);
-            attention_single8_kernel<FORM, QT, D, TWO, true><<<a.walkers / SG_LINE_WARPS, 32 * SG_LINE_WARPS, SG_LINE_WARPS * RING, s>>>(a);
-            const int rc = st_launch_status();
-            if (rc) return rc;
-            // few units have many parts each (150 for four long caches: 16 us with 128 threads, 3 with 256), many units two or three
-            const int units = a.n_items * grid_y;
-            return st_launch_pdl("single8_join", attention_single8_join_kernel<QT>, dim3(units, a.group < R ? a.group : R),
-                                 dim3(units < a.walkers / 8 ? SG_JOIN : 64), 0, s, a, R);
-        }
+    if (a.walkers) {
+        const size_t smem = SG_LINE_WARPS * RING;
+        AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, true>), smem);
+        const int rc = sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, true>, a, dim3(a.walkers / SG_LINE_WARPS), SG_LINE_WARPS, smem, s);
+        if (rc) return rc;
+        // few units have many parts each (150 for four long caches: 16 us with 128 threads, 3 with 256), many units two or three
+        const int units = a.n_items * grid_y;
+        return st_launch_pdl("single8_join", attention_single8_join_kernel<QT, KT>, dim3(units, a.group < R ? a.group : R),
+                             dim3(units < a.walkers / 8 ? SG_JOIN : 64), 0, s, a, R);
     }
     SingleShape shape = sg_shape((long long)a.n_items * grid_y, max_keys, KT);
     while (shape.warps * RING > 200 * 1024) shape.warps /= 2;     // a block's shared memory
     a.splits = shape.splits;
     const size_t parts = (size_t)shape.warps * R * (D + 2) * 4, rings = shape.warps * RING, smem = parts > rings ? parts : rings;
     AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, false>), smem);
-    return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, false>, a, shape.warps, smem, grid_y, s);
+    return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, false>, a, dim3((unsigned)a.n_items * a.splits, grid_y), shape.warps,
+                     smem, s);
 }
 template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a, int max_keys, cudaStream_t s) {
     if (a.d == 32) return sg_run<FORM, QT, 32, TWO>(a, max_keys, s);
@@ -786,12 +804,16 @@ template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a
     return ST_ERR_BAD_SIZE;
 }
 
-// Walkers of a call that is dealt out as one line, or 0: it pays (two launches, parts through memory) from four runs a warp on.
-static inline int sg_walkers(int n_items, int group, int nkv, int d, int max_keys, bool float_q) {
-    const int R = float_q ? 4 : 8, kt = sg_run_keys(d);          // (8-bit forms: rows of d bytes)
-    const int walkers = st_sm_count() * sg_line_blocks(d) * SG_LINE_WARPS;
-    const long long parts = (long long)n_items * nkv * ((group + R - 1) / R), runs = parts * ((max_keys + kt - 1) / kt);
-    return n_items <= SG_LINE_ITEMS && runs >= 4ll * walkers && runs < (1 << 30) ? walkers : 0;
+// How a call is dealt out as one line, walkers 0 if it is not: it pays (two launches, parts through memory) from four runs a warp on.
+struct LineShape { int walkers, R; long long slots; };
+static inline LineShape sg_line_shape(int n_items, int group, int nkv, int d, int max_keys, bool float_q, int form) {
+    LineShape s{0, float_q || (form == C8_BF16 && group <= 4) ? 4 : 8, 0};
+    const int row = d * c8_bytes(form), kt = sg_run_keys(row), walkers = st_sm_count() * sg_line_blocks(row) * SG_LINE_WARPS;
+    const long long parts = (long long)n_items * nkv * ((group + s.R - 1) / s.R), runs = parts * ((max_keys + kt - 1) / kt);
+    if (n_items > SG_LINE_ITEMS || runs < 4ll * walkers || runs >= (1 << 30)) return s;
+    s.walkers = walkers;
+    s.slots = parts + walkers;
+    return s;
 }
 
 int sg_int8(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);

@@ -245,11 +245,6 @@ def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_tok
     else:
         stride = 0
     st = status if status is not None else _tc_status_word(q.device)
-    scratch = None
-    if plan is None:
-        size = lib().st_attention_single8_scratch(n_items, nh, nkv, d, page_size, max_keys, _ACTS[q.dtype], _FORMS[pool.dtype])
-        if size:
-            scratch = torch.empty(size, dtype=torch.float32, device=q.device)
     n_tiles = total = max_rows = 0
     tiles = info = None
     if plan is not None:
@@ -257,10 +252,11 @@ def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_tok
         _need(plan.n_tokens <= n and plan.n_seqs <= slots.numel(), f"{what}: the plan names tokens or requests that are not there")
         tiles, info, items = plan.tiles, plan.info, plan.items
         n_items, n_tiles, total, max_rows = plan.n_items, plan.n_tiles, plan.total, plan.max_rows
-        if total:
-            # parts of rows that several blocks leave: a slot per (tile, key head) and one per block
-            scratch = torch.empty((n_tiles * nkv + 3 * sm_count(q.device)) * ROWS_PER_TILE * (2 + d), dtype=torch.float32,
-                                  device=q.device)
+    # parts of rows that several blocks leave: a slot per (tile, key head) and one per walker of the line; those of single tokens
+    floats = (n_tiles * nkv + 3 * sm_count(q.device)) * ROWS_PER_TILE * (2 + d) if total else 0
+    if n_items:
+        floats += lib().st_attention_single8_scratch(n_items, nh, nkv, d, page_size, max_keys, _ACTS[q.dtype], _FORMS[pool.dtype])
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     call = _CALL.pack(q.data_ptr(), out.data_ptr(), pool.data_ptr(), _ptr(scales), block_table.data_ptr(), positions.data_ptr(),
                       _ptr(seq_of_token), slots.data_ptr(), _ptr(items), _ptr(tiles), _ptr(info), _ptr(scratch), st.data_ptr(),
                       stride, n_pages, scratch.numel() if scratch is not None else 0,
