@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs 
     w.begin(p, blockIdx.x);
     RowPiece pc;
     if (!w.next(p, pc) || pc.chunk0 == 0) return;                   // the run begins with a unit of its own
-    const int n = ar_chunks(pc.t), x0 = pc.t.start + pc.head * n, c0 = x0 / p.run, c1 = (x0 + n - 1) / p.run;
+    int c0, c1;
+    ar_walkers(p, pc.t, pc.head, ar_chunks(pc.t), c0, c1);
     if (c0 != (int)blockIdx.x - 1) return;
     ST_PDL_WAIT();
     const int pieces = (d + 3) / 4, total = pc.t.n_tok * g * pieces;
@@ -444,7 +445,7 @@ static int ar_rows(RowArgs a, int act, int form, int max_rows, cudaStream_t s) {
     return aa_rows<C8_F32, float>(a, max_rows, s);
 }
 
-// The runs a plan's line of chunks is cut into: as many as are walked at the same time, two per SM by the tensor-core kernel, one by every
+// The runs a plan's line is cut into: as many as are walked at the same time, two per SM by the tensor-core kernel, one by every
 // block of the float kernel.
 static void ar_deal(RowArgs& a, int act, int form) {
     const int most = st_sm_count() * (ar_tc(a, act, form) ? 2 : a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);

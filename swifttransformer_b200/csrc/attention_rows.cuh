@@ -3,8 +3,10 @@
 //
 // A row is one (token, query head).  A tile holds the rows of up to 128 / g tokens, for one key head, g = query heads per key
 // head: row r is head r % g of the group of token r / g.  The tile's keys [key_lo, key_hi) are walked in chunks of AR_CHUNK.
-// All chunks of all (tile, key head) pairs ("units"), one unit's behind the other's, form one line of `total` chunks which is cut
-// into runs of `run` chunks, one per walker (a block, or one of a block's two groups): every walker gets the same work however
+// All chunks of all (tile, key head) pairs ("units"), one unit's behind the other's, each unit with a place of its own in front for what
+// its begin and end cost (about a chunk's time: without it the walkers of a prompt's first, short units were the last by a factor of
+// two), form one line of `total` places which is cut
+// into runs of `run` places, one per walker (a block, or one of a block's two groups): every walker gets the same work however
 // unequal the tiles are, and a unit that a cut goes through is put together from parts.  Part (unit u, walker c) has slot u + c: a
 // new slot begins with every unit and with every run, so no two parts share one.
 //
@@ -18,7 +20,7 @@
 #define AR_LOG2E 1.4426950408889634f
 
 // a tile of a plan: six numbers in the plan's array
-struct RowTile { int first, n_tok, seq, key_lo, key_hi, start; };   // start: the line's chunk where key head 0's share begins
+struct RowTile { int first, n_tok, seq, key_lo, key_hi, start; };   // start: the line's place where key head 0's share begins
 
 struct RowPlan {
     const int* tiles;        // [n_tiles][6]
@@ -57,6 +59,8 @@ __device__ __forceinline__ RowTile ar_tile(const RowPlan& p, int i) {
 __device__ __forceinline__ int ar_chunks(const RowTile& t) {
     return t.key_hi > t.key_lo ? (t.key_hi - (t.key_lo & ~(AR_CHUNK - 1)) + AR_CHUNK - 1) / AR_CHUNK : 0;
 }
+__device__ __forceinline__ int ar_places(int chunks) { return chunks > 0 ? chunks + 1 : 0; }      // of a unit in the line
+
 // A walker's way along its run: pieces of one (tile, key head) pair.  A walker behind the line's end has none.
 struct RowPiece {
     RowTile t;
@@ -82,23 +86,34 @@ struct RowWalk {
     __device__ __forceinline__ bool next(const RowPlan& p, RowPiece& out) {
         if (at >= end) return false;
         int n = ar_chunks(t);
-        while (at >= t.start + n * p.nkv) {
+        while (at >= t.start + ar_places(n) * p.nkv) {
             if (++tile >= p.n_tiles) return false;
             t = ar_tile(p, tile);
             n = ar_chunks(t);
         }
-        const int in = at - t.start;
+        const int in = at - t.start, head = in / ar_places(n);
+        int c = in - head * ar_places(n);
+        if (c == 0) {                                    // the unit's own place
+            c = 1;
+            if (++at >= end) return false;
+        }
         out.t = t;
         out.tile = tile;
-        out.head = in / n;
-        out.unit = tile * p.nkv + out.head;
-        out.chunk0 = in - out.head * n;
+        out.head = head;
+        out.unit = tile * p.nkv + head;
+        out.chunk0 = c - 1;
         out.chunks = min(n - out.chunk0, end - at);
         out.whole = out.chunks == n;
         at += out.chunks;
         return true;
     }
 };
+// the walkers of unit (tile t, key head) with n > 0 chunks: c0 to c1
+__device__ __forceinline__ void ar_walkers(const RowPlan& p, const RowTile& t, int head, int n, int& c0, int& c1) {
+    const int x0 = t.start + head * ar_places(n) + 1;
+    c0 = x0 / p.run;
+    c1 = (x0 + n - 1) / p.run;
+}
 
 __device__ __forceinline__ float ar_exp2(float x) {      // 2 ulp, exp2(-inf) = 0
     float y;

@@ -80,8 +80,9 @@ __device__ __forceinline__ SharedParts sg_shared_parts(const SingleArgs& a, int 
     const RowTile t = ar_tile(a.plan, tile);
     const int n = ar_chunks(t);
     if (n == 0) return SharedParts{0, 0};
-    const int x0 = t.start + key_head * n, c0 = x0 / a.plan.run;
-    return SharedParts{(size_t)(tile * a.plan.nkv + key_head + c0) * AR_ROWS + place * a.group, (x0 + n - 1) / a.plan.run - c0 + 1};
+    int c0, c1;
+    ar_walkers(a.plan, t, key_head, n, c0, c1);
+    return SharedParts{(size_t)(tile * a.plan.nkv + key_head + c0) * AR_ROWS + place * a.group, c1 - c0 + 1};
 }
 
 // The warps' parts of R rows x D, then the cluster's, then the prefix's, to the output.  smem: W x R x (D + 2) floats: (R, l) of each

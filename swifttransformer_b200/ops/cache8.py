@@ -136,7 +136,7 @@ class RowPlan:
     """Which query rows share a pass over which keys: made on the host once per step, used by all its layers.
 
     ``tiles``: int32 [n_tiles, 6] on the device: first token (or place in ``items``), tokens, request (-1: that of the first
-    item), first and last + 1 key, and where the tile's chunks begin in the line of all chunks.  ``items``: the tokens of
+    item), first and last + 1 key, and where the tile begins in the line of all units (a place per unit and per chunk of keys).  ``items``: the tokens of
     a plan for shared prefixes in the tiles' order; ``info`` [items, 3]: keys shared with the group, tile, place in the tile."""
 
     def __init__(self, kind: str, nh: int, nkv: int, device):
@@ -159,7 +159,8 @@ class RowPlan:
         rows = []
         for first, n, seq, lo, hi in tiles:
             rows.append((first, n, seq, lo, hi, start))
-            start += self._chunks(lo, hi) * self.nkv
+            chunks = self._chunks(lo, hi)
+            start += (chunks + 1) * self.nkv if chunks else 0
         _need(start < 1 << 31 and len(rows) * self.nkv < 1 << 22, "a plan of more keys than one call serves")
         self.total, self.n_tiles = start, len(rows)
         self.max_rows = max((r[1] for r in rows), default=0) * (self.nh // self.nkv)

@@ -17,9 +17,9 @@ def walk(plan, ctas):
     for c in range(ctas):
         for x in range(bounds[c], bounds[c + 1]):
             t = max(i for i, r in enumerate(tiles) if r[5] <= x and chunks(r) > 0)
-            n = chunks(tiles[t])
-            head, chunk = divmod(x - tiles[t][5], n)
-            pieces.append((c, t, head, chunk))
+            head, place = divmod(x - tiles[t][5], chunks(tiles[t]) + 1)
+            if place:                                   # place 0 stands for what a unit costs beside its chunks
+                pieces.append((c, t, head, place - 1))
     return pieces
 
 
@@ -38,7 +38,7 @@ def test_every_key_of_every_row_is_in_one_chunk(seed):
     starts = [rng.choice([0, 1, 128, rng.randint(0, 900)]) for _ in lens]
     plan = ops.portion_plan(lens, starts, nh, nkv, window, "cpu")
     tiles = plan.tiles.view(-1, 6).tolist() if plan.n_tiles else []
-    assert plan.n_tokens == sum(lens) and plan.total == sum(chunks(t) for t in tiles) * nkv
+    assert plan.n_tokens == sum(lens) and plan.total == sum(chunks(t) + 1 for t in tiles if chunks(t)) * nkv
     rows = []
     first = 0
     for seq, (n, s) in enumerate(zip(lens, starts)):
@@ -57,15 +57,15 @@ def test_every_key_of_every_row_is_in_one_chunk(seed):
     if plan.total:
         for ctas in (1, 2, 7, 148):
             got = walk(plan, min(ctas, plan.total))
-            assert len(got) == len(set(p[1:] for p in got)) == plan.total
+            assert len(got) == len(set(p[1:] for p in got)) == sum(chunks(t) for t in tiles) * nkv
 
 
 def test_shared_plan():
     plan = ops.shared_prefix_plan([[5, 2, 9], [], [0], [7, 8]], [300, 10, 0, 128], 64, 1, "cpu", 17)
     assert plan.tokens_per_tile == 2 and plan.items.tolist() == [5, 2, 9, 0, 7, 8]
-    assert plan.tiles.view(-1, 6).tolist() == [[0, 2, -1, 0, 300, 0], [2, 1, -1, 0, 300, 3], [3, 1, -1, 0, 0, 6], [4, 2, -1, 0, 128, 6]]
+    assert plan.tiles.view(-1, 6).tolist() == [[0, 2, -1, 0, 300, 0], [2, 1, -1, 0, 300, 4], [3, 1, -1, 0, 0, 8], [4, 2, -1, 0, 128, 8]]
     assert plan.info.view(-1, 3).tolist() == [[300, 0, 0], [300, 0, 1], [300, 1, 0], [0, 2, 0], [128, 3, 0], [128, 3, 1]]
-    assert plan.total == 7 and plan.n_items == 6 and plan.max_rows == 128 and plan.n_tokens == 10 and plan.max_own == 17
+    assert plan.total == 10 and plan.n_items == 6 and plan.max_rows == 128 and plan.n_tokens == 10 and plan.max_own == 17
 
 
 @pytest.mark.parametrize("make", [
