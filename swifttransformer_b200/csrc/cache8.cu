@@ -4,13 +4,13 @@
 //
 // A row of head_dim elements is held by a group of 1 to 32 lanes, eight elements each, from the load to the store: the bias sum,
 // the largest magnitude (butterflies inside the group), the codes.  So a row is read once and written once, which is the floor;
-// the write of 2000 tokens of OPT-6.7B (32 heads of 128) is bound by memory, a decode step's by the launch and the chain
-// position -> request -> slot -> page, which runs beside the loads.
+// a decode step's write is bound by the launch and the chain position -> request -> slot -> page, which runs beside the loads,
+// a prompt's by that chain, by its arithmetic (150 instructions for eight elements of a warp) and by memory about alike.
 //
-// Rounding: t = x * (1 / scale) is off by less than 2^-22 of itself, so t (1 - 2^-21) and t (1 + 2^-21) bracket the exact quotient;
-// where both round to the same code that is the code.  Otherwise (about one in ten thousand) the quotient is formed in 64 bits,
-// whose rounding can neither reach nor leave the middle between two codes: a quotient of two 24-bit numbers that is not such
-// a middle, of at most 9 bits, is further than 2^-34 of itself away from it.
+// Rounding: t = x * (1 / scale) is off by less than 2^-22 of itself.  Where no t of a thread's eight is that near the middle between two
+// codes, their roundings are those of the exact quotients; otherwise (one time in two thousand) the quotients are formed in 64
+// bits, whose rounding can neither reach nor leave a middle: a quotient of two 24-bit numbers that is not such a middle, of at most
+// 9 bits, is further than 2^-34 of itself away from it.  The scale likewise: max|x| (1 / M) in 64 bits, rounded once.
 #include "cache8.cuh"
 
 #define C8_THREADS 256
@@ -27,32 +27,63 @@ template <int FORM> __device__ __noinline__ uint32_t c8_exact(float x, float sca
     return c8_two_e4m3(f, f) & 0xffu;
 }
 // codes of eight elements, four to a word
-template <int FORM> __device__ __forceinline__ uint2 c8_codes(const float* x, float scale, float inv) {
-    uint32_t w[2] = {0, 0};
-    constexpr float DN = 1.f - 0x1p-21f, UP = 1.f + 0x1p-21f;
+template <int FORM> __device__ __forceinline__ uint2 c8_codes(const float* x, float scale) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(scale));     // 1 ulp; 2^-126 <= scale < 2^122: neither end is subnormal
+    uint32_t w[2];
+    bool near;
+    if (FORM == C8_INT8) {
+        // t + 1.5 2^23 has round(t) in its low byte
+        constexpr float MAGIC = 12582912.f;
+        uint32_t u[8];
+        float off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const float t0 = x[i] * inv, t1 = x[i + 1] * inv;
-        uint32_t lo, hi;
-        if (FORM == C8_INT8) {
-            const int a0 = __float2int_rn(t0 * DN), b0 = __float2int_rn(t0 * UP), a1 = __float2int_rn(t1 * DN), b1 = __float2int_rn(t1 * UP);
-            lo = (a0 & 0xff) | (a1 & 0xff) << 8;
-            hi = (b0 & 0xff) | (b1 & 0xff) << 8;
-            // t can lie a little above 127: 127 (1 + 2^-21) rounds to 127, no clamp is needed
-        } else {
-            lo = c8_two_e4m3(t0 * DN, t1 * DN);
-            hi = c8_two_e4m3(t0 * UP, t1 * UP);
+        for (int i = 0; i < 8; ++i) {
+            const float t = x[i] * inv, m = t + MAGIC;
+            u[i] = __float_as_uint(m);
+            off = fmaxf(off, fabsf(t - (m - MAGIC)));
         }
-        if (lo != hi) lo = c8_exact<FORM>(x[i], scale) | c8_exact<FORM>(x[i + 1], scale) << 8;
-        w[i >> 2] |= (lo & 0xffffu) << ((i & 2) * 8);
+        near = off > 0.5f - 0x1p-14f;                                  // |t| <= 127 (1 + 2^-22): off by 2^-15 at most
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            w[k] = __byte_perm(__byte_perm(u[4 * k], u[4 * k + 1], 0x0040), __byte_perm(u[4 * k + 2], u[4 * k + 3], 0x0040), 0x5410);
+    } else {
+        // the middle between two codes from 2^-6 on: the bits behind the third are 1000...; below 2^-6 the codes lie otherwise
+        uint32_t least = 0xffffffffu;
+        float small = 1.f;
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float t0 = x[i] * inv, t1 = x[i + 1] * inv;
+            least = min(least, min((__float_as_uint(t0) + (8u - 0x80000u)) & 0xfffffu, (__float_as_uint(t1) + (8u - 0x80000u)) & 0xfffffu));
+            small = fminf(small, fminf(fabsf(t0), fabsf(t1)));
+            h[i >> 1] = c8_two_e4m3(t0, t1);
+        }
+        near = least < 16u || small < 0x1p-6f;
+        w[0] = h[0] | h[1] << 16;
+        w[1] = h[2] | h[3] << 16;
+    }
+    if (near) {
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v |= c8_exact<FORM>(k ? x[4 + i] : x[i], scale) << (8 * i);
+            w[k] = v;
+        }
     }
     return make_uint2(w[0], w[1]);
 }
-// the scale of a row whose largest magnitude has these bits, and whether the row is finite
-template <int FORM> __device__ __forceinline__ float c8_scale(uint32_t amax_bits, bool& finite) {
-    finite = amax_bits < 0x7f800000u;
+__device__ __forceinline__ float c8_max_nan(float a, float b) {       // of magnitudes; NaN if one is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
+// the scale of a row whose largest magnitude this is (or NaN), and whether the row is finite
+template <int FORM> __device__ __forceinline__ float c8_scale(float amax, bool& finite) {
+    finite = amax < INFINITY;
     if (!finite) return __uint_as_float(0x7fffffffu);
-    return fmaxf(__fdiv_rn(__uint_as_float(amax_bits), FORM == C8_INT8 ? 127.f : 448.f), C8_TINY);
+    return fmaxf(__double2float_rn((double)amax * (FORM == C8_INT8 ? 1.0 / 127.0 : 1.0 / 448.0)), C8_TINY);
 }
 
 struct Cache8Write {
@@ -68,17 +99,26 @@ struct Cache8Write {
     int nh, d, write_kv;
 };
 
-template <typename T> __device__ __forceinline__ void c8_load8(const T* p, float* f);
-template <> __device__ __forceinline__ void c8_load8<float>(const float* p, float* f) {
-    const float4 a = load4(p), b = load4(p + 4);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-template <> __device__ __forceinline__ void c8_load8<bf16>(const bf16* p, float* f) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// eight elements as they lie in memory, and as floats
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = load4(p); b = load4(p + 4); }
+    __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void floats(float* f) const {
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+};
+template <> struct Eight<bf16> {
+    uint4 u;
+    __device__ __forceinline__ void load(const bf16* p) { u = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void clear() { u = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void floats(float* f) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
+        for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+};
 __device__ __forceinline__ void c8_store8(float* p, const float* f) {
     store4(p, make_float4(f[0], f[1], f[2], f[3]));
     store4(p + 4, make_float4(f[4], f[5], f[6], f[7]));
@@ -93,54 +133,59 @@ __device__ __forceinline__ void c8_store8(bf16* p, const float* f) {
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// G lanes per row of d <= 8 G elements (d a multiple of 8), TURN rows per thread, all loaded before the first is worked on
-template <typename T, int FORM, int G, int TURN>
-__global__ void __launch_bounds__(C8_THREADS) cache8_write_kernel(const Cache8Write a) {
+// G lanes per row of d <= 8 G elements (d a multiple of 8), TURN rows per thread, all loaded before the first is worked on and kept as
+// they were loaded.
+template <typename T, int FORM, int G, int TURN, bool FULL>
+__global__ void __launch_bounds__(C8_THREADS, 6) cache8_write_kernel(const Cache8Write a) {
     const int t = blockIdx.x;
-    const int nkv = a.kv.nkv, d = a.d, rows = a.nh + 2 * nkv;
+    const int pos = a.positions[t];
+    constexpr int PER = C8_THREADS / G;                  // rows of a turn
+    const int nkv = a.kv.nkv, d = FULL ? 8 * G : a.d, rows = a.nh + 2 * nkv;       // FULL: every lane of a group has eight elements
     const int lane = threadIdx.x % G, e = 8 * lane;
-    const int first = blockIdx.y * (C8_THREADS / G * TURN) + threadIdx.x / G;
-    const T* src = (const T*)a.qkv + (size_t)t * rows * d + e;
-    const bool in = e < d;
-    float f[TURN][8];
+    const int first = blockIdx.y * (PER * TURN) + threadIdx.x / G;
+    const bool in = FULL || e < d;
+    const size_t at = ((size_t)t * rows + first) * d + e;
+    const T* src = (const T*)a.qkv + at;
+    Eight<T> held[TURN];
 #pragma unroll
     for (int j = 0; j < TURN; ++j) {
-        const int r = first + j * (C8_THREADS / G);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
-        if (in && r < rows && (r >= a.nh || a.q_out)) c8_load8<T>(src + (size_t)r * d, f[j]);
+        const int r = first + j * PER;
+        held[j].clear();
+        if (in && r < rows && (r >= a.nh || a.q_out)) held[j].load(src + (size_t)(j * PER) * d);
     }
-    const int pos = a.positions[t];
-    int page = -1, off = 0;
+    int page = -1;
+    uint32_t row0 = 0;                                   // of key head 0; a page holds all heads' keys, then all heads' values
     if (a.write_kv && pos >= 0) {        // pos < 0: a padding token, nothing is cached
-        const int index = a.kv.page_index(pos);
         page = a.kv.page(a.kv.table + (size_t)a.slots[a.seq_of_token[t]] * a.kv.max_pages, pos);
-        off = a.kv.offset(pos, index);
+        row0 = a.kv.row0(page, 0, 0) + a.kv.offset(pos, a.kv.page_index(pos));
         if (page < 0 && threadIdx.x == 0) atomicExch(a.kv.status, 1);
     }
 #pragma unroll
     for (int j = 0; j < TURN; ++j) {
-        const int r = first + j * (C8_THREADS / G);      // the same for the lanes of a group; a group stays together below
-        const bool live = r < rows && in;
+        const int r = first + j * PER;                   // the same for the lanes of a group; a group stays together below
+        const bool live = r < rows && in, query = r < a.nh;
+        float f[8];
+        held[j].floats(f);
         if (live && a.bias) {
-            const float4 b0 = load4(a.bias + (size_t)r * d + e), b1 = load4(a.bias + (size_t)r * d + e + 4);
-            f[j][0] += b0.x; f[j][1] += b0.y; f[j][2] += b0.z; f[j][3] += b0.w;
-            f[j][4] += b1.x; f[j][5] += b1.y; f[j][6] += b1.z; f[j][7] += b1.w;
+            const float* bias = a.bias + (first + j * PER) * d + e;
+            const float4 b0 = load4(bias), b1 = load4(bias + 4);
+            f[0] += b0.x; f[1] += b0.y; f[2] += b0.z; f[3] += b0.w;
+            f[4] += b1.x; f[5] += b1.y; f[6] += b1.z; f[7] += b1.w;
         }
-        uint32_t amax = 0;
+        float amax = 0.f;
+        if (!__all_sync(0xffffffffu, query)) {
+            amax = c8_max_nan(c8_max_nan(c8_max_nan(f[0], f[1]), c8_max_nan(f[2], f[3])), c8_max_nan(c8_max_nan(f[4], f[5]), c8_max_nan(f[6], f[7])));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[j][i]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            for (int o = G / 2; o > 0; o >>= 1) amax = c8_max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        }
         if (!live) continue;
-        if (r < a.nh) {
-            if (a.q_out) c8_store8((T*)a.q_out + ((size_t)t * a.nh + r) * d + e, f[j]);
+        if (query) {
+            if (a.q_out) c8_store8((T*)a.q_out + ((size_t)t * a.nh + r) * d + e, f);
         } else if (page >= 0) {
-            const int which = r - a.nh >= nkv, head = r - a.nh - which * nkv;
             bool finite;
             const float scale = c8_scale<FORM>(amax, finite);
-            const uint32_t row = a.kv.row0(page, which, head) + off;
-            const uint2 c = finite ? c8_codes<FORM>(f[j], scale, __frcp_rn(scale)) : make_uint2(0u, 0u);
+            const uint32_t row = row0 + (uint32_t)(r - a.nh) * a.kv.page_size;
+            const uint2 c = finite ? c8_codes<FORM>(f, scale) : make_uint2(0u, 0u);
             *reinterpret_cast<uint2*>(a.pool + (size_t)row * d + e) = c;
             if (lane == 0) a.scales[row] = scale;
         }
@@ -168,10 +213,10 @@ __global__ void __launch_bounds__(C8_THREADS) cache8_write_any_kernel(const Cach
             continue;
         }
         if (page < 0) continue;
-        uint32_t amax = 0;
-        for (int e = lane; e < d; e += 32)
-            amax = max(amax, __float_as_uint(to_f32(src[e]) + (bias ? bias[e] : 0.f)) & 0x7fffffffu);
-        amax = __reduce_max_sync(0xffffffffu, amax);
+        float amax = 0.f;
+        for (int e = lane; e < d; e += 32) amax = c8_max_nan(amax, to_f32(src[e]) + (bias ? bias[e] : 0.f));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = c8_max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const int which = r - a.nh >= nkv, head = r - a.nh - which * nkv;
         bool finite;
         const float scale = c8_scale<FORM>(amax, finite);
@@ -185,13 +230,18 @@ __global__ void __launch_bounds__(C8_THREADS) cache8_write_any_kernel(const Cach
 template <typename T, int FORM, int G>
 static int c8_launch_write(const Cache8Write& a, int n, cudaStream_t s) {
     const int rows = a.nh + 2 * a.kv.nkv, per = C8_THREADS / G;
-    // Four rows per thread once that still leaves two blocks for every SM, else one: with four, their loads are under way together;
-    // with one, a decode step's rows are spread over more SMs.
-    const int by4 = (rows + 4 * per - 1) / (4 * per);
-    if ((long long)by4 * n >= 2 * st_sm_count())
-        cache8_write_kernel<T, FORM, G, 4><<<dim3(n, by4), C8_THREADS, 0, s>>>(a);
-    else
-        cache8_write_kernel<T, FORM, G, 1><<<dim3(n, (rows + per - 1) / per), C8_THREADS, 0, s>>>(a);
+    // Two rows per thread once that still leaves two blocks for every SM, else one, so that a decode step's rows are spread over more
+    // SMs.  (A block's life is the chain of loads to its page: 2000 tokens of 32 heads of 128 take 25 us with two rows and six
+    // blocks on an SM, 28 with four rows, whose registers leave four blocks.)
+    const int by2 = (rows + 2 * per - 1) / (2 * per);
+    const dim3 grid2(n, by2), grid1(n, (rows + per - 1) / per);
+    if ((long long)by2 * n >= 2 * st_sm_count()) {
+        if (a.d == 8 * G) cache8_write_kernel<T, FORM, G, 2, true><<<grid2, C8_THREADS, 0, s>>>(a);
+        else cache8_write_kernel<T, FORM, G, 2, false><<<grid2, C8_THREADS, 0, s>>>(a);
+    } else {
+        if (a.d == 8 * G) cache8_write_kernel<T, FORM, G, 1, true><<<grid1, C8_THREADS, 0, s>>>(a);
+        else cache8_write_kernel<T, FORM, G, 1, false><<<grid1, C8_THREADS, 0, s>>>(a);
+    }
     return st_launch_status();
 }
 template <typename T, int FORM> static int c8_launch_write(const Cache8Write& a, int n, cudaStream_t s) {
@@ -207,19 +257,42 @@ template <typename T, int FORM> static int c8_launch_write(const Cache8Write& a,
     return c8_launch_write<T, FORM, 32>(a, n, s);
 }
 
-// act: 0 float, 1 bfloat16; form: C8_INT8 or C8_E4M3; d up to 256
-ST_EXPORT int st_qkv_to_cache8(const void* qkv, const float* bias, void* q_out, void* pool, float* scales, const int* positions,
-                               const int* seq_of_token, const int* slots, const int* block_table, int max_pages, int num_pages,
-                               int n_layers, int layer, int n_tokens, int nh, int nkv, int d, int page_size, int write_kv, int* status,
-                               int act, int form, void* stream) {
-    if (n_tokens <= 0) return 0;
-    if (nh <= 0 || nkv <= 0 || d <= 0 || page_size <= 0 || layer < 0 || layer >= n_layers || max_pages <= 0 || num_pages <= 0 || !status)
+// what both entry points take, as the caller lays it out; act: 0 float, 1 bfloat16; form: C8_INT8 or C8_E4M3; d up to 256
+struct Cache8Call {
+    const void* qkv;
+    const float* bias;
+    void* q_out;
+    void* pool;
+    float* scales;
+    const int* positions;
+    const int* seq_of_token;
+    const int* slots;
+    const int* block_table;
+    int* status;
+    void* out;                      // rows read back
+    int max_pages, num_pages, n_layers, layer, n_tokens, nh, nkv, d, page_size, write_kv, act, form;
+};
+static_assert(sizeof(Cache8Call) == 11 * 8 + 12 * 4, "the caller lays this out field by field");
+
+static int c8_check(const Cache8Call& c) {
+    if (c.nkv <= 0 || c.d <= 0 || c.page_size <= 0 || c.layer < 0 || c.layer >= c.n_layers || c.max_pages <= 0 || c.num_pages <= 0 || !c.status)
         return ST_ERR_BAD_ARG;
-    if (d > 256) return ST_ERR_TOO_LARGE;
-    if (!c8_rows_fit(num_pages, n_layers, nkv, page_size) || (long long)nh + 2ll * nkv > (1 << 16)) return ST_ERR_TOO_LARGE;
-    Cache8Write a{qkv, bias, q_out, (unsigned char*)pool, scales, positions, seq_of_token, slots,
-                  PagedKV{(const unsigned char*)pool, scales, block_table, max_pages, num_pages, n_layers, layer, nkv, page_size,
-                          c8_shift(page_size), status}, nh, d, write_kv};
+    if (c.d > 256 || c.nkv > (1 << 15) || !c8_rows_fit(c.num_pages, c.n_layers, c.nkv, c.page_size)) return ST_ERR_TOO_LARGE;
+    return 0;
+}
+static PagedKV c8_kv(const Cache8Call& c) {
+    return PagedKV{(const unsigned char*)c.pool, c.scales, c.block_table, c.max_pages, c.num_pages, c.n_layers, c.layer, c.nkv, c.page_size,
+                   c8_shift(c.page_size), c.status};
+}
+ST_EXPORT int st_qkv_to_cache8(const Cache8Call* c, void* stream) {
+    if (c->n_tokens <= 0) return 0;
+    const int bad = c8_check(*c);
+    if (bad) return bad;
+    if (c->nh <= 0) return ST_ERR_BAD_ARG;
+    if ((long long)c->nh + 2ll * c->nkv > (1 << 16)) return ST_ERR_TOO_LARGE;
+    const Cache8Write a{c->qkv, c->bias, c->q_out, (unsigned char*)c->pool, c->scales, c->positions, c->seq_of_token, c->slots, c8_kv(*c),
+                        c->nh, c->d, c->write_kv};
+    const int act = c->act, form = c->form, n_tokens = c->n_tokens;
     cudaStream_t s = (cudaStream_t)stream;
     if (act == 0 && form == C8_INT8) return c8_launch_write<float, C8_INT8>(a, n_tokens, s);
     if (act == 0 && form == C8_E4M3) return c8_launch_write<float, C8_E4M3>(a, n_tokens, s);
@@ -238,18 +311,18 @@ cache8_rows_kernel(const PagedKV kv, T* __restrict__ out, const int* __restrict_
     const int t = blockIdx.x, pos = positions[t];
     if (pos < 0) return;
     const int page = kv.page(kv.table + (size_t)slots[seq_of_token[t]] * kv.max_pages, pos);
-    const int off = kv.offset(pos, kv.page_index(pos));
+    const uint32_t row0 = page >= 0 ? kv.row0(page, 0, 0) + kv.offset(pos, kv.page_index(pos)) : 0u;    // all heads' keys, then all values
     if (page < 0 && threadIdx.x == 0 && kv.status) atomicExch(kv.status, 1);
     const int per = d / W, total = 2 * kv.nkv * per;
     T* dst = out + (size_t)t * 2 * kv.nkv * d;
+#pragma unroll 4
     for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < total; i += gridDim.y * blockDim.x) {
         const int r = i / per, e = (i - r * per) * W;
         float f[W];
 #pragma unroll
         for (int k = 0; k < W; ++k) f[k] = 0.f;
         if (page >= 0) {
-            const int which = r >= kv.nkv;
-            const uint32_t row = kv.row0(page, which, r - which * kv.nkv) + off;
+            const uint32_t row = row0 + (uint32_t)r * kv.page_size;
             const float s = __ldg(kv.scales + row);
             if constexpr (W == 8) {
                 const uint2 c = __ldg(reinterpret_cast<const uint2*>(kv.pool + (size_t)row * d + e));
@@ -282,14 +355,14 @@ static int c8_launch_rows(const PagedKV& kv, void* out, const int* positions, co
     return st_launch_status();
 }
 
-ST_EXPORT int st_cache8_rows(const void* pool, const float* scales, void* out, const int* positions, const int* seq_of_token,
-                             const int* slots, const int* block_table, int max_pages, int num_pages, int n_layers, int layer, int n_tokens,
-                             int nkv, int d, int page_size, int* status, int act, int form, void* stream) {
-    if (n_tokens <= 0) return 0;
-    if (nkv <= 0 || d <= 0 || page_size <= 0 || layer < 0 || layer >= n_layers || max_pages <= 0 || num_pages <= 0) return ST_ERR_BAD_ARG;
-    if (d > 256 || nkv > (1 << 15) || !c8_rows_fit(num_pages, n_layers, nkv, page_size)) return ST_ERR_TOO_LARGE;
-    const PagedKV kv{(const unsigned char*)pool, scales, block_table, max_pages, num_pages, n_layers, layer, nkv, page_size,
-                     c8_shift(page_size), status};
+ST_EXPORT int st_cache8_rows(const Cache8Call* c, void* stream) {
+    if (c->n_tokens <= 0) return 0;
+    const int bad = c8_check(*c);
+    if (bad) return bad;
+    const PagedKV kv = c8_kv(*c);
+    void* out = c->out;
+    const int *positions = c->positions, *seq_of_token = c->seq_of_token, *slots = c->slots;
+    const int act = c->act, form = c->form, n_tokens = c->n_tokens, d = c->d;
     cudaStream_t s = (cudaStream_t)stream;
     if (act == 0 && form == C8_INT8) return c8_launch_rows<float, C8_INT8>(kv, out, positions, seq_of_token, slots, n_tokens, d, s);
     if (act == 0 && form == C8_E4M3) return c8_launch_rows<float, C8_E4M3>(kv, out, positions, seq_of_token, slots, n_tokens, d, s);

@@ -16,14 +16,14 @@ keys count as absent, and a query without any key gets zeros.  Calls launch on t
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import struct
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
 
-from . import KernelError, _check, _p, _stream, _tc_status_word, lib, sm_count
+from . import KernelError, _check, _current_device, _stream, _tc_status_word, lib, sm_count
 
 CACHE8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _FORMS = {torch.int8: 0, torch.float8_e4m3fn: 1, torch.bfloat16: 2, torch.float32: 3}
@@ -48,33 +48,51 @@ def _need(ok: bool, what: str) -> None:
         raise KernelError(what)
 
 
-def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+# The checks below run in every call of a decode step's layers: they name what is wrong only once something is.
+def _same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """All tensors on one CUDA device, the current one: the launch goes there."""
-    if not first.is_cuda:
+    index = tensors[0].get_device()
+    if index < 0:
         raise KernelError("this engine runs on a CUDA device only; got a CPU tensor")
-    index = first.get_device()
-    for t in others:
+    for t in tensors:
         if t is not None and t.get_device() != index:
             raise KernelError(f"{what}: tensors on different devices")
-    if index != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+    if index != _current_device():
+        raise KernelError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{_current_device()}")
 
 
-def _index(what: str, name: str, t: torch.Tensor, dim: int = 1) -> None:
-    if t.dtype != _I32 or t.dim() != dim or not t.is_contiguous():
-        raise KernelError(f"{what}: {name} is a contiguous int32 tensor of {dim} dimension(s)")
+def _index(what: str, positions, seq_of_token, slots, block_table, n: int) -> None:
+    """int32, contiguous, a position and a request for each of n tokens."""
+    for t in (positions, seq_of_token, slots, block_table):
+        if t is not None and not (t.dtype is _I32 and t.is_contiguous() and t.dim() == (2 if t is block_table else 1)):
+            raise KernelError(f"{what}: positions, seq_of_token, slots (one dimension) and block_table (two) are contiguous int32 tensors")
+    if positions.numel() < n or (seq_of_token is not None and seq_of_token.numel() < n):
+        raise KernelError(f"{what}: a position and a request for every token")
 
 
-def _pool8(what: str, pool: torch.Tensor, scales: Optional[torch.Tensor], layer: int) -> None:
-    _need(pool.dim() == 6 and pool.shape[2] == 2 and pool.is_contiguous(),
-          f"{what}: the pool is a contiguous [pages, layers, 2, kv heads, page size, head size]")
-    _need(pool.dtype in _FORMS, f"{what}: unsupported cache type {pool.dtype}")
-    if pool.dtype in CACHE8_TYPES:
-        _need(scales is not None and scales.dtype == torch.float32 and scales.shape == pool.shape[:5] and scales.is_contiguous(),
-              f"{what}: an 8-bit pool comes with contiguous float32 scales [pages, layers, 2, kv heads, page size]")
-    else:
-        _need(scales is None, f"{what}: scales belong to 8-bit pools")
-    _need(0 <= layer < pool.shape[1], f"{what}: the pool has no layer {layer}")
+def _pool8(what: str, pool: torch.Tensor, scales: Optional[torch.Tensor], layer: int, only8: bool):
+    """The pool's sizes (pages, layers, kv heads, page size, head size) and its form."""
+    shape, form = pool.shape, _FORMS.get(pool.dtype)
+    if len(shape) != 6 or shape[2] != 2 or not pool.is_contiguous():
+        raise KernelError(f"{what}: the pool is a contiguous [pages, layers, 2, kv heads, page size, head size]")
+    if form is None or (only8 and form > 1):
+        raise KernelError(f"{what}: unsupported cache type {pool.dtype}")
+    if form <= 1:
+        if scales is None or scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.shape != shape[:5]:
+            raise KernelError(f"{what}: an 8-bit pool comes with contiguous float32 scales [pages, layers, 2, kv heads, page size]")
+    elif scales is not None:
+        raise KernelError(f"{what}: scales belong to 8-bit pools")
+    pages, layers, _, nkv, page_size, d = shape
+    if not 0 <= layer < layers:
+        raise KernelError(f"{what}: the pool has no layer {layer}")
+    return pages, layers, nkv, page_size, d, form
+
+
+_WRITE = struct.Struct("=11Q12i")
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def qkv_to_cache8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: Optional[torch.Tensor], pool: torch.Tensor,
@@ -86,25 +104,24 @@ def qkv_to_cache8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: Option
     ``qkv`` [tokens, (nh + 2 nkv) d] float32 or bfloat16; ``bias`` float32 or None; ``q_out`` [tokens, nh d] of qkv's type, or None: the
     queries stay where they are.  ``write_kv`` False: only the queries move.  Head sizes up to 256."""
     what = "qkv_to_cache8"
-    n = qkv.shape[0]
     _same_device(what, qkv, bias, q_out, pool, scales, positions, seq_of_token, slots, block_table, status)
-    _need(qkv.dtype in _ACTS and qkv.is_contiguous() and qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * d,
-          f"{what}: qkv is a contiguous [tokens, (nh + 2 nkv) d] of float32 or bfloat16")
-    _need(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == qkv.shape[1]),
-          f"{what}: the bias is contiguous float32, one number per column")
-    _need(q_out is None or (q_out.dtype == qkv.dtype and q_out.shape == (n, nh * d) and q_out.is_contiguous()),
-          f"{what}: q_out is a contiguous [tokens, nh d] of qkv's type")
-    _pool8(what, pool, scales, layer)
-    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
-    _need(pool.shape[3] == nkv and pool.shape[5] == d, f"{what}: the pool has other heads or sizes")
-    for name, t, dim in (("positions", positions, 1), ("seq_of_token", seq_of_token, 1), ("slots", slots, 1),
-                         ("block_table", block_table, 2)):
-        _index(what, name, t, dim)
-    _need(positions.numel() >= n and seq_of_token.numel() >= n, f"{what}: a position and a request for every token")
+    act, cols = _ACTS.get(qkv.dtype), (nh + 2 * nkv) * d
+    if act is None or qkv.dim() != 2 or qkv.shape[1] != cols or not qkv.is_contiguous():
+        raise KernelError(f"{what}: qkv is a contiguous [tokens, (nh + 2 nkv) d] of float32 or bfloat16")
+    n = qkv.shape[0]
+    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != cols or not bias.is_contiguous()):
+        raise KernelError(f"{what}: the bias is contiguous float32, one number per column")
+    if q_out is not None and (q_out.dtype is not qkv.dtype or q_out.shape != (n, nh * d) or not q_out.is_contiguous()):
+        raise KernelError(f"{what}: q_out is a contiguous [tokens, nh d] of qkv's type")
+    pages, layers, pool_kv, page_size, pool_d, form = _pool8(what, pool, scales, layer, True)
+    if pool_kv != nkv or pool_d != d:
+        raise KernelError(f"{what}: the pool has other heads or sizes")
+    _index(what, positions, seq_of_token, slots, block_table, n)
     st = status if status is not None else _tc_status_word(qkv.device)
-    _check(lib().st_qkv_to_cache8(_p(qkv), _p(bias), _p(q_out), _p(pool), _p(scales), _p(positions), _p(seq_of_token), _p(slots),
-                                  _p(block_table), block_table.shape[1], pool.shape[0], pool.shape[1], layer, n, nh, nkv, d,
-                                  pool.shape[4], int(write_kv), _p(st), _ACTS[qkv.dtype], _FORMS[pool.dtype], _stream()), what)
+    call = _WRITE.pack(qkv.data_ptr(), _ptr(bias), _ptr(q_out), pool.data_ptr(), scales.data_ptr(), positions.data_ptr(),
+                       seq_of_token.data_ptr(), slots.data_ptr(), block_table.data_ptr(), st.data_ptr(), 0,
+                       block_table.shape[1], pages, layers, layer, n, nh, nkv, d, page_size, 1 if write_kv else 0, act, form)
+    _check(lib().st_qkv_to_cache8(call, _stream()), what)
 
 
 def cache8_rows(pool: torch.Tensor, scales: torch.Tensor, layer: int, out: torch.Tensor, positions: torch.Tensor,
@@ -114,20 +131,17 @@ def cache8_rows(pool: torch.Tensor, scales: torch.Tensor, layer: int, out: torch
     [tokens, 2 nkv d] float32 or bfloat16, code times scale.  A position without a page gives zeros."""
     what = "cache8_rows"
     _same_device(what, out, pool, scales, positions, seq_of_token, slots, block_table, status)
-    _pool8(what, pool, scales, layer)
-    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
-    nkv, page_size, d = pool.shape[3:]
+    pages, layers, nkv, page_size, d, form = _pool8(what, pool, scales, layer, True)
+    act = _ACTS.get(out.dtype)
+    if act is None or out.dim() != 2 or out.shape[1] != 2 * nkv * d or not out.is_contiguous():
+        raise KernelError(f"{what}: out is a contiguous [tokens, 2 nkv d] of float32 or bfloat16")
     n = out.shape[0]
-    _need(out.dtype in _ACTS and out.is_contiguous() and out.shape == (n, 2 * nkv * d),
-          f"{what}: out is a contiguous [tokens, 2 nkv d] of float32 or bfloat16")
-    for name, t, dim in (("positions", positions, 1), ("seq_of_token", seq_of_token, 1), ("slots", slots, 1),
-                         ("block_table", block_table, 2)):
-        _index(what, name, t, dim)
-    _need(positions.numel() >= n and seq_of_token.numel() >= n, f"{what}: a position and a request for every row")
+    _index(what, positions, seq_of_token, slots, block_table, n)
     st = status if status is not None else _tc_status_word(out.device)
-    _check(lib().st_cache8_rows(_p(pool), _p(scales), _p(out), _p(positions), _p(seq_of_token), _p(slots), _p(block_table),
-                                block_table.shape[1], pool.shape[0], pool.shape[1], layer, n, nkv, d, page_size, _p(st),
-                                _ACTS[out.dtype], _FORMS[pool.dtype], _stream()), what)
+    call = _WRITE.pack(0, 0, 0, pool.data_ptr(), scales.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(),
+                       block_table.data_ptr(), st.data_ptr(), out.data_ptr(),
+                       block_table.shape[1], pages, layers, layer, n, 0, nkv, d, page_size, 0, act, form)
+    _check(lib().st_cache8_rows(call, _stream()), what)
     return out
 
 
@@ -213,55 +227,57 @@ def shared_prefix_plan(groups: Sequence[Sequence[int]], shared: Sequence[int], n
 _CALL = struct.Struct("=13Q3q15if")
 
 
-def _ptr(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
+@functools.lru_cache(maxsize=256)
+def _single_scratch(*sizes: int) -> int:
+    return lib().st_attention_single8_scratch(*sizes)
 
 
 def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale, window, status, *,
-            items=None, n_items=0, plan=None, max_keys=0) -> None:
+            only8=True, items=None, n_items=0, plan=None, max_keys=0) -> None:
     _same_device(what, q, pool, scales, out, positions, seq_of_token, slots, block_table, status, items,
                  plan.tiles if plan is not None else None)
-    _pool8(what, pool, scales, layer)
-    n_pages, n_layers, _, nkv, page_size, d = pool.shape
-    n = out.shape[0]
-    _need(nh > 0 and nh % nkv == 0, f"{what}: {nh} heads cannot share {nkv} key/value heads")
-    _need(q.dtype in _ACTS and out.dtype == q.dtype, f"{what}: queries and results are float32 or bfloat16, of one type")
-    _need(pool.dtype in CACHE8_TYPES or pool.dtype == q.dtype, f"{what}: a {pool.dtype} cache with {q.dtype} queries")
-    _need(q.dim() == 2 and out.is_contiguous() and q.shape == out.shape and q.shape[1] == nh * d and q.stride(1) == 1,
-          f"{what}: q and out are [tokens, nh d], out contiguous, q's rows contiguous")
-    stride = q.stride(0) if n > 1 else nh * d
-    _need(scale > 0.0, f"{what}: the scale is positive")
-    _need(window >= 0, f"{what}: the window is not negative")
-    _index(what, "positions", positions)
-    _index(what, "slots", slots)
-    _index(what, "block_table", block_table, 2)
-    if seq_of_token is not None:
-        _index(what, "seq_of_token", seq_of_token)
-    if items is not None:
-        _index(what, "items", items)
-    _need(positions.numel() >= n and (seq_of_token is None or seq_of_token.numel() >= n),
-          f"{what}: a position and a request for every token")
-    if stride != nh * d:
-        _need(plan is not None and plan.kind == "portion" and stride >= nh * d, f"{what}: q is contiguous")
-    else:
-        stride = 0
-    st = status if status is not None else _tc_status_word(q.device)
+    pages, layers, nkv, page_size, d, form = _pool8(what, pool, scales, layer, only8)
+    act = _ACTS.get(q.dtype)
+    if nh <= 0 or nh % nkv:
+        raise KernelError(f"{what}: {nh} heads cannot share {nkv} key/value heads")
+    if act is None or out.dtype is not q.dtype or (form > 1 and pool.dtype is not q.dtype):
+        raise KernelError(f"{what}: queries and results of one type, float32 or bfloat16, that of a cache that is not in 8 bits")
+    width, n = nh * d, out.shape[0]
+    if q.dim() != 2 or q.shape != out.shape or q.shape[1] != width or not out.is_contiguous() or (width > 1 and q.stride(1) != 1):
+        raise KernelError(f"{what}: q and out are [tokens, nh d], out contiguous, q's rows contiguous")
+    stride = q.stride(0) if n > 1 else width
+    if not scale > 0.0 or window < 0:
+        raise KernelError(f"{what}: the scale is positive, the window not negative")
+    _index(what, positions, seq_of_token, slots, block_table, n)
     n_tiles = total = max_rows = 0
     tiles = info = None
     if plan is not None:
-        _need(plan.nh == nh and plan.nkv == nkv, f"{what}: the plan is for {plan.nh} heads over {plan.nkv}")
-        _need(plan.n_tokens <= n and plan.n_seqs <= slots.numel(), f"{what}: the plan names tokens or requests that are not there")
+        if plan.nh != nh or plan.nkv != nkv:
+            raise KernelError(f"{what}: the plan is for {plan.nh} heads over {plan.nkv}")
+        if plan.n_tokens > n or plan.n_seqs > slots.numel():
+            raise KernelError(f"{what}: the plan names tokens or requests that are not there")
         tiles, info, items = plan.tiles, plan.info, plan.items
         n_items, n_tiles, total, max_rows = plan.n_items, plan.n_tiles, plan.total, plan.max_rows
+    elif items is not None and not (items.dtype is _I32 and items.dim() == 1 and items.is_contiguous()):
+        raise KernelError(f"{what}: items is a contiguous int32 tensor of one dimension")
+    if stride != width:
+        if plan is None or plan.kind != "portion" or stride < width:
+            raise KernelError(f"{what}: q is contiguous")
+    else:
+        stride = 0
+    st = status if status is not None else _tc_status_word(q.device)
+    reach = block_table.shape[1] * page_size             # a hint of more keys than the table has room for is none
+    max_keys = min(max_keys, reach) if max_keys > 0 else reach
+    if 0 < window < max_keys:
+        max_keys = window
     # parts of rows that several blocks leave: a slot per (tile, key head) and one per walker of the line; those of single tokens
     floats = (n_tiles * nkv + 3 * sm_count(q.device)) * ROWS_PER_TILE * (2 + d) if total else 0
     if n_items:
-        floats += lib().st_attention_single8_scratch(n_items, nh, nkv, d, page_size, max_keys, _ACTS[q.dtype], _FORMS[pool.dtype])
+        floats += _single_scratch(n_items, nh, nkv, d, page_size, max_keys, act, form)
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     call = _CALL.pack(q.data_ptr(), out.data_ptr(), pool.data_ptr(), _ptr(scales), block_table.data_ptr(), positions.data_ptr(),
                       _ptr(seq_of_token), slots.data_ptr(), _ptr(items), _ptr(tiles), _ptr(info), _ptr(scratch), st.data_ptr(),
-                      stride, n_pages, scratch.numel() if scratch is not None else 0,
-                      block_table.shape[1], n_layers, layer, nh, nkv, d, page_size, window, _ACTS[q.dtype], _FORMS[pool.dtype],
+                      stride, pages, floats, block_table.shape[1], layers, layer, nh, nkv, d, page_size, window, act, form,
                       n_items, n_tiles, total, max_rows, max_keys, scale)
     _check(entry(call, _stream()), what)
 
@@ -275,14 +291,10 @@ def attention_cache8_single(q: torch.Tensor, pool: torch.Tensor, scales: torch.T
     the rows of ``out`` of other tokens stay.  ``max_kv``: about the most keys a token reads (0: what the block table has room
     for); it decides how the work is spread, not the result's meaning."""
     what = "attention_cache8_single"
-    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
-    _need(0 <= n_items <= (items.numel() if items is not None else out.shape[0]), f"{what}: n_items tokens are not there")
-    reach = block_table.shape[-1] * pool.shape[4] if pool.dim() == 6 else 0
-    keys = min(max_kv, reach) if max_kv > 0 else reach
-    if window > 0:
-        keys = min(keys, window)
+    if not 0 <= n_items <= (items.numel() if items is not None else out.shape[0]):
+        raise KernelError(f"{what}: n_items tokens are not there")
     _attend(what, lib().st_attention_single8, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale,
-            window, status, items=items, n_items=n_items, max_keys=keys)
+            window, status, items=items, n_items=n_items, max_keys=max_kv)
     return out
 
 
@@ -293,8 +305,8 @@ def attention_cache8_tiles(q: torch.Tensor, pool: torch.Tensor, scales: torch.Te
     ``portion_plan``, of the same heads and window.  ``q`` may be the first columns of the q|k|v product (any row stride).  The
     portions' own keys and values have been written (``qkv_to_cache8``)."""
     what = "attention_cache8_tiles"
-    _need(pool.dtype in CACHE8_TYPES, f"{what}: an 8-bit pool")
-    _need(plan.kind == "portion" and plan.window == window, f"{what}: the plan is from portion_plan, for this window")
+    if plan.kind != "portion" or plan.window != window:
+        raise KernelError(f"{what}: the plan is from portion_plan, for this window")
     _attend(what, lib().st_attention_tiles8, q, pool, scales, layer, out, positions, None, slots, block_table, nh, scale, window,
             status, plan=plan)
     return out
@@ -312,8 +324,8 @@ def attention_shared_prefix(q: torch.Tensor, pool: torch.Tensor, layer: int, out
     ``window`` of these).  A value that is not finite reaches, in bfloat16 caches, all rows of its group that share it, also those
     whose window or position hides it; in the other forms only rows that see it."""
     what = "attention_shared_prefix"
-    _need(plan.kind == "shared", f"{what}: the plan is from shared_prefix_plan")
-    keys = plan.max_own if plan.max_own > 0 else block_table.shape[-1] * pool.shape[4] if pool.dim() == 6 else 0
+    if plan.kind != "shared":
+        raise KernelError(f"{what}: the plan is from shared_prefix_plan")
     _attend(what, lib().st_attention_shared, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale,
-            window, status, plan=plan, max_keys=keys)
+            window, status, only8=False, plan=plan, max_keys=plan.max_own)
     return out

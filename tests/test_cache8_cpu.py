@@ -130,8 +130,8 @@ class Fake:
 
 @pytest.fixture()
 def fake(monkeypatch):
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     from swifttransformer_b200.ops import cache8
+    monkeypatch.setattr(cache8, "_current_device", lambda: 0)
 
     def reached(*a, **k):
         raise AssertionError("the call reached the library")
@@ -188,7 +188,8 @@ def test_single_tokens_refuse(fake, what, change):
 
 
 def test_another_device_than_the_current_one(fake, monkeypatch):
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    from swifttransformer_b200.ops import cache8
+    monkeypatch.setattr(cache8, "_current_device", lambda: 1)
     with pytest.raises(KernelError, match="current device"):
         ops.attention_cache8_single(**base(fake))
 
