@@ -32,6 +32,7 @@
 #define RT_REGS_ISSUE 32
 #define RT_REGS_ALL (256 * RT_REGS_SOFTMAX + 256 * RT_REGS_BRING + 128 * RT_REGS_ISSUE)
 static_assert(RT_REGS_ALL <= RT_THREADS * 96, "more registers than the block owns");
+#define RT_STAGE 2048                    // bytes a softmax warp's results go through on their way out: 32 rows of 16
 #define RT_META 4                        // tiles whose scales are kept: see below
 
 __device__ __forceinline__ void rt_mbar_arrive(uint32_t mbar) {
@@ -64,6 +65,13 @@ __device__ __forceinline__ uint32_t rt_bits(int lo, int hi) {
     return lo <= 0 ? below : lo >= 32 ? 0u : below & (0xffffffffu << lo);
 }
 
+__device__ __forceinline__ void rt_ld16(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+
 // the keys of a piece: tiles of 64 from k0 on, below k_end
 struct RtKeys { int k0, k_end, n; };
 __device__ __forceinline__ RtKeys rt_keys(const RowPiece& p) {
@@ -89,7 +97,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     constexpr int DB = DP / 64;                                        // blocks of 64 dimensions
     constexpr uint32_t Q_BLK = TC_BM * 128, KV_BLK = TC_BN * 128;      // bytes of a [rows][64] block
     constexpr uint32_t Q_BUF = DB * Q_BLK, BUF = DB * KV_BLK;
-    constexpr uint32_t ALL_BYTES = 2 * Q_BUF + 8 * BUF;
+    constexpr uint32_t ALL_BYTES = 2 * Q_BUF + 8 * BUF + 8 * RT_STAGE;
     constexpr int WG_COLS = 256, T_O = 64, T_P = 64 + DP;              // a group's columns: S, O, P
     constexpr uint32_t NONE = 0xffffffffu;
     extern __shared__ unsigned char rt_raw[];
@@ -365,6 +373,11 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             const int place = nx.t.first + row / g;
             token_n = row < nx.t.n_tok * g ? (a.plan.items ? __ldg(a.plan.items + place) : place) : -1;
             pos_n = token_n >= 0 ? __ldg(a.positions + token_n) : -1;
+            if (token_n >= 0) {                          // the row's lines, for `bring`
+                const bf16* q = (const bf16*)a.q + (size_t)token_n * a.q_stride + (nx.head * g + row % g) * d;
+                asm volatile("prefetch.global.L1 [%0];\n" ::"l"(q));
+                if (DP == 128) asm volatile("prefetch.global.L1 [%0];\n" ::"l"(q + (d > 64 ? 64 : 0)));
+            }
             return true;
         };
         // The warp's 32 rows of `nx` into shared memory: NP neighbouring lanes have a row, RI rows to a load.  All S over the queries
@@ -540,36 +553,59 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             if (alive) alive = tc_wait_warp(mb_o, (n + keys.n - 1) & 1, dead);
             tc_fence_after_sync();
             n += keys.n;
-            // ---- the piece's sums: out, or into its slot
-            const bool direct = a.direct && pc.whole, store = row < rows && pos >= 0 && alive;
-            const size_t slot = ((size_t)(pc.unit + 2 * blockIdx.x + wg)) * AR_ROWS + row;
-            if (!direct && row < rows) { a.parts.r[slot] = ref; a.parts.l[slot] = sum; }
+            // ---- the piece's sums: out, or into its slot.  Sixteen dimensions at a time change hands in shared memory, so that
+            // neighbouring lanes store a row's neighbouring pieces (a thread's own row has a line of its own in every store).
+            const bool direct = a.direct && pc.whole;
+            const size_t slot0 = ((size_t)(pc.unit + 2 * blockIdx.x + wg)) * AR_ROWS;
+            if (!direct && row < rows) { a.parts.r[slot0 + row] = ref; a.parts.l[slot0 + row] = sum; }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            bf16* out = (bf16*)a.out + ((size_t)(token >= 0 ? token : 0) * a.plan.nh + pc.head * g + row % g) * d;
-            float* part = a.parts.o + slot * d;
+            const bool store = row < rows && pos >= 0 && alive;
+            // rows that this lane stores: direct 16 i + lane / 2 (two lanes a row), else 8 i + lane / 4
+            const long long mine = store ? direct ? ((long long)token * a.plan.nh + pc.head * g + row % g) * d : (long long)(slot0 + row) * d : -1;
+            long long to[4];
 #pragma unroll
-            for (int cb = 0; cb < DP / 32; ++cb) {
-                float o[32];
+            for (int i = 0; i < 4; ++i)
+                to[i] = __shfl_sync(0xffffffffu, mine, direct ? (16 * i + (lane >> 1)) & 31 : 8 * i + (lane >> 2));
+            const uint32_t stage = base + 2 * Q_BUF + 8 * BUF + warp * RT_STAGE;
+#pragma unroll
+            for (int cb = 0; cb < DP / 16; ++cb) {
+                float o[16];
                 __syncwarp();
-                tc_ld32(t_wg + T_O + cb * 32, o);
+                rt_ld16(t_wg + T_O + cb * 16, o);
                 tc_ld_wait();
+                // row `lane`: four pieces of 16 bytes, turned by the row so that eight lanes hit all banks
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    // the piece of eight dimensions that is kept at place 4 cb + c
-                    const int at = 4 * cb + c, e = 8 * (HALF && DP == 128 ? (at & 7) * 2 + (at >> 3) : at);
-                    if (!store || e >= d) continue;
-                    const float* v = o + 8 * c;
-                    if (direct) {
-                        uint32_t h[4];
+                for (int c = 0; c < 4; ++c)
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n"
+                                 ::"r"(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)), "f"(direct ? o[4 * c] * inv : o[4 * c]),
+                                   "f"(direct ? o[4 * c + 1] * inv : o[4 * c + 1]), "f"(direct ? o[4 * c + 2] * inv : o[4 * c + 2]),
+                                   "f"(direct ? o[4 * c + 3] * inv : o[4 * c + 3]) : "memory");
+                __syncwarp();
+                auto read = [&](int r, int c) -> float4 {
+                    float4 v;
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                                 : "r"(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) : "memory");
+                    return v;
+                };
+                // the eight dimensions that are kept at place 2 cb + c
+                auto dim = [&](int c) { const int at = 2 * cb + c; return 8 * (HALF && DP == 128 ? (at & 7) * 2 + (at >> 3) : at); };
+                if (direct) {
+                    const int c = lane & 1, e = c ? dim(1) : dim(0);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j] * inv, v[2 * j + 1] * inv);
-                            h[j] = *reinterpret_cast<const uint32_t*>(&b);
-                        }
-                        *reinterpret_cast<uint4*>(out + e) = make_uint4(h[0], h[1], h[2], h[3]);
-                    } else {
-                        store4(part + e, make_float4(v[0], v[1], v[2], v[3]));
-                        store4(part + e + 4, make_float4(v[4], v[5], v[6], v[7]));
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = 16 * i + (lane >> 1);
+                        const float4 x = read(r, 2 * c), y = read(r, 2 * c + 1);
+                        if (to[i] < 0 || e >= d) continue;
+                        const __nv_bfloat162 b[4] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w), __floats2bfloat162_rn(y.x, y.y),
+                                                     __floats2bfloat162_rn(y.z, y.w)};
+                        *reinterpret_cast<uint4*>((bf16*)a.out + to[i] + e) = *reinterpret_cast<const uint4*>(b);
+                    }
+                } else {
+                    const int c = lane & 3, e = (c >> 1 ? dim(1) : dim(0)) + (c & 1) * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 v = read(8 * i + (lane >> 2), c);
+                        if (to[i] >= 0 && e < d) store4(a.parts.o + to[i] + e, v);
                     }
                 }
             }
@@ -584,7 +620,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
 }
 
 template <int FORM, int DP> static int rt_run(const RowArgs& a, cudaStream_t s) {
-    constexpr size_t smem = 2 * (DP / 64) * TC_BM * 128 + 8 * (DP / 64) * TC_BN * 128 + 1024;
+    constexpr size_t smem = 2 * (DP / 64) * TC_BM * 128 + 8 * (DP / 64) * TC_BN * 128 + 8 * RT_STAGE + 1024;
     auto kernel = attention_rows_tc_kernel<FORM, DP>;
     AR_ALLOW_SMEM(kernel, smem);
     // the redistribution of registers moves what the launch got, and waits for more for ever: only for a kernel compiled as assumed
