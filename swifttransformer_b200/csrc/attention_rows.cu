@@ -509,6 +509,7 @@ static RowArgs ar_row_args(const RowCall& c) {
 
 ST_EXPORT int st_attention_rows_per_tile() { return AR_ROWS; }
 ST_EXPORT int st_attention_rows_chunk() { return AR_CHUNK; }
+ST_EXPORT int st_attention_rows_unit() { return AR_UNIT; }
 // floats of scratch that single tokens want for this call (0: none), laid out at `from`
 static long long ar_line(const RowCall& c, SingleArgs* a, float* from) {
     if (c.nkv <= 0 || c.d <= 0 || !ar_single_fast(c.page_size, c.d, c.form)) return 0;

@@ -3,9 +3,9 @@
 //
 // A row is one (token, query head).  A tile holds the rows of up to 128 / g tokens, for one key head, g = query heads per key
 // head: row r is head r % g of the group of token r / g.  The tile's keys [key_lo, key_hi) are walked in chunks of AR_CHUNK.
-// All chunks of all (tile, key head) pairs ("units"), one unit's behind the other's, each unit with a place of its own in front for what
-// its begin and end cost (about a chunk's time: without it the walkers of a prompt's first, short units were the last by a factor of
-// two), form one line of `total` places which is cut
+// All chunks of all (tile, key head) pairs ("units"), one unit's behind the other's, each unit with AR_UNIT places in front for what its
+// begin and end cost (without them the walkers of a prompt's first, short units were the last by a factor of two), form one line
+// of `total` places which is cut
 // into runs of `run` places, one per walker (a block, or one of a block's two groups): every walker gets the same work however
 // unequal the tiles are, and a unit that a cut goes through is put together from parts.  Part (unit u, walker c) has slot u + c: a
 // new slot begins with every unit and with every run, so no two parts share one.
@@ -16,7 +16,8 @@
 #include "cache8.cuh"
 
 #define AR_ROWS 128
-#define AR_CHUNK 128
+#define AR_CHUNK 64
+#define AR_UNIT 3                 // what a unit's begin and end cost, in chunks
 #define AR_LOG2E 1.4426950408889634f
 
 // a tile of a plan: six numbers in the plan's array
@@ -59,7 +60,7 @@ __device__ __forceinline__ RowTile ar_tile(const RowPlan& p, int i) {
 __device__ __forceinline__ int ar_chunks(const RowTile& t) {
     return t.key_hi > t.key_lo ? (t.key_hi - (t.key_lo & ~(AR_CHUNK - 1)) + AR_CHUNK - 1) / AR_CHUNK : 0;
 }
-__device__ __forceinline__ int ar_places(int chunks) { return chunks > 0 ? chunks + 1 : 0; }      // of a unit in the line
+__device__ __forceinline__ int ar_places(int chunks) { return chunks > 0 ? chunks + AR_UNIT : 0; }      // of a unit in the line
 
 // A walker's way along its run: pieces of one (tile, key head) pair.  A walker behind the line's end has none.
 struct RowPiece {
@@ -71,14 +72,19 @@ struct RowPiece {
 struct RowWalk {
     int at, end, tile;
     RowTile t;
+    // by a whole warp
     __device__ __forceinline__ void begin(const RowPlan& p, int c) {
         at = min(c * p.run, p.total);
         end = min(at + p.run, p.total);
-        // the last tile that starts at or before `at` (tiles without chunks start where the next one does)
-        int lo = 0, hi = p.n_tiles - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (__ldg(p.tiles + 6 * mid + 5) <= at) lo = mid; else hi = mid - 1;
+        // the last tile that starts at or before `at` (tiles without chunks start where the next one does), by 32 at a time
+        int lo = 0, n = p.n_tiles;
+        while (n > 1) {
+            const int step = (n + 31) / 32, i = lo + (int)(threadIdx.x & 31) * step;
+            const bool before = i < lo + n && __ldg(p.tiles + 6 * i + 5) <= at;
+            const uint32_t set = __ballot_sync(0xffffffffu, before);
+            const int k = set ? 31 - __clz(set) : 0;
+            n = min(step, n - k * step);
+            lo += k * step;
         }
         tile = lo;
         t = ar_tile(p, tile);
@@ -93,15 +99,16 @@ struct RowWalk {
         }
         const int in = at - t.start, head = in / ar_places(n);
         int c = in - head * ar_places(n);
-        if (c == 0) {                                    // the unit's own place
-            c = 1;
-            if (++at >= end) return false;
+        if (c < AR_UNIT) {                               // the unit's own places
+            at += AR_UNIT - c;
+            c = AR_UNIT;
+            if (at >= end) return false;
         }
         out.t = t;
         out.tile = tile;
         out.head = head;
         out.unit = tile * p.nkv + head;
-        out.chunk0 = c - 1;
+        out.chunk0 = c - AR_UNIT;
         out.chunks = min(n - out.chunk0, end - at);
         out.whole = out.chunks == n;
         at += out.chunks;
@@ -110,7 +117,7 @@ struct RowWalk {
 };
 // the walkers of unit (tile t, key head) with n > 0 chunks: c0 to c1
 __device__ __forceinline__ void ar_walkers(const RowPlan& p, const RowTile& t, int head, int n, int& c0, int& c1) {
-    const int x0 = t.start + head * ar_places(n) + 1;
+    const int x0 = t.start + head * ar_places(n) + AR_UNIT;
     c0 = x0 / p.run;
     c1 = (x0 + n - 1) / p.run;
 }

@@ -131,7 +131,11 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         tc_mbar_init_fence();
         s_dead = 0;
     }
-    if (tid == 32 || tid == 64) s_walk[(tid >> 5) - 1].begin(a.plan, 2 * blockIdx.x + (tid >> 5) - 1);
+    if (warp == 1 || warp == 2) {
+        RowWalk w;
+        w.begin(a.plan, 2 * blockIdx.x + warp - 1);
+        if (lane == 0) s_walk[warp - 1] = w;
+    }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");

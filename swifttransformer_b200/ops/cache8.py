@@ -29,9 +29,10 @@ CACHE8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _FORMS = {torch.int8: 0, torch.float8_e4m3fn: 1, torch.bfloat16: 2, torch.float32: 3}
 _ACTS = {torch.float32: 0, torch.bfloat16: 1}
 _I32 = torch.int32
-# query rows of a tile, keys of a chunk (the library's; see st_attention_rows_per_tile, st_attention_rows_chunk)
+# the library's: query rows of a tile, keys of a chunk, places of a (tile, key head) beside its chunks (csrc/attention_rows.cuh)
 ROWS_PER_TILE = 128
-ROWS_CHUNK = 128
+ROWS_CHUNK = 64
+ROWS_UNIT = 3
 
 
 def cache8_pool(num_pages: int, n_layers: int, nkv: int, page_size: int, d: int, dtype: torch.dtype, device):
@@ -150,7 +151,7 @@ class RowPlan:
     """Which query rows share a pass over which keys: made on the host once per step, used by all its layers.
 
     ``tiles``: int32 [n_tiles, 6] on the device: first token (or place in ``items``), tokens, request (-1: that of the first
-    item), first and last + 1 key, and where the tile begins in the line of all units (a place per unit and per chunk of keys).  ``items``: the tokens of
+    item), first and last + 1 key, and where the tile begins in the line of all units (places per unit and per chunk of keys).  ``items``: the tokens of
     a plan for shared prefixes in the tiles' order; ``info`` [items, 3]: keys shared with the group, tile, place in the tile."""
 
     def __init__(self, kind: str, nh: int, nkv: int, device):
@@ -174,7 +175,7 @@ class RowPlan:
         for first, n, seq, lo, hi in tiles:
             rows.append((first, n, seq, lo, hi, start))
             chunks = self._chunks(lo, hi)
-            start += (chunks + 1) * self.nkv if chunks else 0
+            start += (chunks + ROWS_UNIT) * self.nkv if chunks else 0
         _need(start < 1 << 31 and len(rows) * self.nkv < 1 << 22, "a plan of more keys than one call serves")
         self.total, self.n_tiles = start, len(rows)
         self.max_rows = max((r[1] for r in rows), default=0) * (self.nh // self.nkv)

@@ -6,6 +6,9 @@ import torch
 
 from swifttransformer_b200 import ops
 from swifttransformer_b200.ops import KernelError
+from swifttransformer_b200.ops.cache8 import ROWS_CHUNK as CHUNK
+from swifttransformer_b200.ops.cache8 import ROWS_PER_TILE
+from swifttransformer_b200.ops.cache8 import ROWS_UNIT as UNIT
 
 
 def walk(plan, ctas):
@@ -17,15 +20,15 @@ def walk(plan, ctas):
     for c in range(ctas):
         for x in range(bounds[c], bounds[c + 1]):
             t = max(i for i, r in enumerate(tiles) if r[5] <= x and chunks(r) > 0)
-            head, place = divmod(x - tiles[t][5], chunks(tiles[t]) + 1)
-            if place:                                   # place 0 stands for what a unit costs beside its chunks
-                pieces.append((c, t, head, place - 1))
+            head, place = divmod(x - tiles[t][5], chunks(tiles[t]) + UNIT)
+            if place >= UNIT:                           # the first places stand for what a unit costs beside its chunks
+                pieces.append((c, t, head, place - UNIT))
     return pieces
 
 
 def chunks(tile):
     lo, hi = tile[3], tile[4]
-    return -(-(hi - lo // 128 * 128) // 128) if hi > lo else 0
+    return -(-(hi - lo // CHUNK * CHUNK) // CHUNK) if hi > lo else 0
 
 
 @pytest.mark.parametrize("seed", range(6))
@@ -38,7 +41,7 @@ def test_every_key_of_every_row_is_in_one_chunk(seed):
     starts = [rng.choice([0, 1, 128, rng.randint(0, 900)]) for _ in lens]
     plan = ops.portion_plan(lens, starts, nh, nkv, window, "cpu")
     tiles = plan.tiles.view(-1, 6).tolist() if plan.n_tiles else []
-    assert plan.n_tokens == sum(lens) and plan.total == sum(chunks(t) + 1 for t in tiles if chunks(t)) * nkv
+    assert plan.n_tokens == sum(lens) and plan.total == sum(chunks(t) + UNIT for t in tiles if chunks(t)) * nkv
     rows = []
     first = 0
     for seq, (n, s) in enumerate(zip(lens, starts)):
@@ -60,12 +63,17 @@ def test_every_key_of_every_row_is_in_one_chunk(seed):
             assert len(got) == len(set(p[1:] for p in got)) == sum(chunks(t) for t in tiles) * nkv
 
 
+def test_the_plans_sizes_are_the_librarys():
+    lib = ops.lib()
+    assert (ROWS_PER_TILE, CHUNK, UNIT) == (lib.st_attention_rows_per_tile(), lib.st_attention_rows_chunk(), lib.st_attention_rows_unit())
+
+
 def test_shared_plan():
     plan = ops.shared_prefix_plan([[5, 2, 9], [], [0], [7, 8]], [300, 10, 0, 128], 64, 1, "cpu", 17)
     assert plan.tokens_per_tile == 2 and plan.items.tolist() == [5, 2, 9, 0, 7, 8]
-    assert plan.tiles.view(-1, 6).tolist() == [[0, 2, -1, 0, 300, 0], [2, 1, -1, 0, 300, 4], [3, 1, -1, 0, 0, 8], [4, 2, -1, 0, 128, 8]]
+    assert plan.tiles.view(-1, 6).tolist() == [[0, 2, -1, 0, 300, 0], [2, 1, -1, 0, 300, 8], [3, 1, -1, 0, 0, 16], [4, 2, -1, 0, 128, 16]]
     assert plan.info.view(-1, 3).tolist() == [[300, 0, 0], [300, 0, 1], [300, 1, 0], [0, 2, 0], [128, 3, 0], [128, 3, 1]]
-    assert plan.total == 10 and plan.n_items == 6 and plan.max_rows == 128 and plan.n_tokens == 10 and plan.max_own == 17
+    assert plan.total == 21 and plan.n_items == 6 and plan.max_rows == 128 and plan.n_tokens == 10 and plan.max_own == 17
 
 
 @pytest.mark.parametrize("make", [
