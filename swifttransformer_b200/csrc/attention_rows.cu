@@ -513,7 +513,7 @@ ST_EXPORT int st_attention_rows_unit() { return AR_UNIT; }
 // floats of scratch that single tokens want for this call (0: none), laid out at `from`
 static long long ar_line(const RowCall& c, SingleArgs* a, float* from) {
     if (c.nkv <= 0 || c.d <= 0 || !ar_single_fast(c.page_size, c.d, c.form)) return 0;
-    const LineShape s = sg_line_shape(c.n_items, c.nh / c.nkv, c.nkv, c.d, c.max_keys, c.act == 0, c.form);
+    const LineShape s = sg_line_shape(c.n_items, c.nh / c.nkv, c.nkv, c.d, c.max_keys, (long long)c.max_pages * c.page_size, c.act == 0, c.form);
     if (!s.walkers) return 0;
     const long long rows = s.slots * s.R, units = s.slots - s.walkers;
     if (a) {
@@ -523,9 +523,9 @@ static long long ar_line(const RowCall& c, SingleArgs* a, float* from) {
     }
     return rows * (2 + c.d) + 2 * units;
 }
-ST_EXPORT long long st_attention_single8_scratch(int n_items, int nh, int nkv, int d, int page_size, int max_keys, int act, int form) {
+ST_EXPORT long long st_attention_single8_scratch(int n_items, int nh, int nkv, int d, int page_size, int max_pages, int max_keys, int act, int form) {
     RowCall c{};
-    c.n_items = n_items; c.nh = nh; c.nkv = nkv; c.d = d; c.page_size = page_size; c.max_keys = max_keys; c.act = act; c.form = form;
+    c.n_items = n_items; c.nh = nh; c.nkv = nkv; c.d = d; c.page_size = page_size; c.max_pages = max_pages; c.max_keys = max_keys; c.act = act; c.form = form;
     return ar_line(c, nullptr, nullptr);
 }
 

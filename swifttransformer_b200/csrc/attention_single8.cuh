@@ -807,11 +807,12 @@ template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a
 
 // How a call is dealt out as one line, walkers 0 if it is not: it pays (two launches, parts through memory) from four runs a warp on.
 struct LineShape { int walkers, R; long long slots; };
-static inline LineShape sg_line_shape(int n_items, int group, int nkv, int d, int max_keys, bool float_q, int form) {
+static inline LineShape sg_line_shape(int n_items, int group, int nkv, int d, int max_keys, long long reach, bool float_q, int form) {
     LineShape s{0, float_q || (form == C8_BF16 && group <= 4) ? 4 : 8, 0};
     const int row = d * c8_bytes(form), kt = sg_run_keys(row), walkers = st_sm_count() * sg_line_blocks(row) * SG_LINE_WARPS;
     const long long parts = (long long)n_items * nkv * ((group + s.R - 1) / s.R), runs = parts * ((max_keys + kt - 1) / kt);
-    if (n_items > SG_LINE_ITEMS || runs < 4ll * walkers || runs >= (1 << 30)) return s;
+    // (the device counts the line's runs, of up to `reach` keys a token, in 32 bits)
+    if (n_items > SG_LINE_ITEMS || runs < 4ll * walkers || parts * (reach / kt + 2) >= (1 << 30)) return s;
     s.walkers = walkers;
     s.slots = parts + walkers;
     return s;

@@ -274,7 +274,7 @@ def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_tok
     # parts of rows that several blocks leave: a slot per (tile, key head) and one per walker of the line; those of single tokens
     floats = (n_tiles * nkv + 3 * sm_count(q.device)) * ROWS_PER_TILE * (2 + d) if total else 0
     if n_items:
-        floats += _single_scratch(n_items, nh, nkv, d, page_size, max_keys, act, form)
+        floats += _single_scratch(n_items, nh, nkv, d, page_size, block_table.shape[1], max_keys, act, form)
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     call = _CALL.pack(q.data_ptr(), out.data_ptr(), pool.data_ptr(), _ptr(scales), block_table.data_ptr(), positions.data_ptr(),
                       _ptr(seq_of_token), slots.data_ptr(), _ptr(items), _ptr(tiles), _ptr(info), _ptr(scratch), st.data_ptr(),

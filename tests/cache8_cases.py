@@ -38,7 +38,7 @@ class Step:
     (requests, keys in common): the members' first keys are the first member's."""
 
     def __init__(self, requests, heads, kv, dim, form, act, page_size=16, seed=0, shared=(), pad=0, layers=2, layer=1, q_std=1.5,
-                 k_std=0.6, v_std=1.0):
+                 k_std=0.6, v_std=1.0, table_wide=0):
         gen = torch.Generator(device="cuda").manual_seed(seed)
         rng = random.Random(seed)
         self.heads, self.kv, self.dim, self.form, self.act, self.layer, self.page_size = heads, kv, dim, form, act, layer, page_size
@@ -49,7 +49,7 @@ class Step:
         rng.shuffle(order)
         n_slots = len(requests) + 1
         slots = rng.sample(range(n_slots), len(requests))
-        table = torch.full((n_slots, max(need) + 1), -1, dtype=torch.int32)
+        table = torch.full((n_slots, max(max(need) + 1, table_wide)), -1, dtype=torch.int32)
         k = [torch.randn((kv, e, dim), generator=gen, device="cuda") * k_std for e in ends]
         v = [torch.randn((kv, e, dim), generator=gen, device="cuda") * v_std for e in ends]
         for x in v:

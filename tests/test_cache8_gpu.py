@@ -172,6 +172,40 @@ def test_many_single_tokens(form, act):
     check(step, single(step))
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (8, 2, 128), (24, 2, 64), (12, 3, 80), (6, 2, 96), (2, 2, 32), (20, 2, 128)])
+@pytest.mark.parametrize("form,act", [("int8", "bf16"), ("e4m3", "bf16"), ("int8", "f32"), ("e4m3", "f32")])
+def test_tokens_dealt_out_as_one_line(form, act, heads, kv, dim):
+    """A block table with room for so many keys that the calls are dealt out run by run: units in one warp, cut by one warp's end, by many."""
+    step = Step([(0, 1), (2900, 1), (40, 2), (7, 1), (640, 1), (33, 1), (64, 1)], heads, kv, dim, form, act, 16, seed=dim + 1, pad=2, table_wide=4000)
+    check(step, single(step))
+    assert int(step.status) == 0
+    check(step, single(step, window=70), window=70)
+    got = single(step, items=ints([6, -1, 1, 9, 3]), n_items=5)
+    check(step, got, rows=[1, 3, 6])
+    others = [0, 2, 4, 5, 7, 8, 9]
+    assert float(got[others].min()) == 77.0 and float(got[others].max()) == 77.0
+    assert torch.equal(single(step), single(step))
+    s = step.slots.tolist()
+    step.table[s[1], 3] = -1
+    step.table[s[4], :] = 99999
+    hidden = [(1, j) for j in range(48, 64)] + [(4, j) for j in range(641)]
+    check(step, single(step), hidden=hidden)
+    assert int(step.status) == 1
+
+
+@pytest.mark.parametrize("form,act,heads,dim", [("int8", "bf16", 8, 64), ("e4m3", "bf16", 16, 128), ("e4m3", "f32", 8, 64)])
+def test_a_line_of_windows(form, act, heads, dim):
+    """So many windows that the call is dealt out as one line: whole ones, ones that reach before the first key, empty lengths."""
+    step = Step([(11 * i % 700, 1) for i in range(190)], heads, 8, dim, form, act, 16, seed=6)
+    check(step, single(step, window=400), window=400)
+    assert int(step.status) == 0
+
+
+def test_more_tokens_than_a_line_takes():
+    step = Step([(13 * i % 61, 1) for i in range(1100)], 4, 2, 64, "int8", "bf16", 16, seed=7, table_wide=40)
+    check(step, single(step))
+
+
 def test_listed_tokens_only():
     step = Step([(40, 3), (0, 2), (9, 1)], 4, 4, 64, "int8", "bf16", 16, seed=5)
     got = single(step, items=ints([4, -1, 2, 0]), n_items=4)

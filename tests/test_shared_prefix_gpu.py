@@ -32,6 +32,19 @@ def test_groups(form, act, heads, kv, dim):
     check(step, shared(step, groups, lens, window=20), window=20)
 
 
+@pytest.mark.parametrize("form,act", [f for f in FORMS if f[0] != "f32"])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (8, 2, 128), (24, 2, 64), (6, 2, 80)])
+def test_own_keys_dealt_out_as_one_line(form, act, heads, kv, dim):
+    """With room for so many keys in the block table that the tokens' own keys are dealt out run by run: tokens with many of them, with
+    one, inside the prefix with none, and in a group that shares nothing."""
+    requests = [(200, 1), (1500, 1), (208, 1), (300, 1), (201, 1), (33, 1), (60, 1), (45, 1), (10, 1), (0, 1)]
+    groups, lens = [[0, 1, 2, 3, 4], [6, 5], [7], [8, 9]], [200, 33, 46, 0]
+    step = Step(requests, heads, kv, dim, form, act, 16, seed=dim, shared=[([0, 1, 2, 3, 4], 200), ([6, 5], 33)], pad=2, table_wide=5000)
+    check(step, shared(step, groups, lens))
+    check(step, shared(step, groups, lens, window=20), window=20)
+    assert int(step.status) == 0
+
+
 @pytest.mark.parametrize("form,act", FORMS)
 @pytest.mark.parametrize("page_size", [1, 7, 8, 64])
 def test_pages(form, act, page_size):
