@@ -67,8 +67,8 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
             sq[r * ld + e] = token >= 0 && e < d
                 ? to_f32(((const QT*)a.q)[(size_t)token * a.q_stride + (size_t)(pc.head * g + r % g) * d + e]) * a.scale_log2 : 0.f;
         }
-        const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
-        const int* bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
+        const int seq = ar_request(a, pc.t);
+        const int* bt = seq >= 0 ? a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages : nullptr;
         float ref = -INFINITY, sum = 0.f;                           // of row tid / TPR
         float2 acc[RPT][DT][2];
 #pragma unroll
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
             for (int j = tid; j < KEYS; j += AA_THREADS) {
                 const int key = k0 + j;
                 uint32_t row = 0xffffffffu;
-                if (key >= pc.t.key_lo && key < k_end) {
+                if (bt && key >= pc.t.key_lo && key < k_end) {
                     const int page = a.kv.page(bt, key);
                     if (page >= 0) row = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, a.kv.page_index(key));
                     else if (a.kv.status) *a.kv.status = 1;
@@ -262,15 +262,14 @@ template <typename QT>
 __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs a) {
     const RowPlan& p = a.plan;
     const int x = blockIdx.x * p.run, d = a.d, g = p.group;
-    if (x == 0 || x >= p.total) return;
     RowWalk w;
     w.begin(p, blockIdx.x);
     RowPiece pc;
-    if (!w.next(p, pc) || pc.chunk0 == 0) return;                   // the run begins with a unit of its own
-    int c0, c1;
-    ar_walkers(p, pc.t, pc.head, ar_chunks(pc.t), c0, c1);
-    if (c0 != (int)blockIdx.x - 1) return;
-    ST_PDL_WAIT();
+    int c0 = -1, c1 = -1;
+    if (x > 0 && x < p.total && w.next(p, pc) && pc.chunk0 > 0)     // else the run begins with a unit of its own
+        ar_walkers(p, pc.t, pc.head, ar_chunks(pc.t), c0, c1);
+    ST_PDL_WAIT();                                                  // by all blocks: what follows this kernel follows the tiles' too
+    if (c0 < 0 || c0 != (int)blockIdx.x - 1) return;
     const int pieces = (d + 3) / 4, total = pc.t.n_tok * g * pieces;
     for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < total; i += gridDim.y * blockDim.x) {
         const int r = i / pieces, e = (i - r * pieces) * 4, place = pc.t.first + r / g, token = p.items ? p.items[place] : place;
@@ -311,6 +310,8 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
     const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     if (a.info) lo = max(lo, a.info[3 * item]);
+    const int last = min(pos, a.kv.reach - 1);                      // what lies past the table has no page
+    if (last < pos && a.kv.status) *a.kv.status = 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
     float q[8], acc[8];
@@ -321,10 +322,10 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
         acc[i] = 0.f;
     }
     float ref = -INFINITY, sum = 0.f;
-    for (int b = lo + (split * W + warp) * 32; b <= pos; b += a.splits * W * 32) {
+    for (int b = lo + (split * W + warp) * 32; b <= last; b += a.splits * W * 32) {
         uint32_t row = 0xffffffffu;
         float ks = 1.f, vs = 1.f;
-        if (b + lane <= pos) {
+        if (b + lane <= last) {
             const int page = a.kv.page(bt, b + lane);
             if (page >= 0) {
                 row = a.kv.row0(page, 0, key_head) + a.kv.offset(b + lane, a.kv.page_index(b + lane));
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
             }
         }
         float z = -INFINITY;
-        const int n = min(32, pos - b + 1);
+        const int n = min(32, last - b + 1);
 #pragma unroll 4
         for (int j = 0; j < n; ++j) {
             const uint32_t r = __shfl_sync(0xffffffffu, row, j);
@@ -488,7 +489,7 @@ static int ar_check(const RowCall& c) {
 }
 static PagedKV ar_kv(const RowCall& c) {
     return PagedKV{(const unsigned char*)c.pool, c.scales, c.table, c.max_pages, (int)c.num_pages, c.n_layers, c.layer, c.nkv, c.page_size,
-                   c8_shift(c.page_size), c.status};
+                   c8_shift(c.page_size), c8_reach(c.max_pages, c.page_size), c.status};
 }
 static SingleArgs ar_single_args(const RowCall& c) {
     SingleArgs a{};

@@ -62,6 +62,18 @@ __device__ __forceinline__ int ar_chunks(const RowTile& t) {
 }
 __device__ __forceinline__ int ar_places(int chunks) { return chunks > 0 ? chunks + AR_UNIT : 0; }      // of a unit in the line
 
+// The request whose block table a tile's keys are found by: that of its tokens, or of its first item that is not padding (whose request
+// may be any number); -1: all are padding, no key is read.
+__device__ __forceinline__ int ar_request(const RowArgs& a, const RowTile& t) {
+    if (t.seq >= 0) return t.seq;
+    for (int i = 0; i < t.n_tok; ++i) {
+        const int token = __ldg(a.plan.items + t.first + i);
+        const int pos = __ldg(a.positions + token);
+        if (pos >= 0) return __ldg(a.seq_of_token + token);
+    }
+    return -1;
+}
+
 // A walker's way along its run: pieces of one (tile, key head) pair.  A walker behind the line's end has none.
 struct RowPiece {
     RowTile t;

@@ -225,14 +225,14 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             if (i >= keys.n) {
                 if (!walk.next(a.plan, pc)) { have = false; return; }
                 keys = rt_keys(pc);
-                const int seq = pc.t.seq >= 0 ? pc.t.seq : a.seq_of_token[a.plan.items[pc.t.first]];
-                bt = a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages;
+                const int seq = ar_request(a, pc.t);
+                bt = seq >= 0 ? a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages : nullptr;
                 head = pc.head;
                 i = 0;
             }
             const int key = keys.k0 + TC_BN * i + row;
             ++i;
-            if (key >= pc.t.key_lo && key < keys.k_end) {
+            if (bt && key >= pc.t.key_lo && key < keys.k_end) {
                 const int index = a.kv.page_index(key);
                 wanted = true;
                 off = a.kv.offset(key, index);

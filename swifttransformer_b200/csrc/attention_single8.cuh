@@ -210,12 +210,14 @@ template <bool LINE> struct SingleLine {
 template <int KT> __device__ __forceinline__ int sg_runs(const SingleArgs& a, int item, int pos) {     // of a token's own keys
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     if (a.info) lo = max(lo, a.info[3 * item]);
-    return pos >= lo ? (pos + 1 - (lo & ~7) + KT - 1) / KT : 0;
+    const int hi = min(pos, a.kv.reach - 1) + 1;                 // what lies past the table has no page
+    return hi > lo ? (hi - (lo & ~7) + KT - 1) / KT : 0;
 }
 template <int KT> __device__ __forceinline__ void sg_line_begin(const SingleArgs& a, SingleLine<true>& s) {
     for (int i = threadIdx.x; i < a.n_items; i += blockDim.x) {
         const int token = a.items ? a.items[i] : i, pos = token >= 0 ? a.positions[token] : -1;
         s.before[i + 1] = sg_runs<KT>(a, i, pos);
+        if (pos >= a.kv.reach && a.kv.status) *a.kv.status = 1;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -257,15 +259,15 @@ __global__ void __launch_bounds__(SG_JOIN) attention_single8_join_kernel(const S
     __shared__ float4 s_o[SG_JOIN];
     const int unit = blockIdx.x, part = unit / a.n_items, item = unit - part * a.n_items, d = a.d, r = blockIdx.y;
     const int key_head = part / a.row_blocks, head = key_head * a.group + (part % a.row_blocks) * R + r;
-    if (head >= (key_head + 1) * a.group) return;
+    if (head >= (key_head + 1) * a.group) return;                // (row 0 of the unit is there and waits)
     const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
-    if (pos < 0) return;
     const SharedParts shared = sg_shared_parts(a, item, key_head);
     const size_t shared_row = shared.row + (head - key_head * a.group);
-    const bool own = sg_runs<KT>(a, item, pos) > 0;
-    ST_PDL_WAIT();
+    const bool own = pos >= 0 && sg_runs<KT>(a, item, pos) > 0;
+    ST_PDL_WAIT();                                               // by all, so that what follows this kernel follows the one before it too
+    if (pos < 0) return;
     const int c0 = own ? __ldcg(a.span + 2 * unit) : 0, c1 = own ? __ldcg(a.span + 2 * unit + 1) : -1;
-    if (!a.info && c0 == c1) return;                             // one walker had it all and has stored it
+    if (!a.info && own && c0 == c1) return;                             // one walker had it all and has stored it
     const int lanes = d / 4, groups = blockDim.x / lanes, mine = threadIdx.x / lanes, e = threadIdx.x % lanes * 4;
     const int n_own = c1 - c0 + 1, n = n_own + shared.n;
     float m = -INFINITY;
@@ -364,7 +366,8 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
     const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     if (a.info) lo = max(lo, a.info[3 * item]);
-    const int hi = pos + 1;
+    const int hi = min(pos, a.kv.reach - 1) + 1;
+    if (!LINE && pos >= a.kv.reach && a.kv.status) *a.kv.status = 1;
     const int i0 = i;
     // offset of this lane's word w in a key row: pieces of 16 bytes per lane while the row lasts, then 8, then 4
     auto key_byte = [&](int w) -> int {
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
         if (w < full + two) return full * 16 + t * 8 + (w - full) * 4;
         return (full + two) * 16 + t * 4;
     };
-    const int base0 = lo & ~7, runs = min(i_end, hi > base0 ? (hi - base0 + KT - 1) / KT : 0);
+    const int base0 = lo & ~7, runs = min(i_end, hi > lo ? (hi - base0 + KT - 1) / KT : 0);
     // A run's keys are four aligned blocks of NK, each within a page.  Lane (g, t) looks up block t, two runs ahead (ask), and
     // turns the page into a row of the pool one run ahead (resolve); its rows' keys are in block g / 2, whose row lane g / 2 has.
     constexpr uint32_t NONE = 0xffffffffu;

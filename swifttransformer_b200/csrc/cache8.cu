@@ -282,7 +282,7 @@ static int c8_check(const Cache8Call& c) {
 }
 static PagedKV c8_kv(const Cache8Call& c) {
     return PagedKV{(const unsigned char*)c.pool, c.scales, c.block_table, c.max_pages, c.num_pages, c.n_layers, c.layer, c.nkv, c.page_size,
-                   c8_shift(c.page_size), c.status};
+                   c8_shift(c.page_size), c8_reach(c.max_pages, c.page_size), c.status};
 }
 ST_EXPORT int st_qkv_to_cache8(const Cache8Call* c, void* stream) {
     if (c->n_tokens <= 0) return 0;
@@ -350,6 +350,7 @@ static int c8_launch_rows(const PagedKV& kv, void* out, const int* positions, co
     const int total = 2 * kv.nkv * d / (vec ? 8 : 1);
     int y = (total + C8_THREADS - 1) / C8_THREADS;
     if (n >= 2 * st_sm_count() && y > 1) y = (y + 3) / 4;      // four turns a thread where the tokens alone fill the device
+    if (y > 65535) y = 65535;
     if (vec) cache8_rows_kernel<T, FORM, 8><<<dim3(n, y), C8_THREADS, 0, s>>>(kv, (T*)out, positions, seq_of_token, slots, d);
     else cache8_rows_kernel<T, FORM, 1><<<dim3(n, y), C8_THREADS, 0, s>>>(kv, (T*)out, positions, seq_of_token, slots, d);
     return st_launch_status();

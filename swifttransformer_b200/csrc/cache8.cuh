@@ -28,6 +28,7 @@ struct PagedKV {
     const float* scales;                 // null for 16- and 32-bit caches
     const int* table;                    // [slots][max_pages]
     int max_pages, num_pages, n_layers, layer, nkv, page_size, page_shift;   // page_shift: log2 of page_size, or -1
+    int reach;                           // positions that the table has room for
     int* status;                         // set to 1 where a needed key has no page
 
     __device__ __forceinline__ int page_index(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
@@ -49,6 +50,11 @@ static inline int c8_shift(int page_size) {
     for (int s = 0; s < 30; ++s)
         if ((1 << s) == page_size) return s;
     return -1;
+}
+// a little below 2^31 at most: sums of a position and a run's keys stay in an int
+static inline int c8_reach(int max_pages, int page_size) {
+    const long long n = (long long)max_pages * page_size;
+    return n < 0x7fff0000ll ? (int)n : 0x7fff0000;
 }
 // rows of a pool fit 32-bit unsigned indices
 static inline bool c8_rows_fit(long long num_pages, int n_layers, int nkv, int page_size) {

@@ -176,7 +176,7 @@ class RowPlan:
             rows.append((first, n, seq, lo, hi, start))
             chunks = self._chunks(lo, hi)
             start += (chunks + ROWS_UNIT) * self.nkv if chunks else 0
-        _need(start < 1 << 31 and len(rows) * self.nkv < 1 << 22, "a plan of more keys than one call serves")
+        _need(start < 1 << 30 and len(rows) * self.nkv < 1 << 22, "a plan of more keys than one call serves")
         self.total, self.n_tiles = start, len(rows)
         self.max_rows = max((r[1] for r in rows), default=0) * (self.nh // self.nkv)
         flat = np.asarray(rows, dtype=np.int32).reshape(-1)
@@ -267,8 +267,9 @@ def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_tok
     else:
         stride = 0
     st = status if status is not None else _tc_status_word(q.device)
-    reach = block_table.shape[1] * page_size             # a hint of more keys than the table has room for is none
+    reach = min(block_table.shape[1] * page_size, 1 << 30)       # a hint of more keys than the table has room for is none
     max_keys = min(max_keys, reach) if max_keys > 0 else reach
+    window = min(window, 0x7fffffff)
     if 0 < window < max_keys:
         max_keys = window
     # parts of rows that several blocks leave: a slot per (tile, key head) and one per walker of the line; those of single tokens
@@ -318,8 +319,8 @@ def attention_shared_prefix(q: torch.Tensor, pool: torch.Tensor, layer: int, out
                             nh: int, scale: float, window: int = 0, scales: Optional[torch.Tensor] = None,
                             status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of single query tokens whose requests share their first keys: the result of ``attention_decode`` for every token of
-    ``plan`` (from ``shared_prefix_plan``), with a group's shared keys and values read once for the group, through the block table of its
-    first token's request.  The cache is of q's type, or an 8-bit one with its ``scales``.
+    ``plan`` (from ``shared_prefix_plan``), with a group's shared keys and values read once for the group, through the block table of the
+    request of its first token that is not padding.  The cache is of q's type, or an 8-bit one with its ``scales``.
 
     A token's position may lie anywhere, inside the shared keys too: it sees keys 0 .. its own position (``window`` > 0: the last
     ``window`` of these).  A value that is not finite reaches, in bfloat16 caches, all rows of its group that share it, also those

@@ -38,14 +38,14 @@ class Step:
     (requests, keys in common): the members' first keys are the first member's."""
 
     def __init__(self, requests, heads, kv, dim, form, act, page_size=16, seed=0, shared=(), pad=0, layers=2, layer=1, q_std=1.5,
-                 k_std=0.6, v_std=1.0, table_wide=0):
+                 k_std=0.6, v_std=1.0, table_wide=0, spare=2):
         gen = torch.Generator(device="cuda").manual_seed(seed)
         rng = random.Random(seed)
         self.heads, self.kv, self.dim, self.form, self.act, self.layer, self.page_size = heads, kv, dim, form, act, layer, page_size
         self.requests, self.scale = requests, 1.0 / math.sqrt(dim)
         ends = [b + n for b, n in requests]
         need = [-(-e // page_size) for e in ends]
-        order = list(range(sum(need) + 2))
+        order = list(range(sum(need) + spare))
         rng.shuffle(order)
         n_slots = len(requests) + 1
         slots = rng.sample(range(n_slots), len(requests))

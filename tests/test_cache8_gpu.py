@@ -206,6 +206,47 @@ def test_more_tokens_than_a_line_takes():
     check(step, single(step))
 
 
+@pytest.mark.parametrize("form,act,dim", [("int8", "bf16", 64), ("e4m3", "f32", 128), ("int8", "f32", 24)])
+@pytest.mark.parametrize("table_wide", [0, 5000])
+@pytest.mark.parametrize("far", [3, 2 ** 31 - 1])
+def test_positions_past_the_block_table(form, act, dim, table_wide, far):
+    """A token that stands behind all keys the table has room for sees those that are there; one whose window lies behind them sees none."""
+    step = Step([(31, 1), (47, 1), (20, 1)], 4, 2, dim, form, act, 16, seed=dim, table_wide=table_wide)
+    reach = step.table.shape[1] * 16
+    step.positions[1] = reach + far if far < 1000 else far
+    check(step, single(step))
+    assert int(step.status) == 1
+    got = single(step, window=3)
+    check(step, got, window=3, rows=[0, 2])
+    assert float(got[1].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("table_wide", [0, 5000])
+def test_the_same_token_twice_and_padding_alone(table_wide):
+    step = Step([(40, 1), (700, 1), (9, 1)], 4, 2, 64, "int8", "bf16", 16, seed=8, pad=2, table_wide=table_wide)
+    check(step, single(step, items=ints([1, 0, 1, 1, 2, 0]), n_items=6), rows=[0, 1, 2])
+    assert float(single(step, items=ints([3, 4, -1]), n_items=3).min()) == 77.0
+
+
+@pytest.mark.parametrize("form,act", [("int8", "bf16"), ("e4m3", "f32")])
+def test_a_pool_of_more_than_four_gigabytes(form, act):
+    """Pages all over it, for single tokens, for portions, for the write and for rows read back."""
+    step = Step([(500, 40), (100, 1), (290, 7)], 8, 8, 128, form, act, 64, seed=9, spare=20000)
+    assert step.pool.numel() > 2 ** 32
+    check(step, single(step))
+    check(step, portion(step))
+    from swifttransformer_b200 import ops
+    rows = torch.empty((step.n, 2 * 8 * 128), dtype=TYPES[act], device="cuda")
+    ops.cache8_rows(step.pool, step.scales, step.layer, rows, step.positions, step.seq, step.slots, step.table, step.status)
+    qkv = torch.cat([step.q, rows], dim=1)
+    before, scales = rows.clone(), step.scales.nan_to_num()
+    ops.qkv_to_cache8(qkv, None, None, step.pool, step.scales, step.layer, step.positions, step.seq, step.slots, step.table, 8, 8, 128, step.status)
+    ops.cache8_rows(step.pool, step.scales, step.layer, rows, step.positions, step.seq, step.slots, step.table, step.status)
+    assert torch.allclose(rows.float(), before.float(), rtol=2.0 ** -3, atol=2.0 ** -6 * float(before.abs().max()))
+    changed = (step.scales.nan_to_num() != scales).sum()
+    assert int(changed) <= step.n * 2 * 8 and int(step.status) == 0
+
+
 def test_listed_tokens_only():
     step = Step([(40, 3), (0, 2), (9, 1)], 4, 4, 64, "int8", "bf16", 16, seed=5)
     got = single(step, items=ints([4, -1, 2, 0]), n_items=4)

@@ -73,6 +73,28 @@ def test_positions_inside_the_prefix(form, act, dim):
     check(step, shared(step, [[2, 0, 1, 3, 4, 5, 6, 7]], [128]))
 
 
+@pytest.mark.parametrize("form,act", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 40])
+@pytest.mark.parametrize("gone", [[0], [0, 1, 3], [0, 1, 2, 3]])
+def test_members_that_have_left(form, act, dim, gone):
+    """Members that are padding now, the first of the group among them: their requests and slots may be anything."""
+    step = Step([(70, 1), (75, 1), (64, 1), (90, 1), (20, 1)], 4, 2, dim, form, act, 16, seed=1, shared=[([0, 1, 2, 3], 64)])
+    step.positions[gone] = -1
+    step.seq[gone] = -1000000000
+    got = shared(step, [[0, 1, 2, 3], [4]], [64, 0])
+    left = [t for t in range(5) if t not in gone]
+    check(step, got, rows=left)
+    assert float(got[gone].min()) == 77.0 and float(got[gone].max()) == 77.0
+    assert int(step.status) == 0
+
+
+@pytest.mark.parametrize("form,act", [("bf16", "bf16"), ("f32", "f32"), ("e4m3", "bf16")])
+def test_a_pool_of_more_than_four_gigabytes(form, act):
+    step = Step([(500, 1), (530, 1), (690, 1)], 8, 8, 128, form, act, 64, seed=9, shared=[([0, 1, 2], 490)], spare=20000)
+    assert step.pool.numel() > 2 ** 32
+    check(step, shared(step, [[0, 1, 2]], [490]))
+
+
 def test_tokens_without_a_group_stay():
     step = Step([(40, 1), (41, 1), (42, 1)], 2, 2, 64, "bf16", "bf16", 16, shared=[([0, 2], 32)])
     got = shared(step, [[0, 2]], [32])
