@@ -29,6 +29,21 @@ template <int ROWS> static size_t aa_smem(int d) {
     return (size_t)(ROWS * aa_stride(d) + 2 * AnyShape<ROWS>::KEYS * aa_stride(d) + ROWS * (AnyShape<ROWS>::KEYS + 4)) * 4;
 }
 
+// four neighbouring elements of a cache row as they lie in memory, and as floats
+template <int FORM> struct AnyRaw {
+    using type = uint32_t;
+    static __device__ __forceinline__ float4 floats(uint32_t w) {
+        uint32_t h[2];
+        c8_halves<FORM == C8_E4M3 ? C8_E4M3 : C8_INT8>(w, h[0], h[1]);
+        const float2 x = sg_unpack<true>(h[0]), y = sg_unpack<true>(h[1]);
+        return make_float4(x.x, x.y, y.x, y.y);
+    }
+};
+template <> struct AnyRaw<C8_F32> {
+    using type = float4;
+    static __device__ __forceinline__ float4 floats(float4 v) { return v; }
+};
+
 template <int FORM, typename QT, int ROWS, int DP>
 __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const RowArgs a) {
     using S = AnyShape<ROWS>;
@@ -48,6 +63,8 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
     constexpr int LP = KEYS + 4;
     const int tid = threadIdx.x, rg = tid / KG, kg = tid % KG, g = a.plan.group;
     const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
+    // four elements of a query row at once
+    const bool wide = d % 4 == 0 && a.q_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
     ST_PDL_TRIGGER();
     RowWalk walk;
     walk.begin(a.plan, blockIdx.x);
@@ -61,11 +78,24 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
             s_pos[r] = token >= 0 ? a.positions[token] : -1;
         }
         __syncthreads();
-        for (int i = tid; i < ROWS * nv * 4; i += AA_THREADS) {
-            const int r = i / (nv * 4), e = i - r * nv * 4;
+#pragma unroll 4
+        for (int i = tid; i < ROWS * nv; i += AA_THREADS) {
+            const int r = i / nv, e = (i - r * nv) * 4;
             const int token = s_token[r];
-            sq[r * ld + e] = token >= 0 && e < d
-                ? to_f32(((const QT*)a.q)[(size_t)token * a.q_stride + (size_t)(pc.head * g + r % g) * d + e]) * a.scale_log2 : 0.f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (token >= 0) {
+                const QT* q = (const QT*)a.q + (size_t)token * a.q_stride + (size_t)(pc.head * g + r % g) * d + e;
+                if (wide) {
+                    x = load4(q);
+                } else {
+                    x.x = to_f32(q[0]);
+                    if (e + 1 < d) x.y = to_f32(q[1]);
+                    if (e + 2 < d) x.z = to_f32(q[2]);
+                    if (e + 3 < d) x.w = to_f32(q[3]);
+                }
+                x.x *= a.scale_log2; x.y *= a.scale_log2; x.z *= a.scale_log2; x.w *= a.scale_log2;
+            }
+            store4(sq + r * ld + e, x);
         }
         const int seq = ar_request(a, pc.t);
         const int* bt = seq >= 0 ? a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages : nullptr;
@@ -77,57 +107,84 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
             for (int c = 0; c < DT; ++c) acc[i][c][0] = acc[i][c][1] = make_float2(0.f, 0.f);
         const int k_begin = (pc.t.key_lo & ~(AR_CHUNK - 1)) + pc.chunk0 * AR_CHUNK;
         const int k_end = min(k_begin + pc.chunks * AR_CHUNK, pc.t.key_hi);
+        // key k0 + tid (tid < KEYS): its page, looked up while the run before is worked on, then its row and scales
+        int page = -1;
+        bool wanted = false;
+        auto ask = [&](int k0) {
+            const int key = k0 + tid, index = a.kv.page_index(key);
+            wanted = tid < KEYS && bt && key >= pc.t.key_lo && key < k_end;
+            page = wanted && index < a.kv.max_pages ? __ldg(bt + index) : -1;
+        };
+        uint32_t row_of = 0xffffffffu;
+        float ks_of = 1.f, vs_of = 1.f;
+        auto resolve = [&](int k0) {
+            const int key = k0 + tid;
+            row_of = 0xffffffffu;
+            ks_of = vs_of = 1.f;
+            if (!wanted) return;
+            if ((unsigned)page >= (unsigned)a.kv.num_pages) {
+                if (a.kv.status) *a.kv.status = 1;
+                return;
+            }
+            row_of = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, a.kv.page_index(key));
+            if (FORM < C8_BF16) { ks_of = __ldg(a.kv.scales + row_of); vs_of = __ldg(a.kv.scales + row_of + to_values); }
+        };
+        ask(k_begin);
+        resolve(k_begin);
         for (int k0 = k_begin; k0 < k_end; k0 += KEYS) {
             __syncthreads();
             if (tid == 0) s_odd = 0;
-            for (int j = tid; j < KEYS; j += AA_THREADS) {
-                const int key = k0 + j;
-                uint32_t row = 0xffffffffu;
-                if (bt && key >= pc.t.key_lo && key < k_end) {
-                    const int page = a.kv.page(bt, key);
-                    if (page >= 0) row = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, a.kv.page_index(key));
-                    else if (a.kv.status) *a.kv.status = 1;
-                }
-                s_row[j] = row;
-                s_ks[j] = FORM < C8_BF16 && row != 0xffffffffu ? a.kv.scales[row] : 1.f;
-                s_vs[j] = FORM < C8_BF16 && row != 0xffffffffu ? a.kv.scales[row + to_values] : 1.f;
-            }
+            if (tid < KEYS) { s_row[tid] = row_of; s_ks[tid] = ks_of; s_vs[tid] = vs_of; }
             __syncthreads();
-            // rows as floats; what lies past d or has no key is zero
+            ask(k0 + KEYS);
+            // rows as floats; what lies past d or has no key is zero.  Two pieces' loads are under way together.
             bool odd = false;
-            for (int i = tid; i < KEYS * nv; i += AA_THREADS) {
-                const int j = i / nv, e = (i - j * nv) * 4;
-                const uint32_t row = s_row[j];
-                float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (row != 0xffffffffu) {
-                    const size_t at = (size_t)row * d + e, vt = (size_t)(row + to_values) * d + e;
-                    if (d % 4 == 0 && FORM == C8_F32) {
-                        const float4 x = *reinterpret_cast<const float4*>(a.kv.pool + at * 4), y = *reinterpret_cast<const float4*>(a.kv.pool + vt * 4);
-                        k[0] = x.x; k[1] = x.y; k[2] = x.z; k[3] = x.w;
-                        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
-                    } else if (d % 4 == 0 && FORM < C8_BF16) {
-                        uint32_t h[4];
-                        c8_halves<FORM>(*reinterpret_cast<const uint32_t*>(a.kv.pool + at), h[0], h[1]);
-                        c8_halves<FORM>(*reinterpret_cast<const uint32_t*>(a.kv.pool + vt), h[2], h[3]);
-                        const float2 x = sg_unpack<true>(h[0]), y = sg_unpack<true>(h[1]), z = sg_unpack<true>(h[2]), w = sg_unpack<true>(h[3]);
-                        k[0] = x.x; k[1] = x.y; k[2] = y.x; k[3] = y.y;
-                        v[0] = z.x; v[1] = z.y; v[2] = w.x; v[3] = w.y;
-                    } else {
+            if (FORM != C8_BF16 && d % 4 == 0) {
+                using Raw = typename AnyRaw<FORM>::type;
+                const Raw* keys = reinterpret_cast<const Raw*>(a.kv.pool);
+                for (int i0 = tid; i0 < KEYS * nv; i0 += 2 * AA_THREADS) {
+                    Raw k[2], v[2];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (e + c < d) { k[c] = c8_value<FORM>(a.kv.pool, at + c); v[c] = c8_value<FORM>(a.kv.pool, vt + c); }
+                    for (int c = 0; c < 2; ++c) {
+                        const int i = i0 + c * AA_THREADS, j = i / nv;
+                        const uint32_t row = i < KEYS * nv ? s_row[j] : 0xffffffffu;
+                        k[c] = v[c] = Raw{};
+                        if (row != 0xffffffffu) {
+                            k[c] = __ldg(keys + (size_t)row * nv + (i - j * nv));
+                            v[c] = __ldg(keys + (size_t)(row + to_values) * nv + (i - j * nv));
+                        }
                     }
-                    if (FORM < C8_BF16) {
-                        const float s = s_vs[j];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) v[c] *= s;
+                    for (int c = 0; c < 2; ++c) {
+                        const int i = i0 + c * AA_THREADS, j = i / nv;
+                        if (i >= KEYS * nv) continue;
+                        const float4 x = AnyRaw<FORM>::floats(k[c]);
+                        float4 y = AnyRaw<FORM>::floats(v[c]);
+                        if (FORM < C8_BF16) {
+                            const float s = s_vs[j];
+                            y.x *= s; y.y *= s; y.z *= s; y.w *= s;
+                        }
+                        odd |= !(isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w));
+                        store4(sk + j * ld + (i - j * nv) * 4, x);
+                        store4(sv + j * ld + (i - j * nv) * 4, y);
                     }
-                    odd |= !(isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3]));
                 }
-                store4(sk + j * ld + e, make_float4(k[0], k[1], k[2], k[3]));
-                store4(sv + j * ld + e, make_float4(v[0], v[1], v[2], v[3]));
+            } else {
+                for (int i = tid; i < KEYS * nv * 4; i += AA_THREADS) {
+                    const int j = i / (nv * 4), e = i - j * nv * 4;
+                    const uint32_t row = e < d ? s_row[j] : 0xffffffffu;
+                    float k = 0.f, v = 0.f;
+                    if (row != 0xffffffffu) {
+                        k = c8_value<FORM>(a.kv.pool, (size_t)row * d + e);
+                        v = c8_value<FORM>(a.kv.pool, (size_t)(row + to_values) * d + e) * s_vs[j];
+                    }
+                    odd |= !isfinite(v);
+                    sk[j * ld + e] = k;
+                    sv[j * ld + e] = v;
+                }
             }
             if (odd) s_odd = 1;
+            resolve(k0 + KEYS);
             __syncthreads();
             // ---- scores
             if (rg < rows) {
@@ -201,6 +258,7 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
                         for (int h = 0; h < 2; ++h) { acc[i][c][h].x *= corr; acc[i][c][h].y *= corr; }
                 }
                 const int n_keys = min(KEYS, k_end - k0);
+#pragma unroll 4
                 for (int j = 0; j < n_keys; ++j) {
                     float p[RPT];
 #pragma unroll
@@ -242,6 +300,10 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
                 for (int c = 0; c < DT; ++c) {
                     const int e = 4 * (kg + KG * c);
                     const float o[4] = {acc[i][c][0].x, acc[i][c][0].y, acc[i][c][1].x, acc[i][c][1].y};
+                    if (d % 4 == 0 && !direct) {
+                        if (e < d) store4(a.parts.o + (slot + r) * d + e, make_float4(o[0], o[1], o[2], o[3]));
+                        continue;
+                    }
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         if (e + h >= d) continue;
@@ -270,30 +332,51 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs 
         ar_walkers(p, pc.t, pc.head, ar_chunks(pc.t), c0, c1);
     ST_PDL_WAIT();                                                  // by all blocks: what follows this kernel follows the tiles' too
     if (c0 < 0 || c0 != (int)blockIdx.x - 1) return;
-    const int pieces = (d + 3) / 4, total = pc.t.n_tok * g * pieces;
+    const int pieces = (d + 3) / 4, total = pc.t.n_tok * g * pieces, n = c1 - c0 + 1;
+    const bool vec = d % 4 == 0, wide = vec && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    const size_t row0 = (size_t)(pc.unit + c0) * AR_ROWS;
     for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < total; i += gridDim.y * blockDim.x) {
         const int r = i / pieces, e = (i - r * pieces) * 4, place = pc.t.first + r / g, token = p.items ? p.items[place] : place;
-        if (a.positions[token] < 0) continue;
+        const int pos = a.positions[token];
+        // two parts at a time, all of their numbers under way together; what was summed before moves to the largest reference so far
         float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(a.parts.r + (size_t)(pc.unit + c) * AR_ROWS + r));
-        for (int c = c0; c <= c1; ++c) {
-            const size_t at = (size_t)(pc.unit + c) * AR_ROWS + r;
-            const float f = ar_weight(__ldcg(a.parts.r + at), m);
-            const float* part = a.parts.o + at * d + e;
-            l += f * __ldcg(a.parts.l + at);
-            if (d % 4 == 0) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(part));
-                o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
-            } else {
+        for (int k = 0; k < n; k += 2) {
+            float ref[2], sum[2], x[2][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (e + k < d) o[k] += f * __ldcg(part + k);
+            for (int h = 0; h < 2; ++h) {
+                const size_t at = row0 + (size_t)(k + (k + h < n ? h : 0)) * AR_ROWS + r;
+                const float* part = a.parts.o + at * d + e;
+                ref[h] = __ldcg(a.parts.r + at);
+                sum[h] = __ldcg(a.parts.l + at);
+                if (vec) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(part));
+                    x[h][0] = v.x; x[h][1] = v.y; x[h][2] = v.z; x[h][3] = v.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[h][j] = e + j < d ? __ldcg(part + j) : 0.f;
+                }
             }
-        }
-        QT* out = (QT*)a.out + ((size_t)token * p.nh + pc.head * g + r % g) * d + e;
+            if (k + 1 >= n) {                                       // there is no second one: the first was read again
+                ref[1] = -INFINITY;
+                sum[1] = x[1][0] = x[1][1] = x[1][2] = x[1][3] = 0.f;
+            }
+            const float most = fmaxf(m, fmaxf(ref[0], ref[1]));
+            const float f = ar_weight(m, most), f0 = ar_weight(ref[0], most), f1 = ar_weight(ref[1], most);
+            m = most;
+            l = l * f + (f0 * sum[0] + f1 * sum[1]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (e + k < d) out[k] = from_f32<QT>(l == 0.f ? 0.f : o[k] / l);
+            for (int j = 0; j < 4; ++j) o[j] = o[j] * f + (f0 * x[0][j] + f1 * x[1][j]);
+        }
+        if (pos < 0) continue;
+        QT* out = (QT*)a.out + ((size_t)token * p.nh + pc.head * g + r % g) * d + e;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (wide) {
+            store4(out, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (e + j < d) out[j] = from_f32<QT>(o[j] * inv);
+        }
     }
 }
 
