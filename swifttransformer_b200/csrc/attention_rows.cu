@@ -6,8 +6,8 @@
 // head's dimensions, the rows' softmax by 256 / ROWS threads each, weights times values by 4 (2) rows x dimensions per thread; both
 // products two multiply-adds to an instruction.  Bound by these and by the shared memory's reads (two of 16 bytes per eight
 // of them for the scores).  ROWS 16 for tiles of at most 16 rows: with 128 only one thread in eight would have work.
-// attention_single_any_kernel: a warp per key in turn, lanes along the head's dimensions; for single tokens where the kernel of
-// attention_single8.cuh has no instance.  Both visit or use no row that a query does not see: numbers that are not finite
+// attention_single_any_kernel: 32 keys to a warp, a lane per key for the scores, lanes along the head's dimensions for the values; for
+// single tokens where the kernel of attention_single8.cuh has no instance.  Both visit or use no row that a query does not see: numbers that are not finite
 // stay where they are.
 #include "attention_single8.cuh"
 
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs 
 // ---- single tokens, anything ----------------------------------------------------------------------------------------
 template <int FORM, typename QT>
 __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleArgs a) {
-    extern __shared__ float smem[];
+    extern __shared__ __align__(16) float smem[];
     const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, head = blockIdx.y, key_head = head / a.group, d = a.d;
     const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
     if (pos < 0) {
@@ -397,13 +397,14 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
     if (last < pos && a.kv.status) *a.kv.status = 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;
-    float q[8], acc[8];
+    float* sq = smem;                                              // the query row, scaled, then zeros up to a multiple of four
+    float* parts = smem + ((d + 3) & ~3);
+    for (int e = threadIdx.x; e < ((d + 3) & ~3); e += blockDim.x)
+        sq[e] = e < d ? to_f32(((const QT*)a.q)[((size_t)token * a.nh + head) * d + e]) * a.scale_log2 : 0.f;
+    __syncthreads();
+    float acc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int e = lane + 32 * i;
-        q[i] = e < d ? to_f32(((const QT*)a.q)[((size_t)token * a.nh + head) * d + e]) * a.scale_log2 : 0.f;
-        acc[i] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     float ref = -INFINITY, sum = 0.f;
     for (int b = lo + (split * W + warp) * 32; b <= last; b += a.splits * W * 32) {
         uint32_t row = 0xffffffffu;
@@ -412,24 +413,29 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
             const int page = a.kv.page(bt, b + lane);
             if (page >= 0) {
                 row = a.kv.row0(page, 0, key_head) + a.kv.offset(b + lane, a.kv.page_index(b + lane));
-                if (FORM < C8_BF16) { ks = a.kv.scales[row]; vs = a.kv.scales[row + to_values]; }
+                if (FORM < C8_BF16) { ks = __ldg(a.kv.scales + row); vs = __ldg(a.kv.scales + row + to_values); }
             } else if (a.kv.status) {
                 *a.kv.status = 1;
             }
         }
+        // a lane has a key of its own for the scores, dimensions lane, lane + 32, ... for the values
         float z = -INFINITY;
         const int n = min(32, last - b + 1);
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) {
-            const uint32_t r = __shfl_sync(0xffffffffu, row, j);
+        if (row != 0xffffffffu) {
             float dot = 0.f;
-            if (r != 0xffffffffu) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (lane + 32 * i < d) dot += q[i] * c8_value<FORM>(a.kv.pool, (size_t)r * d + lane + 32 * i);
+            if (FORM != C8_BF16 && d % 4 == 0) {
+                using Raw = typename AnyRaw<FORM>::type;
+                const Raw* key = reinterpret_cast<const Raw*>(a.kv.pool) + (size_t)row * (d / 4);
+#pragma unroll 8
+                for (int e = 0; e < d / 4; ++e) {
+                    const float4 x = AnyRaw<FORM>::floats(__ldg(key + e)), y = load4(sq + 4 * e);
+                    dot += (x.x * y.x + x.y * y.y) + (x.z * y.z + x.w * y.w);
+                }
+            } else {
+#pragma unroll 4
+                for (int e = 0; e < d; ++e) dot += sq[e] * c8_value<FORM>(a.kv.pool, (size_t)row * d + e);
             }
-            dot = warp_sum(dot);
-            if (lane == j && r != 0xffffffffu) z = dot * ks;
+            z = dot * ks;
         }
         const float mx = warp_max(z), m = fmaxf(ref, mx), use = m == -INFINITY ? 0.f : m;
         const float corr = ref == -INFINITY ? 0.f : exp2f(ref - m), p = exp2f(z - use);
@@ -438,7 +444,7 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] *= corr;
         const float w = p * vs;
-#pragma unroll 4
+#pragma unroll 8
         for (int j = 0; j < n; ++j) {
             const uint32_t r = __shfl_sync(0xffffffffu, row, j);
             const float wj = __shfl_sync(0xffffffffu, w, j);
@@ -450,11 +456,11 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
         }
     }
     sum = warp_sum(sum);
-    if (lane == 0) { smem[warp] = ref; smem[W + warp] = sum; }
+    if (lane == 0) { parts[warp] = ref; parts[W + warp] = sum; }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < d) smem[2 * W + warp * d + lane + 32 * i] = acc[i];
-    sg_finish<QT>(a, smem, W, 1, 1, d, token, item, head, key_head);
+        if (lane + 32 * i < d) parts[2 * W + warp * d + lane + 32 * i] = acc[i];
+    sg_finish<QT>(a, parts, W, 1, 1, d, token, item, head, key_head);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -479,7 +485,7 @@ template <int FORM, typename QT> static int aa_single(SingleArgs a, int max_keys
     a.row_blocks = 1;
     const int warps = shape.warps < 4 ? shape.warps : 4;
     return sg_launch("single_any", attention_single_any_kernel<FORM, QT>, a, dim3((unsigned)a.n_items * a.splits, a.nh), warps,
-                     (size_t)warps * (a.d + 2) * 4, s);
+                     ((size_t)warps * (a.d + 2) + ((a.d + 3) & ~3)) * 4, s);
 }
 
 template <int FORM, typename QT, int ROWS> static int aa_rows(const RowArgs& a, cudaStream_t s) {

@@ -127,14 +127,14 @@ __device__ __forceinline__ void sg_finish(const SingleArgs& a, float* smem, int 
         const size_t row = shared.row + (head0 - key_head * a.group) + r;
         float m = -INFINITY, l = 0.f, o = 0.f;
         for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.splits > 1 ? sg_remote(ref + r, s) : ref[r]);
-#pragma unroll 4
+#pragma unroll 8
         for (int p = 0; p < shared.n; ++p) m = fmaxf(m, __ldcg(a.parts.r + row + (size_t)p * AR_ROWS));
         for (int s = 0; s < a.splits; ++s) {
             const float w = ar_weight(a.splits > 1 ? sg_remote(ref + r, s) : ref[r], m);
             l += w * (a.splits > 1 ? sg_remote(sum + r, s) : sum[r]);
             o += w * (a.splits > 1 ? sg_remote(acc + i, s) : acc[i]);
         }
-#pragma unroll 4
+#pragma unroll 8
         for (int p = 0; p < shared.n; ++p) {
             const size_t at = row + (size_t)p * AR_ROWS;
             const float w = ar_weight(__ldcg(a.parts.r + at), m);
