@@ -1,5 +1,6 @@
-// Attention of single query tokens over paged caches in 8 and 16 bits (and, in 16 bits, of the keys behind a shared prefix): one
-// block per (token, key head, up to eight of its query heads, share of the keys).
+// Attention of single query tokens over paged caches in 8 and 16 bits, of all keys or of those behind a shared prefix.  A unit is a
+// (token, key head, up to eight of its query heads).  Few keys: a block or a cluster of blocks per unit, whose warps take its runs of
+// keys in turn and join their parts through shared memory.  Many keys: all units' runs are one line that is cut evenly (SingleLine).
 //
 // Mathematics: s_j = (q . c_j) ks_j, o = sum_j p_j vs_j c'_j / sum_j p_j with the codes c, c' and the rows' scales ks, vs: the
 // scales leave both products, whose operands are then exact in 16 bits: codes of either 8-bit form are halves; a bfloat16 query
@@ -26,7 +27,10 @@
 // one page per run; the weights change lanes in one transposition (movmatrix) per 8 x 8.  Rows are kept permuted (sg_key_at,
 // sg_value_at) so that lanes that read together hit different banks.
 //
-// Bound by memory where there are many keys.
+// Many keys: bound by memory and the issue of instructions together: 4.5 TB/s at 57 % of the issue slots (64 requests of 500 to 1500
+// keys, 32 heads of 64, e4m3: 60 us), 3.2 TB/s where 4 of the 8 columns are used (4 requests of 30000 keys, 4 heads of 128: 38 us),
+// 2.4 TB/s for float queries, whose products are twice as many (28 us).  Few: by the chain of loads to the first keys and the join
+// (one request of 500 keys: 7 us).
 #pragma once
 #include "attention_rows.cuh"
 
@@ -311,7 +315,7 @@ __device__ __forceinline__ uint32_t sg_transpose(uint32_t a) {
 
 // FORM: the cache's; QT: query and output type; D: head size; TWO: weights (and float queries) in two numbers, four heads to a block
 // instead of eight.  Pages hold a multiple of 8 positions.
-// LINE: see SingleLine below.
+// LINE: see SingleLine.
 template <int FORM, typename QT, int D, bool TWO, bool LINE>
 __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS, LINE ? sg_line_blocks(D * c8_bytes(FORM)) : 1) attention_single8_kernel(const SingleArgs a) {
     constexpr bool HALF = FORM != C8_BF16;
@@ -808,14 +812,17 @@ template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a
     return ST_ERR_BAD_SIZE;
 }
 
-// How a call is dealt out as one line, walkers 0 if it is not: it pays (two launches, parts through memory) from four runs a warp on.
+// How a call is dealt out as one line, walkers 0 if it is not.  The line costs a second launch and parts through memory, and pays from
+// two runs a warp on.  Blocks against the line, in us, 32 heads of 64 in int8: 5.4 / 8.9 at 0.4 runs a warp, 9.6 / 11.6 at 1.7,
+// 14.9 / 13.0 at 2.6, 18.3 / 16.1 at 3.5, 26.6 / 24.4 at 10, 63.4 / 61.7 at 41; 4 heads of 128 behind long caches: 18.4 / 16.9
+// at 1.1, 38.3 / 25.8 at 4.5, 57.2 / 35.7 at 9.
 struct LineShape { int walkers, R; long long slots; };
 static inline LineShape sg_line_shape(int n_items, int group, int nkv, int d, int max_keys, long long reach, bool float_q, int form) {
     LineShape s{0, float_q || (form == C8_BF16 && group <= 4) ? 4 : 8, 0};
     const int row = d * c8_bytes(form), kt = sg_run_keys(row), walkers = st_sm_count() * sg_line_blocks(row) * SG_LINE_WARPS;
     const long long parts = (long long)n_items * nkv * ((group + s.R - 1) / s.R), runs = parts * ((max_keys + kt - 1) / kt);
     // (the device counts the line's runs, of up to `reach` keys a token, in 32 bits)
-    if (n_items > SG_LINE_ITEMS || runs < 4ll * walkers || parts * (reach / kt + 2) >= (1 << 30)) return s;
+    if (n_items > SG_LINE_ITEMS || runs < 2ll * walkers || parts * (reach / kt + 2) >= (1 << 30)) return s;
     s.walkers = walkers;
     s.slots = parts + walkers;
     return s;
