@@ -161,3 +161,7 @@ static inline int ar_device() {
 // tiles on the tensor cores (attention_rows_tc.cu): bfloat16 queries, 8-bit and bfloat16 caches, head sizes that are multiples of 16
 // up to 128
 int ar_rows_tc(const RowArgs& a, int form, cudaStream_t s);
+// tiles in float arithmetic, every size (attention_rows_any.cuh)
+int aa_rows_int8(const RowArgs& a, bool float_q, int max_rows, cudaStream_t s);
+int aa_rows_e4m3(const RowArgs& a, bool float_q, int max_rows, cudaStream_t s);
+int aa_rows_wide(const RowArgs& a, bool float_q, int max_rows, cudaStream_t s);

@@ -30,7 +30,7 @@
 // Many keys: bound by memory and the issue of instructions together: 4.5 TB/s at 57 % of the issue slots (64 requests of 500 to 1500
 // keys, 32 heads of 64, e4m3: 60 us), 3.2 TB/s where 4 of the 8 columns are used (4 requests of 30000 keys, 4 heads of 128: 38 us),
 // 2.4 TB/s for float queries, whose products are twice as many (28 us).  Few: by the chain of loads to the first keys and the join
-// (one request of 500 keys: 7 us).
+// (one request of 1000 keys: 7 us).
 #pragma once
 #include "attention_rows.cuh"
 
@@ -831,3 +831,7 @@ static inline LineShape sg_line_shape(int n_items, int group, int nkv, int d, in
 int sg_int8(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);
 int sg_e4m3(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);
 int sg_bf16(const SingleArgs& a, int max_keys, cudaStream_t s);
+// the kernels in float arithmetic, for every size (attention_rows_any.cuh)
+int aa_single_int8(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);
+int aa_single_e4m3(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);
+int aa_single_wide(const SingleArgs& a, bool float_q, int max_keys, cudaStream_t s);

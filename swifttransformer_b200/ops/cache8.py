@@ -9,6 +9,9 @@ keeps its cache in the type of its activations (src/csrc/kernel/kvcache_mgmt.cu:
 Against bfloat16 a cache takes 0.53 (head size 64) or 0.52 (128) of the memory, and a decode step reads that much less.  int8
 stores a row's elements to 1 / 254 of its largest, e4m3 every element to 1 / 16 of itself.
 
+The attention multiplies codes in half precision with weights p_j vs_j in half precision (float queries: both in two halves): exact
+codes, weights to 2^-11 (2^-22), as long as the value scales of a row's keys lie within 2^20 of one another; smaller ones lose bits.
+
 All functions take the index tensors of the other paged operations: ``positions`` and ``seq_of_token`` per token, ``slots`` per
 request, ``block_table`` [slots, pages], int32 on the device.  A token whose position is negative is padding and left out.
 ``status`` (int32, by default a word that ``ops.kernel_status`` reads) is set to 1 when a key that a query needs has no page; such
@@ -103,7 +106,8 @@ def qkv_to_cache8(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: Option
     """q_out = q + bias; the rows k + bias and v + bias (float32 sums) quantised into an 8-bit cache at each token's position.
 
     ``qkv`` [tokens, (nh + 2 nkv) d] float32 or bfloat16; ``bias`` float32 or None; ``q_out`` [tokens, nh d] of qkv's type, or None: the
-    queries stay where they are.  ``write_kv`` False: only the queries move.  Head sizes up to 256."""
+    queries stay where they are.  ``write_kv`` False: only the queries move.  Head sizes up to 256.  No two tokens of a call have
+    the same request and position."""
     what = "qkv_to_cache8"
     _same_device(what, qkv, bias, q_out, pool, scales, positions, seq_of_token, slots, block_table, status)
     act, cols = _ACTS.get(qkv.dtype), (nh + 2 * nkv) * d
