@@ -247,6 +247,46 @@ def test_a_pool_of_more_than_four_gigabytes(form, act):
     assert int(changed) <= step.n * 2 * 8 and int(step.status) == 0
 
 
+@pytest.mark.parametrize("form,act", [("int8", "bf16"), ("e4m3", "f32")])
+def test_captured_steps_on_two_streams_at_once(form, act):
+    """Single tokens as one line, and portions, recorded in two graphs that replay beside one another; a third graph on the first one's
+    stream, and eager calls between: the bits of calls made one by one."""
+    steps = [Step([(0, 30), (900 + 100 * i, 3), (250, 140)], 4, 2, 64, form, act, 16, seed=i, table_wide=4000) for i in range(3)]
+    streams, graphs, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [], []
+
+    def both(step):
+        return torch.stack([single(step), portion(step)])
+
+    for step in steps:
+        both(step)
+    from swifttransformer_b200 import ops
+    plans = [ops.portion_plan([n for _, n in s.requests], [b for b, _ in s.requests], 4, 2, 0, "cuda") for s in steps]
+    torch.cuda.synchronize()
+    for i, s in enumerate(steps):
+        out, g = [s.out(), s.out()], torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i % 2]):
+            ops.attention_cache8_single(s.q, s.pool, s.scales, s.layer, out[0], None, s.n, s.positions, s.seq, s.slots, s.table, 4, s.scale,
+                                        status=s.status)
+            ops.attention_cache8_tiles(s.q, s.pool, s.scales, s.layer, out[1], plans[i], s.positions, s.slots, s.table, 4, s.scale,
+                                       status=s.status)
+        graphs.append(g)
+        outs.append(out)
+    for turn in range(4):
+        for i, s in enumerate(steps):
+            s.q.copy_(torch.randn(s.q.shape, generator=torch.Generator(device="cuda").manual_seed(10 * turn + i), device="cuda"))
+            s.positions[-1] = 389 - 30 * turn
+        torch.cuda.synchronize()
+        for i in (0, 1, 2, 0, 1):
+            with torch.cuda.stream(streams[i % 2]):
+                graphs[i].replay()
+        between = both(steps[1])
+        torch.cuda.synchronize()
+        for i, s in enumerate(steps):
+            want = both(s)
+            assert torch.equal(torch.stack(outs[i]), want), (turn, i)
+        assert torch.equal(between, both(steps[1]))
+
+
 def test_listed_tokens_only():
     step = Step([(40, 3), (0, 2), (9, 1)], 4, 4, 64, "int8", "bf16", 16, seed=5)
     got = single(step, items=ints([4, -1, 2, 0]), n_items=4)
