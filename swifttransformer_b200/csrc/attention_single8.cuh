@@ -28,8 +28,8 @@
 // sg_value_at) so that lanes that read together hit different banks.
 //
 // Many keys: bound by memory and the issue of instructions together: 4.5 TB/s at 57 % of the issue slots (64 requests of 500 to 1500
-// keys, 32 heads of 64, e4m3: 60 us), 3.2 TB/s where 4 of the 8 columns are used (4 requests of 30000 keys, 4 heads of 128: 38 us),
-// 2.4 TB/s for float queries, whose products are twice as many (28 us).  Few: by the chain of loads to the first keys and the join
+// keys, 32 heads of 64, e4m3: 60 us), 3.4 TB/s where 4 of the 8 columns are used (4 requests of 30000 keys, 4 heads of 128: 35 us),
+// 2.4 TB/s for float queries, whose products are twice as many (27 us).  Few: by the chain of loads to the first keys and the join
 // (one request of 1000 keys: 7 us).
 #pragma once
 #include "attention_rows.cuh"
@@ -41,7 +41,7 @@
 __host__ __device__ constexpr int sg_run_keys(int row) { return row <= 128 ? 32 : 16; }
 __host__ __device__ constexpr int sg_stages(int row) { return row <= 80 ? 3 : 2; }
 __host__ __device__ constexpr int sg_line_blocks(int row) { return row <= 64 ? 4 : 3; }
-#define SG_JOIN 256                  // the most threads that join a row's parts
+#define SG_JOIN 512                  // the most threads that join a row's parts
 
 // what the finished row goes through, for all kernels of single tokens
 struct SingleArgs {
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(SG_JOIN) attention_single8_join_kernel(const S
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (mine < groups) {
-#pragma unroll 4
+#pragma unroll 8
         for (int p = mine; p < n; p += groups) {
             const RowParts& from = p < n_own ? a.line : a.parts;
             const size_t at = p < n_own ? (size_t)(unit + c0 + p) * R + r : shared_row + (size_t)(p - n_own) * AR_ROWS;
@@ -790,7 +790,7 @@ static int sg_run(SingleArgs a, int max_keys, cudaStream_t s) {
         AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, true>), smem);
         const int rc = sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, true>, a, dim3(a.walkers / SG_LINE_WARPS), SG_LINE_WARPS, smem, s);
         if (rc) return rc;
-        // few units have many parts each (150 for four long caches: 16 us with 128 threads, 3 with 256), many units two or three
+        // few units have many parts each (110 for four long caches: 35.4 us in all with 512 threads, 36.9 with 256), many units two or three
         const int units = a.n_items * grid_y;
         return st_launch_pdl("single8_join", attention_single8_join_kernel<QT, KT>, dim3(units, a.group < R ? a.group : R),
                              dim3(units < a.walkers / 8 ? SG_JOIN : 64), 0, s, a, R);
