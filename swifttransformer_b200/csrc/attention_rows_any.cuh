@@ -325,12 +325,13 @@ template <int FORM, typename QT>
 __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleArgs a) {
     extern __shared__ __align__(128) float smem[];
     const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, head = blockIdx.y, key_head = head / a.group, d = a.d;
-    const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
+    const int token = a.items ? a.items[item] : item, pos = token >= 0 ? __ldg(a.positions + token) : -1;
+    const int seq = token >= 0 ? __ldg(a.seq_of_token + token) : 0;
     if (pos < 0) {
         if (a.info) ST_PDL_WAIT();
         return;
     }
-    const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
+    const int* bt = a.kv.table + (size_t)__ldg(a.slots + seq) * a.kv.max_pages;
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     if (a.info) lo = max(lo, a.info[3 * item]);
     const int last = min(pos, a.kv.reach - 1);                      // what lies past the table has no page

@@ -362,12 +362,13 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
     }
     const int key_head = part / a.row_blocks, head0 = key_head * a.group + (part % a.row_blocks) * R;
     const int rows = min(R, (key_head + 1) * a.group - head0);
-    const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
+    const int token = a.items ? a.items[item] : item, pos = token >= 0 ? __ldg(a.positions + token) : -1;
+    const int seq = token >= 0 ? __ldg(a.seq_of_token + token) : 0;
     if (!LINE && pos < 0) {                                      // (the same for all blocks of a cluster)
         if (a.info) ST_PDL_WAIT();                               // this kernel never ends before the one it was let in by
         return;
     }
-    const int* bt = a.kv.table + (size_t)a.slots[a.seq_of_token[token]] * a.kv.max_pages;
+    const int* bt = a.kv.table + (size_t)__ldg(a.slots + seq) * a.kv.max_pages;
     int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     if (a.info) lo = max(lo, a.info[3 * item]);
     const int hi = min(pos, a.kv.reach - 1) + 1;

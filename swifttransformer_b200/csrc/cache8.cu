@@ -4,8 +4,9 @@
 //
 // A row of head_dim elements is held by a group of 1 to 32 lanes, eight elements each, from the load to the store: the bias sum,
 // the largest magnitude (butterflies inside the group), the codes.  So a row is read once and written once, which is the floor;
-// a decode step's write is bound by the launch and the chain position -> request -> slot -> page, which runs beside the loads,
-// a prompt's by that chain, by its arithmetic (150 instructions for eight elements of a warp) and by memory about alike.
+// a decode step's write is bound by the launch and the chain position, request -> slot -> page, which runs beside the loads (8 tokens
+// with their rows read back: 5.5 us), a prompt's by the loads that its blocks have under way (2000 tokens of 32 heads of 128: 26 us,
+// 3.1 TB/s; fewer instructions, of 150 for eight elements of a warp, and a shorter chain changed nothing).
 //
 // Rounding: t = x * (1 / scale) is off by less than 2^-22 of itself.  Where no t of a thread's eight is that near the middle between two
 // codes, their roundings are those of the exact quotients; otherwise (one time in two thousand) the quotients are formed in 64
@@ -138,7 +139,7 @@ __device__ __forceinline__ void c8_store8(bf16* p, const float* f) {
 template <typename T, int FORM, int G, int TURN, bool FULL>
 __global__ void __launch_bounds__(C8_THREADS, 6) cache8_write_kernel(const Cache8Write a) {
     const int t = blockIdx.x;
-    const int pos = a.positions[t];
+    const int pos = __ldg(a.positions + t), seq = __ldg(a.seq_of_token + t);       // (a padding token's request may be any number)
     constexpr int PER = C8_THREADS / G;                  // rows of a turn
     const int nkv = a.kv.nkv, d = FULL ? 8 * G : a.d, rows = a.nh + 2 * nkv;       // FULL: every lane of a group has eight elements
     const int lane = threadIdx.x % G, e = 8 * lane;
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(C8_THREADS, 6) cache8_write_kernel(const Cache
     int page = -1;
     uint32_t row0 = 0;                                   // of key head 0; a page holds all heads' keys, then all heads' values
     if (a.write_kv && pos >= 0) {        // pos < 0: a padding token, nothing is cached
-        page = a.kv.page(a.kv.table + (size_t)a.slots[a.seq_of_token[t]] * a.kv.max_pages, pos);
+        page = a.kv.page(a.kv.table + (size_t)__ldg(a.slots + seq) * a.kv.max_pages, pos);
         row0 = a.kv.row0(page, 0, 0) + a.kv.offset(pos, a.kv.page_index(pos));
         if (page < 0 && threadIdx.x == 0) atomicExch(a.kv.status, 1);
     }
@@ -308,9 +309,9 @@ template <typename T, int FORM, int W>
 __global__ void __launch_bounds__(C8_THREADS)
 cache8_rows_kernel(const PagedKV kv, T* __restrict__ out, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
                    const int* __restrict__ slots, int d) {
-    const int t = blockIdx.x, pos = positions[t];
+    const int t = blockIdx.x, pos = __ldg(positions + t), seq = __ldg(seq_of_token + t);
     if (pos < 0) return;
-    const int page = kv.page(kv.table + (size_t)slots[seq_of_token[t]] * kv.max_pages, pos);
+    const int page = kv.page(kv.table + (size_t)__ldg(slots + seq) * kv.max_pages, pos);
     const uint32_t row0 = page >= 0 ? kv.row0(page, 0, 0) + kv.offset(pos, kv.page_index(pos)) : 0u;    // all heads' keys, then all values
     if (page < 0 && threadIdx.x == 0 && kv.status) atomicExch(kv.status, 1);
     const int per = d / W, total = 2 * kv.nkv * per;
