@@ -172,6 +172,11 @@ static RowArgs ar_row_args(const RowCall& c) {
 ST_EXPORT int st_attention_rows_per_tile() { return AR_ROWS; }
 ST_EXPORT int st_attention_rows_chunk() { return AR_CHUNK; }
 ST_EXPORT int st_attention_rows_unit() { return AR_UNIT; }
+// the keys that a single token reads itself, as lo | hi << 32
+ST_EXPORT long long st_attention_single8_span(int pos, int window, int shared, int reach) {
+    const SingleSpan k = sg_span(pos, window, shared, reach);
+    return k.lo | (long long)k.hi << 32;
+}
 // floats of scratch that single tokens want for this call (0: none), laid out at `from`
 static long long ar_line(const RowCall& c, SingleArgs* a, float* from) {
     if (c.nkv <= 0 || c.d <= 0 || !ar_single_fast(c.page_size, c.d, c.form)) return 0;

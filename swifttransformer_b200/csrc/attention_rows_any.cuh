@@ -332,9 +332,8 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
         return;
     }
     const int* bt = a.kv.table + (size_t)__ldg(a.slots + seq) * a.kv.max_pages;
-    int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (a.info) lo = max(lo, a.info[3 * item]);
-    const int last = min(pos, a.kv.reach - 1);                      // what lies past the table has no page
+    const SingleSpan span = sg_span(a, item, pos);
+    const int lo = span.lo, last = span.hi - 1;
     if (last < pos && a.kv.status) *a.kv.status = 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const uint32_t to_values = (uint32_t)a.kv.nkv * a.kv.page_size;

@@ -65,6 +65,16 @@ struct SingleArgs {
     int walkers;                 // 0: no line
 };
 
+// The keys [lo, hi) that a token reads itself: those of its window behind the `shared` ones, as far as the table reaches (what lies past it
+// has no page).  lo <= hi <= reach also where there are none, as for a window that lies wholly past the table: warps form the
+// keys of their first runs before they know that there are none, and these stay in an int (c8_reach).
+struct SingleSpan { int lo, hi; };
+__host__ __device__ inline SingleSpan sg_span(int pos, int window, int shared, int reach) {
+    const int hi = (pos < reach - 1 ? pos : reach - 1) + 1, first = window > 0 && pos >= window ? pos - window + 1 : 0;
+    const int lo = first > shared ? first : shared;
+    return SingleSpan{lo < hi ? lo : hi, hi};
+}
+
 __device__ __forceinline__ void sg_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -211,11 +221,12 @@ template <bool LINE> struct SingleLine {
     int length, total, run;
     int before[LINE ? SG_LINE_ITEMS + 1 : 1];
 };
+__device__ __forceinline__ SingleSpan sg_span(const SingleArgs& a, int item, int pos) {
+    return sg_span(pos, a.window, a.info ? a.info[3 * item] : 0, a.kv.reach);
+}
 template <int KT> __device__ __forceinline__ int sg_runs(const SingleArgs& a, int item, int pos) {     // of a token's own keys
-    int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (a.info) lo = max(lo, a.info[3 * item]);
-    const int hi = min(pos, a.kv.reach - 1) + 1;                 // what lies past the table has no page
-    return hi > lo ? (hi - (lo & ~7) + KT - 1) / KT : 0;
+    const SingleSpan k = sg_span(a, item, pos);
+    return k.hi > k.lo ? (k.hi - (k.lo & ~7) + KT - 1) / KT : 0;
 }
 template <int KT> __device__ __forceinline__ void sg_line_begin(const SingleArgs& a, SingleLine<true>& s) {
     for (int i = threadIdx.x; i < a.n_items; i += blockDim.x) {
@@ -369,9 +380,8 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
         return;
     }
     const int* bt = a.kv.table + (size_t)__ldg(a.slots + seq) * a.kv.max_pages;
-    int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (a.info) lo = max(lo, a.info[3 * item]);
-    const int hi = min(pos, a.kv.reach - 1) + 1;
+    const SingleSpan span = sg_span(a, item, pos);
+    const int lo = span.lo, hi = span.hi;
     if (!LINE && pos >= a.kv.reach && a.kv.status) *a.kv.status = 1;
     const int i0 = i;
     // offset of this lane's word w in a key row: pieces of 16 bytes per lane while the row lasts, then 8, then 4
