@@ -62,16 +62,60 @@ __device__ __forceinline__ int ar_chunks(const RowTile& t) {
 }
 __device__ __forceinline__ int ar_places(int chunks) { return chunks > 0 ? chunks + AR_UNIT : 0; }      // of a unit in the line
 
-// The request whose block table a tile's keys are found by: that of its tokens, or of its first item that is not padding (whose request
-// may be any number); -1: all are padding, no key is read.
-__device__ __forceinline__ int ar_request(const RowArgs& a, const RowTile& t) {
-    if (t.seq >= 0) return t.seq;
-    for (int i = 0; i < t.n_tok; ++i) {
-        const int token = __ldg(a.plan.items + t.first + i);
-        const int pos = __ldg(a.positions + token);
-        if (pos >= 0) return __ldg(a.seq_of_token + token);
+// Token i of a tile, and its position (-1: padding, whose request may be any number).
+struct RowMember { int token, pos; };
+__device__ __forceinline__ RowMember ar_member(const RowArgs& a, const RowTile& t, int i) {
+    RowMember m{-1, -1};
+    if (i < t.n_tok) {
+        m.token = a.plan.items ? __ldg(a.plan.items + t.first + i) : t.first + i;
+        m.pos = __ldg(a.positions + m.token);
     }
-    return -1;
+    return m;
+}
+__device__ __forceinline__ int ar_low(const RowArgs& a, int pos) { return a.window > 0 ? pos - a.window + 1 : 0; }   // the first key seen from pos
+
+// The block table's row by which keys lo .. hi of a tile are found: its request's for all keys; of a tile of shared keys that of the first
+// member that is not padding, for the keys that this one sees.  Of other keys it may have none, be it that it stands before them or
+// that its window has left them behind: these belong to the first member that sees them (ar_first), and to nobody if none does.
+struct RowTable { const int* row; int lo, hi; };
+__device__ __forceinline__ const int* ar_row(const RowArgs& a, int seq) { return a.kv.table + (size_t)__ldg(a.slots + seq) * a.kv.max_pages; }
+template <bool SHARED> __device__ __forceinline__ RowTable ar_table(const RowArgs& a, const RowTile& t) {        // by a whole warp
+    if (!SHARED) return RowTable{ar_row(a, t.seq), 0, 0x7fffffff};
+    for (int i = 0; i < t.n_tok; i += 32) {
+        const RowMember m = ar_member(a, t, i + (threadIdx.x & 31));
+        const int seq = m.token >= 0 ? __ldg(a.seq_of_token + m.token) : 0;      // beside the positions, though one member's is used
+        const uint32_t live = __ballot_sync(0xffffffffu, m.pos >= 0);
+        if (!live) continue;
+        const int src = __ffs(live) - 1, pos = __shfl_sync(0xffffffffu, m.pos, src);
+        return RowTable{ar_row(a, __shfl_sync(0xffffffffu, seq, src)), ar_low(a, pos), pos};
+    }
+    return RowTable{nullptr, 1, 0};
+}
+// The first token of a tile that sees `key`, or -1: by a whole warp, a key per lane that asks.
+__device__ __forceinline__ int ar_first(const RowArgs& a, const RowTile& t, int key, bool asks) {
+    int found = -1;
+    for (int i = 0; i < t.n_tok && __any_sync(0xffffffffu, asks && found < 0); i += 32) {
+        const RowMember m = ar_member(a, t, i + (threadIdx.x & 31));
+        const int n = min(32, t.n_tok - i);
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+            const int token = __shfl_sync(0xffffffffu, m.token, j), pos = __shfl_sync(0xffffffffu, m.pos, j);
+            if (asks && found < 0 && key <= pos && key >= ar_low(a, pos)) found = token;
+        }
+    }
+    return found;
+}
+// The block table's row by which a lane's key is found; null: the key is not asked for.  By a whole warp.
+template <bool SHARED>
+__device__ __forceinline__ const int* ar_row_of(const RowArgs& a, const RowTile& t, const RowTable& table, int key, bool in_tile) {
+    if (!SHARED) return in_tile ? table.row : nullptr;
+    const bool there = in_tile && key >= table.lo && key <= table.hi, other = in_tile && !there;
+    const int* row = there ? table.row : nullptr;
+    if (__any_sync(0xffffffffu, other)) {
+        const int token = ar_first(a, t, key, other);
+        if (token >= 0) row = ar_row(a, __ldg(a.seq_of_token + token));
+    }
+    return row;
 }
 
 // A walker's way along its run: pieces of one (tile, key head) pair.  A walker behind the line's end has none.

@@ -100,8 +100,7 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
             }
             store4(sq + r * ld + e, x);
         }
-        const int seq = ar_request(a, pc.t);
-        const int* bt = seq >= 0 ? a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages : nullptr;
+        const RowTable table = pc.t.seq < 0 ? ar_table<true>(a, pc.t) : ar_table<false>(a, pc.t);
         float ref = -INFINITY, sum = 0.f;                           // of row tid / TPR
         float2 acc[RPT][DT][2];
 #pragma unroll
@@ -114,9 +113,11 @@ __global__ void __launch_bounds__(AA_THREADS) attention_rows_any_kernel(const Ro
         int page = -1;
         bool wanted = false;
         auto ask = [&](int k0) {
+            if (tid >= KEYS) return;                                // (whole warps)
             const int key = k0 + tid, index = a.kv.page_index(key);
-            wanted = tid < KEYS && bt && key >= pc.t.key_lo && key < k_end;
-            page = wanted && index < a.kv.max_pages ? __ldg(bt + index) : -1;
+            const int* const from = ar_row_of<true>(a, pc.t, table, key, key >= pc.t.key_lo && key < k_end);
+            wanted = from != nullptr;
+            page = wanted && index < a.kv.max_pages ? __ldg(from + index) : -1;
         };
         uint32_t row_of = 0xffffffffu;
         float ks_of = 1.f, vs_of = 1.f;

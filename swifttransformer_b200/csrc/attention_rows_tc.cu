@@ -96,7 +96,8 @@ struct RtMeta {
     uint32_t seen[RT_META][2];           // bit c: key c of that half is one of the tile's and has a page
 };
 
-template <int FORM, int DP>
+// SHARED: tiles of single tokens over the keys that their requests share; else of neighbouring tokens of one request.
+template <int FORM, int DP, bool SHARED>
 __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const RowArgs a) {
     constexpr bool HALF = FORM != C8_BF16;
     constexpr int DB = DP / 64;                                        // blocks of 64 dimensions
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         uint32_t n = 0;                  // tiles so far
         RtKeys keys;
         keys.n = 0;
-        const int* bt = nullptr;
+        RowTable table{nullptr, 1, 0};
         int i = 0;                       // the next tile of the piece
         bool have = true;
         // A lane looks up the page of its row two tiles ahead (ask), turns it into a row of the pool one tile ahead (resolve).
@@ -230,18 +231,18 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             if (i >= keys.n) {
                 if (!walk.next(a.plan, pc)) { have = false; return; }
                 keys = rt_keys(pc);
-                const int seq = ar_request(a, pc.t);
-                bt = seq >= 0 ? a.kv.table + (size_t)a.slots[seq] * a.kv.max_pages : nullptr;
+                table = ar_table<SHARED>(a, pc.t);
                 head = pc.head;
                 i = 0;
             }
             const int key = keys.k0 + TC_BN * i + row;
             ++i;
-            if (bt && key >= pc.t.key_lo && key < keys.k_end) {
+            const int* const from = ar_row_of<SHARED>(a, pc.t, table, key, key >= pc.t.key_lo && key < keys.k_end);
+            if (from) {
                 const int index = a.kv.page_index(key);
                 wanted = true;
                 off = a.kv.offset(key, index);
-                page = index < a.kv.max_pages ? __ldg(bt + index) : -1;
+                page = index < a.kv.max_pages ? __ldg(from + index) : -1;
             }
         };
         uint32_t at = NONE;              // the lane's row among the keys
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
         auto look = [&]() -> bool {
             if (!walk.next(a.plan, nx)) return false;
             const int place = nx.t.first + row / g;
-            token_n = row < nx.t.n_tok * g ? (a.plan.items ? __ldg(a.plan.items + place) : place) : -1;
+            token_n = row < nx.t.n_tok * g ? (SHARED ? __ldg(a.plan.items + place) : place) : -1;
             pos_n = token_n >= 0 ? __ldg(a.positions + token_n) : -1;
             if (token_n >= 0) {                          // the row's lines, for `bring`
                 const bf16* q = (const bf16*)a.q + (size_t)token_n * a.q_stride + (nx.head * g + row % g) * d;
@@ -628,9 +629,9 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
 
-template <int FORM, int DP> static int rt_run(const RowArgs& a, cudaStream_t s) {
+template <int FORM, int DP, bool SHARED> static int rt_run(const RowArgs& a, cudaStream_t s) {
     constexpr size_t smem = 2 * (DP / 64) * TC_BM * 128 + 8 * (DP / 64) * TC_BN * 128 + 8 * RT_STAGE + 1024;
-    auto kernel = attention_rows_tc_kernel<FORM, DP>;
+    auto kernel = attention_rows_tc_kernel<FORM, DP, SHARED>;
     AR_ALLOW_SMEM(kernel, smem);
     // the redistribution of registers moves what the launch got, and waits for more for ever: only for a kernel compiled as assumed
     static int regs[64] = {0};
@@ -646,8 +647,13 @@ template <int FORM, int DP> static int rt_run(const RowArgs& a, cudaStream_t s) 
     return st_launch_status();
 }
 
+template <int FORM> static int rt_run(const RowArgs& a, cudaStream_t s) {
+    if (a.plan.items) return a.d <= 64 ? rt_run<FORM, 64, true>(a, s) : rt_run<FORM, 128, true>(a, s);
+    if constexpr (FORM != C8_BF16) return a.d <= 64 ? rt_run<FORM, 64, false>(a, s) : rt_run<FORM, 128, false>(a, s);
+    return ST_ERR_BAD_DTYPE;             // portions over bfloat16 caches have kernels of their own
+}
 int ar_rows_tc(const RowArgs& a, int form, cudaStream_t s) {
-    if (form == C8_INT8) return a.d <= 64 ? rt_run<C8_INT8, 64>(a, s) : rt_run<C8_INT8, 128>(a, s);
-    if (form == C8_E4M3) return a.d <= 64 ? rt_run<C8_E4M3, 64>(a, s) : rt_run<C8_E4M3, 128>(a, s);
-    return a.d <= 64 ? rt_run<C8_BF16, 64>(a, s) : rt_run<C8_BF16, 128>(a, s);
+    if (form == C8_INT8) return rt_run<C8_INT8>(a, s);
+    if (form == C8_E4M3) return rt_run<C8_E4M3>(a, s);
+    return rt_run<C8_BF16>(a, s);
 }

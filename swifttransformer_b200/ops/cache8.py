@@ -323,8 +323,9 @@ def attention_shared_prefix(q: torch.Tensor, pool: torch.Tensor, layer: int, out
                             nh: int, scale: float, window: int = 0, scales: Optional[torch.Tensor] = None,
                             status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of single query tokens whose requests share their first keys: the result of ``attention_decode`` for every token of
-    ``plan`` (from ``shared_prefix_plan``), with a group's shared keys and values read once for the group, through the block table of the
-    request of its first token that is not padding.  The cache is of q's type, or an 8-bit one with its ``scales``.
+    ``plan`` (from ``shared_prefix_plan``), with a group's shared keys and values read once for the group: each by the block table of
+    the request of the group's first token that sees it, so that members may stand in any order.  Keys that no member sees, as they lie
+    before all windows or behind all positions, need no page.  The cache is of q's type, or an 8-bit one with its ``scales``.
 
     A token's position may lie anywhere, inside the shared keys too: it sees keys 0 .. its own position (``window`` > 0: the last
     ``window`` of these).  A value that is not finite reaches, in bfloat16 caches, all rows of its group that share it, also those
