@@ -96,11 +96,16 @@ __device__ __forceinline__ int ar_first(const RowArgs& a, const RowTile& t, int 
     int found = -1;
     for (int i = 0; i < t.n_tok && __any_sync(0xffffffffu, asks && found < 0); i += 32) {
         const RowMember m = ar_member(a, t, i + (threadIdx.x & 31));
+        const int low = m.pos >= 0 ? ar_low(a, m.pos) : 0x7fffffff;
+        // most keys that the tile's first member does not see nobody sees: they lie outside of all members' keys
+        const int last = __reduce_max_sync(0xffffffffu, m.pos), first = __reduce_min_sync(0xffffffffu, low);
+        if (!__any_sync(0xffffffffu, asks && found < 0 && key <= last && key >= first)) continue;
         const int n = min(32, t.n_tok - i);
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
             const int token = __shfl_sync(0xffffffffu, m.token, j), pos = __shfl_sync(0xffffffffu, m.pos, j);
-            if (asks && found < 0 && key <= pos && key >= ar_low(a, pos)) found = token;
+            const int least = __shfl_sync(0xffffffffu, low, j);
+            if (asks && found < 0 && key <= pos && key >= least) found = token;
         }
     }
     return found;
