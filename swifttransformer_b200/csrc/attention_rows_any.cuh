@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(128) attention_single_any_kernel(const SingleA
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (lane + 32 * i < d) parts[2 * W + warp * d + lane + 32 * i] = acc[i];
-    sg_finish<QT>(a, parts, W, 1, 1, d, token, item, head, key_head);
+    sg_finish<QT>(a, parts, W, 1, 1, d, token, pos, item, head, key_head);
 }
 
 template <int FORM, typename QT> static int aa_single(SingleArgs a, int max_keys, cudaStream_t s) {

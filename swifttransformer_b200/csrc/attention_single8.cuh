@@ -88,10 +88,11 @@ __device__ __forceinline__ float sg_remote(const float* local, uint32_t rank) { 
 
 // The parts of a token's shared keys: rows row, row + AR_ROWS, ... (n of them) of a.parts, for the key head's first query head.
 struct SharedParts { size_t row; int n; };
-__device__ __forceinline__ SharedParts sg_shared_parts(const SingleArgs& a, int item, int key_head) {
+__device__ __forceinline__ SharedParts sg_shared_parts(const SingleArgs& a, int item, int key_head, int pos) {
     if (!a.info) return SharedParts{0, 0};
     const int tile = a.info[3 * item + 1], place = a.info[3 * item + 2];
     const RowTile t = ar_tile(a.plan, tile);
+    if (a.window > 0 && pos >= 0 && max(0, pos - a.window + 1) < t.key_lo && threadIdx.x == 0) *a.kv.status = 1;   // keys that the plan left out
     const int n = ar_chunks(t);
     if (n == 0) return SharedParts{0, 0};
     int c0, c1;
@@ -102,7 +103,7 @@ __device__ __forceinline__ SharedParts sg_shared_parts(const SingleArgs& a, int 
 // The warps' parts of R rows x D, then the cluster's, then the prefix's, to the output.  smem: W x R x (D + 2) floats: (R, l) of each
 // warp and row, then O.  `rows` of the R are real; head0 is the first one's query head.
 template <typename QT>
-__device__ __forceinline__ void sg_finish(const SingleArgs& a, float* smem, int W, int R, int rows, int D, int token, int item,
+__device__ __forceinline__ void sg_finish(const SingleArgs& a, float* smem, int W, int R, int rows, int D, int token, int pos, int item,
                                           int head0, int key_head) {
     float* ref = smem;
     float* sum = ref + W * R;
@@ -133,7 +134,7 @@ __device__ __forceinline__ void sg_finish(const SingleArgs& a, float* smem, int 
     } else {
         __syncthreads();
     }
-    SharedParts shared = sg_shared_parts(a, item, key_head);
+    SharedParts shared = sg_shared_parts(a, item, key_head, pos);
     if (a.info) ST_PDL_WAIT();                         // the prefix's parts are complete
     QT* out = (QT*)a.out + ((size_t)token * a.nh + head0) * D;
     for (int i = threadIdx.x + rank * blockDim.x; i < rows * D; i += blockDim.x * a.splits) {
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(SG_JOIN) attention_single8_join_kernel(const S
     const int key_head = part / a.row_blocks, head = key_head * a.group + (part % a.row_blocks) * R + r;
     if (head >= (key_head + 1) * a.group) return;                // (row 0 of the unit is there and waits)
     const int token = a.items ? a.items[item] : item, pos = token >= 0 ? a.positions[token] : -1;
-    const SharedParts shared = sg_shared_parts(a, item, key_head);
+    const SharedParts shared = sg_shared_parts(a, item, key_head, pos);
     const size_t shared_row = shared.row + (head - key_head * a.group);
     const bool own = pos >= 0 && sg_runs<KT>(a, item, pos) > 0;
     ST_PDL_WAIT();                                               // by all, so that what follows this kernel follows the one before it too
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(LINE ? 32 * SG_LINE_WARPS : 32 * SG_MAX_WARPS,
             }
     }
     if constexpr (!LINE) {
-        sg_finish<QT>(a, smem, W, R, rows, D, token, item, head0, key_head);
+        sg_finish<QT>(a, smem, W, R, rows, D, token, pos, item, head0, key_head);
         return;
     }
     if (i0 == 0 && lane == 0) {

@@ -210,20 +210,27 @@ def portion_plan(lens: Sequence[int], starts: Sequence[int], nh: int, nkv: int, 
 
 
 def shared_prefix_plan(groups: Sequence[Sequence[int]], shared: Sequence[int], nh: int, nkv: int, device="cuda",
-                       max_own: int = 0) -> RowPlan:
+                       max_own: int = 0, window: int = 0, starts: Optional[Sequence[int]] = None) -> RowPlan:
     """The plan of a step of single tokens: ``groups[i]`` lists the tokens whose requests have their first ``shared[i]`` keys in common
-    (0: none).  ``max_own``: about the most keys a token has behind its shared ones (it decides how the work is spread)."""
+    (0: none).  ``max_own``: about the most keys a token has behind its shared ones (it decides how the work is spread).
+
+    For calls with a window, ``window`` and ``starts`` leave out the shared keys that it hides: no token of ``groups[i]`` stands before
+    position ``starts[i]``, neither now nor when the plan is used again.  A plan without them serves every window, and walks all keys."""
     plan = RowPlan("shared", nh, nkv, device)
     _need(len(groups) == len(shared) and all(s >= 0 for s in shared), "shared_prefix_plan: a shared length per group, none negative")
+    _need(window >= 0 and (starts is not None) == (window > 0), "shared_prefix_plan: a window, not negative, comes with starts")
+    _need(starts is None or (len(starts) == len(groups) and all(s >= 0 for s in starts)),
+          "shared_prefix_plan: a start per group, none negative")
     per, tiles, items, info = plan.tokens_per_tile, [], [], []
-    for tokens, n in zip(groups, shared):
+    for i, (tokens, n) in enumerate(zip(groups, shared)):
+        lo = min(n, max(0, starts[i] - window + 1)) if window else 0
         for off in range(0, len(tokens), per):
             part = [int(t) for t in tokens[off:off + per]]
-            tiles.append((len(items), len(part), -1, 0, int(n)))
+            tiles.append((len(items), len(part), -1, int(lo), int(n)))
             info += [(int(n), len(tiles) - 1, k) for k in range(len(part))]
             items += part
     _need(all(t >= 0 for t in items) and len(set(items)) == len(items), "shared_prefix_plan: every token at most once, none negative")
-    plan.n_tokens, plan.max_own = max(items, default=-1) + 1, int(max_own)
+    plan.n_tokens, plan.max_own, plan.window = max(items, default=-1) + 1, int(max_own), int(window)
     plan._upload(tiles, items, info)
     return plan
 
@@ -328,11 +335,11 @@ def attention_shared_prefix(q: torch.Tensor, pool: torch.Tensor, layer: int, out
     before all windows or behind all positions, need no page.  The cache is of q's type, or an 8-bit one with its ``scales``.
 
     A token's position may lie anywhere, inside the shared keys too: it sees keys 0 .. its own position (``window`` > 0: the last
-    ``window`` of these).  A value that is not finite reaches, in bfloat16 caches, all rows of its group that share it, also those
+    ``window`` of these).  A token that sees keys before those of the plan (its ``starts``) sets the status.  A value that is not finite reaches, in bfloat16 caches, all rows of its group that share it, also those
     whose window or position hides it; in the other forms only rows that see it."""
     what = "attention_shared_prefix"
-    if plan.kind != "shared":
-        raise KernelError(f"{what}: the plan is from shared_prefix_plan")
+    if plan.kind != "shared" or plan.window not in (0, window):
+        raise KernelError(f"{what}: the plan is from shared_prefix_plan, for this window or for any")
     _attend(what, lib().st_attention_shared, q, pool, scales, layer, out, positions, seq_of_token, slots, block_table, nh, scale,
             window, status, only8=False, plan=plan, max_keys=plan.max_own)
     return out

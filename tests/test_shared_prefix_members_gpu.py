@@ -96,3 +96,44 @@ def test_a_prefix_that_nobody_has_reached(form, act, dim):
     step = Step([(40, 1), (60, 1), (7, 1)], 4, 2, dim, form, act, 16, seed=4, shared=[([1, 0], 41), ([1, 2], 8)])
     check(step, shared(step, [[0, 1, 2]], [500]))
     assert int(step.status) == 0
+
+
+def windowed(step, groups, lens, window, starts):
+    from swifttransformer_b200 import ops
+    plan = ops.shared_prefix_plan(groups, lens, step.heads, step.kv, "cuda", 300, window, starts)
+
+    def call():
+        return ops.attention_shared_prefix(step.q, step.pool, step.layer, step.out(), plan, step.positions, step.seq, step.slots, step.table,
+                                           step.heads, step.scale, window, scales=step.scales, status=step.status)
+    return call
+
+
+@pytest.mark.parametrize("form,act", FORMS)
+@pytest.mark.parametrize("window", [1, 20, 100, 400])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (2, 2, 128), (3, 1, 40)])
+def test_plans_for_a_window(form, act, window, heads, kv, dim):
+    """Plans that leave out what their window hides: the same plan again when the tokens have moved on, groups of which nothing shared is
+    seen, and one that shares nothing."""
+    at = [700, 650, 640, 690, 900, 910, 12]
+    step = Step([(p, 1) for p in at], heads, kv, dim, form, act, 16, seed=window, shared=[([0, 1, 2, 3], 640), ([4, 5], 500)])
+    call = windowed(step, [[0, 1, 2, 3], [4, 5], [6]], [640, 500, 0], window, [640, 900, 0])
+    for positions in ([680, 645, 640, 690, 900, 901, 12], at):
+        step.pos_list = list(positions)
+        step.positions.copy_(torch.tensor(positions, dtype=torch.int32))
+        if positions is at:
+            release(step, window)
+        check(step, call(), window=window)
+        assert int(step.status) == 0
+
+
+@pytest.mark.parametrize("form,act", [("bf16", "bf16"), ("int8", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("dim", [64, 40])
+def test_a_token_before_the_plans_start(form, act, dim):
+    step = Step([(700, 1), (640, 1)], 2, 2, dim, form, act, 16, seed=1, shared=[([0, 1], 640)])
+    call = windowed(step, [[0, 1]], [640], 100, [640])
+    check(step, call(), window=100)
+    assert int(step.status) == 0
+    step.positions[1] = 500
+    got = call()
+    check(step, got, window=100, rows=[0])
+    assert int(step.status) == 1
