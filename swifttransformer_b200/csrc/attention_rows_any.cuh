@@ -27,8 +27,10 @@ template <int ROWS> struct AnyShape {
     static constexpr int RG = ROWS / RPT, KG = KEYS / KPT;          // groups of rows, of keys (and of dimensions)
     static_assert(RG * KG == AA_THREADS, "");
 };
-// blocks that share an SM: what their shared memory and the registers of their sums leave room for
-constexpr int aa_blocks(int rows, int dp) { return rows == 16 ? dp <= 64 ? 3 : dp <= 128 ? 2 : 1 : dp <= 64 ? 2 : 1; }
+// Blocks that share an SM: what shared memory and the registers of the sums leave room for.  (With two blocks of 128 rows over 8-bit caches
+// a prompt of 2000 tokens, 32 heads of 64, takes 815 us instead of 993, but one of 300 tokens of 12 heads, which fills no SM twice, 31
+// instead of 26: the registers that two blocks leave are spilled.)
+constexpr int aa_blocks(int form, int rows, int dp) { return rows == 16 ? dp <= 64 ? 3 : dp <= 128 ? 2 : 1 : form == C8_F32 && dp <= 64 ? 2 : 1; }
 __host__ __device__ inline int aa_stride(int d) { return ((d + 3) & ~3) + 4; }
 template <int ROWS> static size_t aa_smem(int d) {
     return (size_t)(ROWS * aa_stride(d) + 2 * AnyShape<ROWS>::KEYS * aa_stride(d) + ROWS * (AnyShape<ROWS>::KEYS + 4)) * 4;
@@ -50,7 +52,7 @@ template <> struct AnyRaw<C8_F32> {
 };
 
 template <int FORM, typename QT, int ROWS, int DP>
-__global__ void __launch_bounds__(AA_THREADS, aa_blocks(ROWS, DP)) attention_rows_any_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(AA_THREADS, aa_blocks(FORM, ROWS, DP)) attention_rows_any_kernel(const RowArgs a) {
     using S = AnyShape<ROWS>;
     constexpr int KEYS = S::KEYS, RPT = S::RPT, KPT = S::KPT, RG = S::RG, KG = S::KG;
     constexpr int DT = (DP + 4 * KG - 1) / (4 * KG);               // pieces of four dimensions per thread
