@@ -110,6 +110,16 @@ __device__ __forceinline__ int ar_first(const RowArgs& a, const RowTile& t, int 
     }
     return found;
 }
+// Whether a token of a tile sees `key`: asked where a key of a portion has no page, which padding behind the portion need not have.
+__device__ __forceinline__ bool ar_needed(const RowArgs& a, const RowTile& t, int key) {
+    bool seen = false;
+#pragma unroll 1
+    for (int i = 0; i < t.n_tok; ++i) {
+        const int pos = __ldg(a.positions + t.first + i);
+        seen |= key <= pos && key >= ar_low(a, pos);
+    }
+    return seen;
+}
 // The block table's row by which a lane's key is found; null: the key is not asked for.  By a whole warp.
 template <bool SHARED>
 __device__ __forceinline__ const int* ar_row_of(const RowArgs& a, const RowTile& t, const RowTable& table, int key, bool in_tile) {

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(AA_THREADS, aa_blocks(FORM, ROWS, DP)) attenti
             ks_of = vs_of = 1.f;
             if (!wanted) return;
             if ((unsigned)page >= (unsigned)a.kv.num_pages) {
-                if (a.kv.status) *a.kv.status = 1;
+                if (pc.t.seq < 0 || ar_needed(a, pc.t, key)) *a.kv.status = 1;
                 return;
             }
             row_of = a.kv.row0(page, 0, pc.head) + a.kv.offset(key, a.kv.page_index(key));

@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             const bool there = (unsigned)page < (unsigned)a.kv.num_pages;
             at = wanted && there ? a.kv.row0(page, 0, head) + off : NONE;
             hole = wanted && !there;
+            if (!SHARED && hole) hole = ar_needed(a, pc.t, keys.k0 + TC_BN * (i - 1) + row);
         };
         // Scales and marks of a tile, into the place of its turn.  RT_META places: the tile four before has been read when this one's key
         // buffer is free, because S of the tile two before was issued after the softmax threads were done with the one before that.

@@ -1,0 +1,24 @@
+"""Tiles of query rows at the edges of what a call may hold."""
+import pytest
+
+from cache8_cases import Step, check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("form,act,dim", [("int8", "bf16", 64), ("e4m3", "bf16", 128), ("int8", "f32", 64), ("e4m3", "f32", 40)])
+@pytest.mark.parametrize("window", [0, 30])
+def test_portions_that_end_in_padding(form, act, dim, window):
+    """Tokens of a portion that are padding need no page, wherever they would stand."""
+    from swifttransformer_b200 import ops
+    step = Step([(20, 90), (0, 70)], 2, 2, dim, form, act, 16, seed=dim)
+    for t in [*range(50, 90), *range(90 + 64, 160)]:
+        step.pos_list[t], step.positions[t] = -1, -1
+    s = step.slots.tolist()
+    step.table[s[0], 70 // 16 + 1:] = -1                           # keys 0 .. 69 are there
+    step.table[s[1], 4:] = -1
+    plan = ops.portion_plan([90, 70], [20, 0], 2, 2, window, "cuda")
+    got = ops.attention_cache8_tiles(step.q, step.pool, step.scales, step.layer, step.out(), plan, step.positions, step.slots, step.table, 2,
+                                     step.scale, window, step.status)
+    check(step, got, window=window)
+    assert int(step.status) == 0
