@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                 if (more) fac_n = bring();
                 continue;
             }
-            const int hi = min(pos + 1, keys.k_end);
+            const int hi = min(pos, keys.k_end - 1) + 1;
             const int lo = max(pc.t.key_lo, a.window > 0 ? pos - a.window + 1 : 0);
             float ref = -INFINITY, sum = 0.f;
             for (int i = 0; i < keys.n; ++i) {

@@ -2,8 +2,20 @@
 import pytest
 
 from cache8_cases import Step, check
+from test_shared_prefix_gpu import FORMS, shared
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("form,act", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 40])
+@pytest.mark.parametrize("far", [2 ** 31 - 1, 2 ** 31 - 2])
+def test_the_last_position_there_is(form, act, dim, far):
+    """A member far past the block table sees the shared keys like the others."""
+    step = Step([(40, 1), (47, 1), (44, 1)], 4, 2, dim, form, act, 16, seed=dim, shared=[([0, 1, 2], 32)])
+    step.positions[1] = far
+    check(step, shared(step, [[0, 1, 2]], [32]))
+    assert int(step.status) == 1
 
 
 @pytest.mark.parametrize("form,act,dim", [("int8", "bf16", 64), ("e4m3", "bf16", 128), ("int8", "f32", 64), ("e4m3", "f32", 40)])
