@@ -243,11 +243,13 @@ __global__ void __launch_bounds__(AA_THREADS, aa_blocks(FORM, ROWS, DP)) attenti
                 const float m = fmaxf(ref, mx), use = m == -INFINITY ? 0.f : m;
                 const float corr = ref == -INFINITY ? 0.f : exp2f(ref - m);
                 float l = 0.f;
+                const bool odd = s_odd != 0;
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     const float p = exp2f(z[j] - use);
                     l += p;
-                    sp[r * LP + sub + TPR * j] = p;
+                    // a weight of zero stands for a key that is hidden, where a value is not finite: one that is seen weighs a little
+                    sp[r * LP + sub + TPR * j] = odd && p == 0.f && z[j] != -INFINITY ? 1e-45f : p;
                 }
                 sum = sum * corr + l;
                 ref = m;
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(AA_THREADS, aa_blocks(FORM, ROWS, DP)) attenti
             __syncthreads();
             // ---- weights times values: rows rg + RG i, dimensions 4 (kg + KG c) .. + 3
             if (rg < rows) {
-                const bool guard = s_odd != 0;                      // a weight of zero must not meet a value that is not finite
+                const bool guard = s_odd != 0;                      // a hidden key's weight must not meet a value that is not finite
 #pragma unroll
                 for (int i = 0; i < RPT; ++i) {
                     const float corr = s_corr[rg + RG * i];
