@@ -13,6 +13,8 @@
 // A part of a row is (R, l, O): p_j = 2^(s_j - R), s in units of log2, l = sum p_j, O = sum p_j v_j, all float; R is a number near
 // the largest s_j (the exact maximum is not needed: only the common factor).  Parts are joined by 2^(R - max R).
 #pragma once
+#include <atomic>
+
 #include "cache8.cuh"
 
 #define AR_ROWS 128
@@ -205,15 +207,16 @@ static inline int ar_device() {
     int dev = 0;
     return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
 }
-// dynamic shared memory above 48 KB is asked for once per kernel and device
-#define AR_ALLOW_SMEM(kernel, bytes)                                                                                     \
+// Dynamic shared memory above 48 KB is asked for once per kernel and device, `most` that any call of the kernel takes: two threads whose first
+// calls meet then set the same number, and neither launches with more than the other has left allowed.
+#define AR_ALLOW_SMEM(kernel, most)                                                                                      \
     do {                                                                                                                 \
-        static size_t allowed[64] = {0};                                                                                 \
-        size_t& have = allowed[ar_device()];                                                                             \
-        if ((size_t)(bytes) > 48 * 1024 && have < (size_t)(bytes)) {                                                     \
-            const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes)); \
+        static std::atomic<bool> allowed[64];                                                                            \
+        std::atomic<bool>& have = allowed[ar_device()];                                                                  \
+        if ((size_t)(most) > 48 * 1024 && !have) {                                                                       \
+            const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(most)); \
             if (err != cudaSuccess) { cudaGetLastError(); return (int)err; }                                             \
-            have = (size_t)(bytes);                                                                                      \
+            have = true;                                                                                                 \
         }                                                                                                                \
     } while (0)
 

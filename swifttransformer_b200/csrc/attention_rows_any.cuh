@@ -423,13 +423,13 @@ template <int FORM, typename QT, int ROWS> static int aa_rows(const RowArgs& a, 
     const size_t smem = aa_smem<ROWS>(a.d);
     const int grid = a.plan.ctas;
     if (a.d <= 64) {
-        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 64>), smem);
+        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 64>), aa_smem<ROWS>(64));
         attention_rows_any_kernel<FORM, QT, ROWS, 64><<<grid, AA_THREADS, smem, s>>>(a);
     } else if (a.d <= 128) {
-        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 128>), smem);
+        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 128>), aa_smem<ROWS>(128));
         attention_rows_any_kernel<FORM, QT, ROWS, 128><<<grid, AA_THREADS, smem, s>>>(a);
     } else {
-        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 256>), smem);
+        AR_ALLOW_SMEM((attention_rows_any_kernel<FORM, QT, ROWS, 256>), aa_smem<ROWS>(256));
         attention_rows_any_kernel<FORM, QT, ROWS, 256><<<grid, AA_THREADS, smem, s>>>(a);
     }
     return st_launch_status();

@@ -635,8 +635,8 @@ template <int FORM, int DP, bool SHARED> static int rt_run(const RowArgs& a, cud
     auto kernel = attention_rows_tc_kernel<FORM, DP, SHARED>;
     AR_ALLOW_SMEM(kernel, smem);
     // the redistribution of registers moves what the launch got, and waits for more for ever: only for a kernel compiled as assumed
-    static int regs[64] = {0};
-    int& have = regs[ar_device()];
+    static std::atomic<int> regs[64];
+    std::atomic<int>& have = regs[ar_device()];
     if (!have) {
         cudaFuncAttributes attr;
         const cudaError_t e = cudaFuncGetAttributes(&attr, kernel);

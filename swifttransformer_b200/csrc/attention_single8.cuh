@@ -41,6 +41,7 @@
 __host__ __device__ constexpr int sg_run_keys(int row) { return row <= 128 ? 32 : 16; }
 __host__ __device__ constexpr int sg_stages(int row) { return row <= 80 ? 3 : 2; }
 __host__ __device__ constexpr int sg_line_blocks(int row) { return row <= 64 ? 4 : 3; }
+#define SG_SMEM (200 * 1024)         // the most shared memory of a block that has one unit; its parts take less than its rings may
 #define SG_JOIN 512                  // the most threads that join a row's parts
 
 // what the finished row goes through, for all kernels of single tokens
@@ -808,10 +809,11 @@ static int sg_run(SingleArgs a, int max_keys, cudaStream_t s) {
                              dim3(units < a.walkers / 8 ? SG_JOIN : 64), 0, s, a, R);
     }
     SingleShape shape = sg_shape((long long)a.n_items * grid_y, max_keys, KT);
-    while (shape.warps * RING > 200 * 1024) shape.warps /= 2;     // a block's shared memory
+    while (shape.warps * RING > SG_SMEM) shape.warps /= 2;
     a.splits = shape.splits;
+    static_assert((size_t)SG_MAX_WARPS * R * (D + 2) * 4 <= SG_SMEM, "");
     const size_t parts = (size_t)shape.warps * R * (D + 2) * 4, rings = shape.warps * RING, smem = parts > rings ? parts : rings;
-    AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, false>), smem);
+    AR_ALLOW_SMEM((attention_single8_kernel<FORM, QT, D, TWO, false>), SG_SMEM);
     return sg_launch("single8", attention_single8_kernel<FORM, QT, D, TWO, false>, a, dim3((unsigned)a.n_items * a.splits, grid_y), shape.warps,
                      smem, s);
 }
