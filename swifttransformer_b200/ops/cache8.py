@@ -36,6 +36,7 @@ _I32 = torch.int32
 ROWS_PER_TILE = 128
 ROWS_CHUNK = 64
 ROWS_UNIT = 3
+MAX_KEYS = 0x7fff0000            # of a request: positions and a few runs of keys behind them stay in an int (c8_reach in csrc/cache8.cuh)
 
 
 def cache8_pool(num_pages: int, n_layers: int, nkv: int, page_size: int, d: int, dtype: torch.dtype, device):
@@ -177,6 +178,7 @@ class RowPlan:
         start = 0
         rows = []
         for first, n, seq, lo, hi in tiles:
+            _need(hi <= MAX_KEYS, f"a plan reaches to at most {MAX_KEYS} keys")
             rows.append((first, n, seq, lo, hi, start))
             chunks = self._chunks(lo, hi)
             start += (chunks + ROWS_UNIT) * self.nkv if chunks else 0
@@ -229,7 +231,8 @@ def shared_prefix_plan(groups: Sequence[Sequence[int]], shared: Sequence[int], n
             tiles.append((len(items), len(part), -1, int(lo), int(n)))
             info += [(int(n), len(tiles) - 1, k) for k in range(len(part))]
             items += part
-    _need(all(t >= 0 for t in items) and len(set(items)) == len(items), "shared_prefix_plan: every token at most once, none negative")
+    _need(all(0 <= t < 1 << 31 for t in items) and len(set(items)) == len(items),
+          "shared_prefix_plan: every token at most once, none negative")
     plan.n_tokens, plan.max_own, plan.window = max(items, default=-1) + 1, int(max_own), int(window)
     plan._upload(tiles, items, info)
     return plan

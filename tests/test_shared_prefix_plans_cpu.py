@@ -31,3 +31,19 @@ def test_calls_refuse_a_plan_for_another_window(fake, window):  # noqa: F811
     plan.tiles = fake(plan.tiles)
     with pytest.raises(KernelError, match="window"):
         ops.attention_shared_prefix(**a, plan=plan)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: ops.shared_prefix_plan([[0]], [2 ** 33], 1, 1, "cpu"), lambda: ops.shared_prefix_plan([[0]], [2 ** 31 - 1], 1, 1, "cpu"),
+    lambda: ops.shared_prefix_plan([[0]], [2 ** 31], 1, 1, "cpu", 0, 10, [2 ** 31]),
+    lambda: ops.shared_prefix_plan([[2 ** 31]], [4], 1, 1, "cpu"), lambda: ops.portion_plan([4], [2 ** 31 - 8], 1, 1, 8, "cpu"),
+    lambda: ops.portion_plan([4], [2 ** 32], 1, 1, 8, "cpu"), lambda: ops.portion_plan([1], [2 ** 31 - 2], 1, 1, device="cpu")])
+def test_plans_refuse_what_passes_an_int(make):
+    with pytest.raises(KernelError):
+        make()
+
+
+def test_the_longest_plans():
+    plan = ops.portion_plan([4], [0x7fff0000 - 4], 1, 1, 8, "cpu")
+    assert plan.tiles.tolist() == [0, 4, 0, 0x7fff0000 - 11, 0x7fff0000, 0] and plan.total == 4
+    assert ops.shared_prefix_plan([[0]], [0x7fff0000], 1, 1, "cpu").total == 0x7fff0000 // 64 + 3
