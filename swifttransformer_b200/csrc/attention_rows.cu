@@ -19,7 +19,6 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs 
     if (c0 < 0 || c0 != (int)blockIdx.x - 1) return;
     const int pieces = (d + 3) / 4, total = pc.t.n_tok * g * pieces, n = c1 - c0 + 1;
     const bool vec = d % 4 == 0, wide = vec && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-    const size_t row0 = (size_t)(pc.unit + c0) * AR_ROWS;
     for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < total; i += gridDim.y * blockDim.x) {
         const int r = i / pieces, e = (i - r * pieces) * 4, place = pc.t.first + r / g, token = p.items ? p.items[place] : place;
         const int pos = a.positions[token];
@@ -29,7 +28,8 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowArgs 
             float ref[2], sum[2], x[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const size_t at = row0 + (size_t)(k + (k + h < n ? h : 0)) * AR_ROWS + r;
+                const int j = k + (k + h < n ? h : 0);              // part 0 ended its walker's run, the others began theirs
+                const size_t at = (size_t)(2 * (c0 + j) + (j == 0)) * AR_ROWS + r;
                 const float* part = a.parts.o + at * d + e;
                 ref[h] = __ldcg(a.parts.r + at);
                 sum[h] = __ldcg(a.parts.l + at);
@@ -108,9 +108,10 @@ static int ar_rows(RowArgs a, int act, int form, int max_rows, cudaStream_t s) {
 }
 
 // The runs a plan's line is cut into: as many as are walked at the same time, two per SM by the tensor-core kernel, one by every
-// block of the float kernel.
+// block of the float kernel.  No kernel has more walkers for a head size than the float kernel.
+static int ar_walkers_most(int d) { return st_sm_count() * (d <= 64 ? 3 : d <= 128 ? 2 : 1); }
 static void ar_deal(RowArgs& a, int act, int form) {
-    const int most = st_sm_count() * (ar_tc(a, act, form) ? 2 : a.d <= 64 ? 3 : a.d <= 128 ? 2 : 1);
+    const int most = ar_tc(a, act, form) ? 2 * st_sm_count() : ar_walkers_most(a.d);
     a.plan.run = a.plan.total > most ? (a.plan.total + most - 1) / most : 1;
     a.plan.ctas = (a.plan.total + a.plan.run - 1) / a.plan.run;
 }
@@ -172,6 +173,12 @@ static RowArgs ar_row_args(const RowCall& c) {
 ST_EXPORT int st_attention_rows_per_tile() { return AR_ROWS; }
 ST_EXPORT int st_attention_rows_chunk() { return AR_CHUNK; }
 ST_EXPORT int st_attention_rows_unit() { return AR_UNIT; }
+// floats of scratch for the parts of a plan's line of `total` places; shared: of its n_tiles x nkv units each
+ST_EXPORT long long st_attention_rows_scratch(int n_tiles, int nkv, int d, int total, int shared) {
+    if (total <= 0 || d <= 0) return 0;
+    const long long walkers = total < ar_walkers_most(d) ? total : ar_walkers_most(d);
+    return (shared ? (long long)n_tiles * nkv + walkers : 2 * walkers) * (long long)ar_part_floats(d);
+}
 // the keys that a single token reads itself, as lo | hi << 32
 ST_EXPORT long long st_attention_single8_span(int pos, int window, int shared, int reach) {
     const SingleSpan k = sg_span(pos, window, shared, reach);
@@ -213,9 +220,8 @@ ST_EXPORT int st_attention_tiles8(const RowCall* c, void* stream) {
     if (c->n_tiles <= 0 || c->total <= 0) return 0;
     if (c->nh / c->nkv > AR_ROWS) return ST_ERR_TOO_LARGE;
     RowArgs a = ar_row_args(*c);
-    const long long slots = (long long)c->n_tiles * c->nkv + a.plan.ctas;
+    const long long slots = 2ll * a.plan.ctas;
     if (c->scratch_floats < slots * (long long)ar_part_floats(c->d)) return ST_ERR_BAD_ARG;
-    if (slots > (1 << 30) / AR_ROWS) return ST_ERR_TOO_LARGE;
     a.parts = ar_parts(c->scratch, slots);
     a.direct = 1;
     const cudaStream_t s = (cudaStream_t)stream;

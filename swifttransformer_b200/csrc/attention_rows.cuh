@@ -7,8 +7,10 @@
 // begin and end cost (without them the walkers of a prompt's first, short units were the last by a factor of two), form one line
 // of `total` places which is cut
 // into runs of `run` places, one per walker (a block, or one of a block's two groups): every walker gets the same work however
-// unequal the tiles are, and a unit that a cut goes through is put together from parts.  Part (unit u, walker c) has slot u + c: a
-// new slot begins with every unit and with every run, so no two parts share one.
+// unequal the tiles are, and a unit that a cut goes through is put together from parts.  Where results leave directly, a walker leaves
+// two parts at most: what it began with, of a unit that a cut in front of it went through, has slot 2 c of walker c, what it ended
+// with, the begin of a unit, slot 2 c + 1.  Of shared keys every piece is a part: that of unit u and walker c has slot u + c (a new slot
+// begins with every unit and with every run, so no two parts share one).
 //
 // A part of a row is (R, l, O): p_j = 2^(s_j - R), s in units of log2, l = sum p_j, O = sum p_j v_j, all float; R is a number near
 // the largest s_j (the exact maximum is not needed: only the common factor).  Parts are joined by 2^(R - max R).
@@ -193,6 +195,10 @@ __device__ __forceinline__ void ar_walkers(const RowPlan& p, const RowTile& t, i
     const int x0 = t.start + head * ar_places(n) + AR_UNIT;
     c0 = x0 / p.run;
     c1 = (x0 + n - 1) / p.run;
+}
+
+__device__ __forceinline__ int ar_slot(const RowArgs& a, const RowPiece& p, int walker) {      // of a piece that is not direct
+    return a.direct ? 2 * walker + (p.chunk0 == 0) : p.unit + walker;
 }
 
 __device__ __forceinline__ float ar_exp2(float x) {      // 2 ulp, exp2(-inf) = 0

@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(AA_THREADS, aa_blocks(FORM, ROWS, DP)) attenti
             if (sub == 0) { s_sum[tid / TPR] = sum; s_sum[ROWS + tid / TPR] = ref; }
             __syncthreads();
             const bool direct = a.direct && pc.whole;
-            const size_t slot = (size_t)(pc.unit + blockIdx.x) * AR_ROWS;
+            const size_t slot = (size_t)ar_slot(a, pc, blockIdx.x) * AR_ROWS;
             if (!direct)
                 for (int r = tid; r < rows; r += AA_THREADS) { a.parts.r[slot + r] = s_sum[ROWS + r]; a.parts.l[slot + r] = s_sum[r]; }
 #pragma unroll

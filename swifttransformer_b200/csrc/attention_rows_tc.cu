@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             // ---- the piece's sums: out, or into its slot.  Sixteen dimensions at a time change hands in shared memory, so that
             // neighbouring lanes store a row's neighbouring pieces (a thread's own row has a line of its own in every store).
             const bool direct = a.direct && pc.whole;
-            const size_t slot0 = ((size_t)(pc.unit + 2 * blockIdx.x + wg)) * AR_ROWS;
+            const size_t slot0 = (size_t)ar_slot(a, pc, 2 * blockIdx.x + wg) * AR_ROWS;
             if (!direct && row < rows) { a.parts.r[slot0 + row] = ref; a.parts.l[slot0 + row] = sum; }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const bool store = row < rows && pos >= 0 && alive;

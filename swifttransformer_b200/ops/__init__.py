@@ -50,6 +50,7 @@ def lib() -> ctypes.CDLL:
         _LIB.st_delta_rule_chunk_floats.restype = ctypes.c_longlong
         _LIB.st_attention_single8_scratch.restype = ctypes.c_longlong
         _LIB.st_attention_single8_span.restype = ctypes.c_longlong
+        _LIB.st_attention_rows_scratch.restype = ctypes.c_longlong
         _LIB.st_uniform_host.restype = ctypes.c_float
         _LIB.st_uniform_host.argtypes = [ctypes.c_longlong, ctypes.c_longlong]
     return _LIB

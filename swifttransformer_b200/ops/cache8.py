@@ -26,7 +26,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
-from . import KernelError, _check, _current_device, _stream, _tc_status_word, lib, sm_count
+from . import KernelError, _check, _current_device, _stream, _tc_status_word, lib
 
 CACHE8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _FORMS = {torch.int8: 0, torch.float8_e4m3fn: 1, torch.bfloat16: 2, torch.float32: 3}
@@ -286,8 +286,8 @@ def _attend(what: str, entry, q, pool, scales, layer, out, positions, seq_of_tok
     window = min(window, 0x7fffffff)
     if 0 < window < max_keys:
         max_keys = window
-    # parts of rows that several blocks leave: a slot per (tile, key head) and one per walker of the line; those of single tokens
-    floats = (n_tiles * nkv + 3 * sm_count(q.device)) * ROWS_PER_TILE * (2 + d) if total else 0
+    # the parts of rows that several blocks leave, and those of single tokens
+    floats = lib().st_attention_rows_scratch(n_tiles, nkv, d, total, 1 if n_items else 0) if total else 0
     if n_items:
         floats += _single_scratch(n_items, nh, nkv, d, page_size, block_table.shape[1], max_keys, act, form)
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
