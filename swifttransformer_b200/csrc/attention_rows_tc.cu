@@ -2,8 +2,10 @@
 // groups of tokens over the prefix they share.
 //
 // Mathematics: as in attention_single8.cuh.  Codes of an 8-bit cache and queries (scaled by a power of two per row) are halves, the rows'
-// scales stay outside: s_j = (q . c_j) ks_j, P_j = p_j vs_j in half; over bfloat16 caches queries, keys, P and values are
-// bfloat16.  S = Q K^T of 128 rows x 64 keys and O += P V are tcgen05 products with their sums in tensor memory; P goes there
+// scales stay outside: s_j = (q . c_j) ks_j, P_j = p_j vs_j in one half (2^-12 of itself at most, beside results of 2^-9: errors of 0.00167 of
+// the norm, of which 0.00165 are the results' rounding); over bfloat16 caches queries, keys and values are bfloat16 and P is two bfloat16
+// numbers, both multiplied (one: 0.0018 to 0.0020 of the norm; 16 members behind 2000 keys took 24.0 us then, 25.0 now, 64 behind 8000,
+// 32 heads of 64, 50.2 and 54.7).  S = Q K^T of 128 rows x 64 keys and O += P V are tcgen05 products with their sums in tensor memory; P goes there
 // straight from the softmax threads' registers (the product's A operand).
 //
 // One block per SM, in it two groups that have nothing to do with one another: each walks its own run of the plan's chunks in tiles of
@@ -13,7 +15,7 @@
 // of a piece is on the tensor cores; its first S then runs under their stores.
 //   8-bit forms: neighbouring lanes read a row in 16-byte loads, a tile ahead of the conversion to halves, which is stored in the 128-byte
 //   swizzled layout that the matrix descriptors expect.  At head size 128 the two halves of every 16 codes go to different blocks of
-//   64 dimensions (rt_dim): neighbouring lanes then store to different banks without sorting; queries are stored alike, results
+//   64 dimensions (rt_place): neighbouring lanes then store to different banks without sorting; queries are stored alike, results
 //   are put in order when they leave.
 //   bfloat16: asynchronous copies into that layout.
 // Page sizes are arbitrary: a lane looks up its row's page two tiles ahead of its loads.
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
     constexpr uint32_t Q_BLK = TC_BM * 128, KV_BLK = TC_BN * 128;      // bytes of a [rows][64] block
     constexpr uint32_t Q_BUF = DB * Q_BLK, BUF = DB * KV_BLK;
     constexpr uint32_t ALL_BYTES = 2 * Q_BUF + 8 * BUF + 8 * RT_STAGE;
-    constexpr int WG_COLS = 256, T_O = 64, T_P = 64 + DP;              // a group's columns: S, O, P
+    constexpr int WG_COLS = 256, T_O = 64, T_P = 64 + DP;              // a group's columns: S, O, P (of bfloat16: its first numbers, its second)
     constexpr uint32_t NONE = 0xffffffffu;
     extern __shared__ unsigned char rt_raw[];
     __shared__ __align__(16) RtMeta s_meta[2];
@@ -198,8 +200,10 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                         tc_fence_after_sync();
                         if (tc_elect()) {
 #pragma unroll
-                            for (int jj = 0; jj < TC_BN / 16; ++jj)
+                            for (int jj = 0; jj < TC_BN / 16; ++jj) {
                                 tc_mma_ts(t_wg + T_O, t_wg + T_P + jj * 8, dv + ((b * BUF + jj * 2048) >> 4), idesc_o, i > 0 || jj > 0);
+                                if (!HALF) tc_mma_ts(t_wg + T_O, t_wg + T_P + TC_BN / 2 + jj * 8, dv + ((b * BUF + jj * 2048) >> 4), idesc_o, 1);
+                            }
                             tc_commit(mb_o);
                             tc_commit(mb_free + 8 * (2 + b));
                         }
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                 if (move) ref = need - 11.f;
                 const float neg = ref == -INFINITY ? 0.f : -ref;
                 float rs[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                uint32_t w[TC_BN / 2];
+                uint32_t w[TC_BN / 2], w2[HALF ? 1 : TC_BN / 2];
 #pragma unroll
                 for (int c = 0; c < TC_BN; c += 4) {
                     float p[4];
@@ -530,9 +534,15 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                         w[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
                         w[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
                     } else {
-                        const __nv_bfloat162 h0 = __floats2bfloat162_rn(p[0], p[1]), h1 = __floats2bfloat162_rn(p[2], p[3]);
-                        w[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-                        w[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                        // p in two numbers: one of 2^-8 would be the largest error of the result
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const __nv_bfloat162 first = __floats2bfloat162_rn(p[2 * h], p[2 * h + 1]);
+                            const uint32_t u = *reinterpret_cast<const uint32_t*>(&first);
+                            const __nv_bfloat162 rest = __floats2bfloat162_rn(p[2 * h] - __uint_as_float(u << 16), p[2 * h + 1] - __uint_as_float(u & 0xffff0000u));
+                            w[c / 2 + h] = u;
+                            w2[c / 2 + h] = *reinterpret_cast<const uint32_t*>(&rest);
+                        }
                     }
                 }
                 if (i > 0) {                             // O += P V of tile i - 1: O may be scaled and P overwritten after it
@@ -554,6 +564,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
                     sum *= corr;
                 }
                 tc_st32(t_wg + T_P, reinterpret_cast<const float*>(w));
+                if constexpr (!HALF) tc_st32(t_wg + T_P + TC_BN / 2, reinterpret_cast<const float*>(w2));
                 sum += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
                 tc_st_wait();
                 tc_fence_before_sync();
