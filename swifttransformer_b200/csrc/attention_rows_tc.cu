@@ -24,8 +24,8 @@
 //
 // Bound by the chain of a tile: about 3500 clocks (head size 64) for each of the two groups, where the exponentials of both take 1024 and
 // the products 512.  Leaving out exponentials, scales or conversions one at a time changed nothing, all of them together a tenth: the waits and
-// hand-overs remain.  2000 tokens of three prompts, 32 heads of 64, int8: 65 us with the join; 1000 tokens behind 1500 keys, 32 heads of
-// 128, e4m3: 94 us.
+// hand-overs remain.  2000 tokens of three prompts, 32 heads of 64, int8: 62.5 us with the join; 1000 tokens behind 1500 keys, 32 heads
+// of 128, e4m3: 95 us.  The bfloat16 prompt kernel takes 36 and 58 us for the like (attention_prefill_tmap.cu: 2450 clocks a tile).
 //
 // Waits are bounded; one that expires marks the block dead, the other waits end, `status` gets 3, tensor memory is freed and the
 // kernel returns.

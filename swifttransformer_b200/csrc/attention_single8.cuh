@@ -829,7 +829,9 @@ template <int FORM, typename QT, bool TWO> static int sg_run(const SingleArgs& a
 // How a call is dealt out as one line, walkers 0 if it is not.  The line costs a second launch and parts through memory, and pays from
 // two runs a warp on.  Blocks against the line, in us, 32 heads of 64 in int8: 5.4 / 8.9 at 0.4 runs a warp, 9.6 / 11.6 at 1.7,
 // 14.9 / 13.0 at 2.6, 18.3 / 16.1 at 3.5, 26.6 / 24.4 at 10, 63.4 / 61.7 at 41; 4 heads of 128 behind long caches: 18.4 / 16.9
-// at 1.1, 38.3 / 25.8 at 4.5, 57.2 / 35.7 at 9.
+// at 1.1, 38.3 / 25.8 at 4.5, 57.2 / 35.7 at 9.  Requests of one length whose blocks fill the device in whole turns lose by it: 32 of 1000
+// keys each (32 heads of 64, int8, 14 runs a warp) 32.6 / 36.4, 64 of them 58.3 / 59.7.  Lengths are in device memory; the host
+// knows about the longest only, and gives this up for 16 of 1000 (25.1 / 24.2), 64 of 250 (28.5 / 25.8) and all unequal ones.
 struct LineShape { int walkers, R; long long slots; };
 static inline LineShape sg_line_shape(int n_items, int group, int nkv, int d, int max_keys, long long reach, bool float_q, int form) {
     LineShape s{0, float_q || (form == C8_BF16 && group <= 4) ? 4 : 8, 0};

@@ -5,8 +5,8 @@
 // A row of head_dim elements is held by a group of 1 to 32 lanes, eight elements each, from the load to the store: the bias sum,
 // the largest magnitude (butterflies inside the group), the codes.  So a row is read once and written once, which is the floor;
 // a decode step's write is bound by the launch and the chain position, request -> slot -> page, which runs beside the loads (8 tokens
-// with their rows read back: 5.5 us), a prompt's by the loads that its blocks have under way (2000 tokens of 32 heads of 128: 26 us,
-// 3.1 TB/s; fewer instructions, of 150 for eight elements of a warp, and a shorter chain changed nothing).
+// with their rows read back: 5.5 us), a prompt's by the loads that its blocks have under way (2000 tokens of 32 heads of 128: 25 us,
+// 3.3 TB/s; fewer instructions, of 150 for eight elements of a warp, and a shorter chain changed nothing).
 //
 // Rounding: t = x * (1 / scale) is off by less than 2^-22 of itself.  Where no t of a thread's eight is that near the middle between two
 // codes, their roundings are those of the exact quotients; otherwise (of eight numbers spread over the codes one time in a thousand

@@ -10,7 +10,8 @@ Against bfloat16 a cache takes 0.53 (head size 64) or 0.52 (128) of the memory, 
 stores a row's elements to 1 / 254 of its largest, e4m3 every element to 1 / 16 of itself.
 
 The attention multiplies codes in half precision with weights p_j vs_j in half precision (float queries: both in two halves): exact
-codes, weights to 2^-11 (2^-22), as long as the value scales of a row's keys lie within 2^20 of one another; smaller ones lose bits.
+codes, weights to 2^-11 (2^-22), as long as the value scales of a row's keys lie within 2^20 of one another; smaller ones lose bits, and from
+2^110 on the softmax's sum does.  Keys of magnitude 2^100 and more may overflow.
 
 All functions take the index tensors of the other paged operations: ``positions`` and ``seq_of_token`` per token, ``slots`` per
 request, ``block_table`` [slots, pages], int32 on the device.  A token whose position is negative is padding and left out.
@@ -196,7 +197,8 @@ class RowPlan:
 
 
 def portion_plan(lens: Sequence[int], starts: Sequence[int], nh: int, nkv: int, window: int = 0, device="cuda") -> RowPlan:
-    """The plan of a step in which request i brings ``lens[i]`` tokens, one behind the other, and has ``starts[i]`` in the cache."""
+    """The plan of a step in which request i brings ``lens[i]`` tokens, one behind the other, and has ``starts[i]`` in the cache.  In a call
+    token j of request i stands at ``starts[i] + j`` or is padding.  Making a plan waits for the current stream."""
     plan = RowPlan("portion", nh, nkv, device)
     _need(len(lens) == len(starts) and all(n >= 0 for n in lens) and all(s >= 0 for s in starts) and window >= 0,
           "portion_plan: a length and a start per request, none negative")
@@ -217,7 +219,10 @@ def shared_prefix_plan(groups: Sequence[Sequence[int]], shared: Sequence[int], n
     (0: none).  ``max_own``: about the most keys a token has behind its shared ones (it decides how the work is spread).
 
     For calls with a window, ``window`` and ``starts`` leave out the shared keys that it hides: no token of ``groups[i]`` stands before
-    position ``starts[i]``, neither now nor when the plan is used again.  A plan without them serves every window, and walks all keys."""
+    position ``starts[i]``, neither now nor when the plan is used again.  A plan without them serves every window, and walks all keys.
+
+    Sharing pays from about 16 thousand members x shared keys on (at 32 key heads of 64; 8 thousand at 32 of 128), as 16 requests behind
+    1000 tokens; below, the single-token attention over the same pages is faster.  Making a plan waits for the current stream."""
     plan = RowPlan("shared", nh, nkv, device)
     _need(len(groups) == len(shared) and all(s >= 0 for s in shared), "shared_prefix_plan: a shared length per group, none negative")
     _need(window >= 0 and (starts is not None) == (window > 0), "shared_prefix_plan: a window, not negative, comes with starts")
