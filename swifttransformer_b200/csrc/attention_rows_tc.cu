@@ -72,13 +72,6 @@ __device__ __forceinline__ uint32_t rt_bits(int lo, int hi) {
     return lo <= 0 ? below : lo >= 32 ? 0u : below & (0xffffffffu << lo);
 }
 
-__device__ __forceinline__ void rt_ld16(uint32_t taddr, float* v) {
-    uint32_t* r = reinterpret_cast<uint32_t*>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
-}
-
 // the keys of a piece: tiles of 64 from k0 on, below k_end
 struct RtKeys { int k0, k_end, n; };
 __device__ __forceinline__ RtKeys rt_keys(const RowPiece& p) {
@@ -593,7 +586,7 @@ __global__ void __launch_bounds__(RT_THREADS, 1) attention_rows_tc_kernel(const 
             for (int cb = 0; cb < DP / 16; ++cb) {
                 float o[16];
                 __syncwarp();
-                rt_ld16(t_wg + T_O + cb * 16, o);
+                tc_ld16(t_wg + T_O + cb * 16, o);
                 tc_ld_wait();
                 // row `lane`: four pieces of 16 bytes, turned by the row so that eight lanes hit all banks
 #pragma unroll
